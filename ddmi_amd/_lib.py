@@ -67,6 +67,14 @@ class StepCoefs(C.Structure):
                                          "noise_scale", "sqrt_ac_next", "c_dir", "sigma")]
 
 
+DTYPE_F32, DTYPE_BF16 = 0, 1
+
+
+class LossIn(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("model_out", "ref_out", "x_t", "second", "sqrt_1mac", "mixing_logit", "ref_mixing_logit", "weight")] + \
+        [("HW", C.c_int64), ("C", C.c_int), ("out_dtype", C.c_int)]
+
+
 # every symbol include/ddmi_hip.h declares: name -> (restype, argtypes)
 _VP, _I, _F = C.c_void_p, C.c_int, C.c_float
 _I64P = C.POINTER(C.c_int64)
@@ -183,6 +191,13 @@ SYMBOLS = {
     "ddmi_train_eps_loss": (_I, [_VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _VP, _I, _I, _I, _VP]),
     "ddmi_train_adamw": (_I, [_VP, _VP, _VP, _VP, C.c_int64, _F, _F, _F, _F, _F, _I, _F, _VP]),
     "ddmi_train_ema": (_I, [_VP, _VP, C.c_int64, _F, _VP]),
+    # fine-tuning (include/ddmi_hip.h "Fine-tuning")
+    "ddmi_train_loss_workspace_bytes": (_I, [_I, _I, C.c_int64, _I, C.POINTER(C.c_size_t)]),
+    "ddmi_train_pref_loss": (_I, [C.POINTER(LossIn), _I, _I, C.c_double, C.c_double, _VP, C.c_size_t, _VP, _VP, _VP, _VP]),
+    "ddmi_train_pref_loss_bwd": (_I, [C.POINTER(LossIn), _I, _I, C.c_double, C.c_double, _VP, C.c_size_t, _VP, _VP, _VP, _VP]),
+    "ddmi_train_policy_loss": (_I, [C.POINTER(LossIn), _I, _VP, _VP, _VP, C.c_double, C.c_double, _VP, C.c_size_t, _VP, _VP, _VP, _VP, _VP]),
+    "ddmi_train_policy_loss_bwd": (_I, [C.POINTER(LossIn), _I, _VP, _VP, C.c_size_t, _VP, _VP, _VP, _VP]),
+    "ddmi_train_adamw_multi": (_I, [_VP, _I, C.c_double, C.c_double, C.c_double, C.c_double, C.c_uint32, _I, _I, _I, _VP]),
 }
 
 _lib: Optional[C.CDLL] = None

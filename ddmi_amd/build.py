@@ -16,7 +16,8 @@ LIBDIR = os.path.join(HERE, "lib")
 OBJDIR = os.path.join(LIBDIR, "obj")
 LIB = os.path.join(LIBDIR, "libddmi_hip.so")
 SOURCES = ["k_elementwise.hip", "k_groupnorm.hip", "k_conv.hip", "k_attention.hip", "k_attnblock.hip", "k_mlp2d.hip", "k_mlp3d.hip", "mlp3d_host.hip", "k_mlpv.hip", "mlpv_host.hip", "k_mcubes.hip", "models_video.hip", "net.hip",
-           "models.hip", "mlp2d_host.hip", "capi.hip", "prof.hip", "k_train.hip", "k_attn_bwd.hip", "train_capi.hip", "k_microbench.hip"]
+           "models.hip", "mlp2d_host.hip", "capi.hip", "prof.hip", "k_train.hip", "k_attn_bwd.hip", "train_capi.hip", "k_microbench.hip", "k_finetune.hip", "k_adamw.hip",
+           "finetune_capi.hip"]
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=on", "-Wall", "-Wno-unused-function",
          "-Wno-unused-variable", "-Wno-unused-but-set-variable",
          # no packed fp32 arithmetic (v_pk_add / mul / fma_f32): hipcc forms it by itself from ordinary float code, and some of its forms have
@@ -43,7 +44,9 @@ def _newest_header() -> float:
 # is an anti-lever beside MFMAs (MI355X_MICROARCH.md, per-instruction cycle constants): measured on one box, attention backward
 # dQ 289 -> 266 us, dK/dV 380 -> 360, the eager-maximum forward 270 -> 261; the lazy forward has none in its hot path (unchanged)
 _ATTN_FLAGS = ["-mllvm", "-amdgpu-mfma-vgpr-form", "-fno-slp-vectorize"]
-EXTRA_FLAGS = {"k_attention.hip": _ATTN_FLAGS, "k_attn_bwd.hip": _ATTN_FLAGS, "k_attnblock.hip": _ATTN_FLAGS}
+EXTRA_FLAGS = {"k_attention.hip": _ATTN_FLAGS, "k_attn_bwd.hip": _ATTN_FLAGS, "k_attnblock.hip": _ATTN_FLAGS,
+               # values rounded to 8-bit codes have one value only when no product is contracted into an FMA
+               "k_adamw.hip": ["-ffp-contract=off"]}
 
 
 def _compile(src: str, force: bool, hdr_mtime: float) -> str:

@@ -1,0 +1,49 @@
+// The fine-tuning losses' kernels (k_finetune.hip) as the C entry points (finetune_capi.hip) see them.
+#pragma once
+#include "common.h"
+
+enum { FT_PREF = 0, FT_POLICY = 1 };
+#define FT_THREADS 256
+#define FT_ROWS 512      // most rows (sample, channel) of one workgroup: their mixing coefficients sit in LDS
+
+struct FtArgs {
+  // inputs; `second` is the noise (preference; second_rows = pairs when both of a pair share it) or the chain's next state (policy)
+  const void* out;
+  const void* ref;
+  const float* x;
+  const float* second;
+  int second_rows;
+  const float* s1;           // sqrt(1 - abar_t) a sample
+  const float* logit;
+  const float* ref_logit;
+  const float* weight;       // a pair / transition; not > 0: left out, its values are not read
+  const float* transition;   // [B][3]: mean = A x_t + E eps, standard deviation
+  const float* logp_old;
+  const float* advantage;
+  double beta, smoothing, clip, kl_coef;
+  // outputs
+  float* loss;
+  float* row_out[3];         // margin, mse | logp, ratio, kl
+  const float* dloss;        // upstream gradient, a device scalar
+  void* d_out;
+  float* d_logit;
+  // plan
+  int B, C, pairs;
+  int64_t T, seg;
+  int wps, rows_per_wg, nseg, log_g;
+  // workspace
+  unsigned* counter;
+  float2* coef;              // a sample: factors of the residual and of the step away from the reference
+  double* term;
+  double2* part;             // a workgroup of sums_kernel
+  double2* chan;             // a (sample, channel, segment, wave): sums the mixing logit's gradient needs
+};
+int ft_plan(FtArgs* a, int B, int C, int64_t HW, bool mixed);
+size_t ft_workspace_bytes(const FtArgs& a);
+void ft_carve(FtArgs* a, void* ws);
+int launch_ft_sums(const FtArgs& a, int mode, int dt, hipStream_t s);
+int launch_ft_grad(const FtArgs& a, int mode, int dt, hipStream_t s);
+
+#define ADAMW_BLOCK 256      // values of a tensor that share one scale of the 8-bit moments
+int launch_adamw_multi(const ddmi_adamw_tensor* t, int n, double beta1, double beta2, double eps, double grad_scale, unsigned seed, int pdt, int gdt,
+                       int state_bits, hipStream_t s);

@@ -1,0 +1,109 @@
+// C ABI of the fine-tuning operators (include/ddmi_hip.h, "Fine-tuning"): no handle, no state; the caller owns every buffer, the losses'
+// workspace among them (so two captured graphs, or two streams, that use workspaces of their own share nothing).
+#include "finetune.h"
+
+namespace {
+bool dtype_ok(int dt) { return dt == DDMI_DTYPE_F32 || dt == DDMI_DTYPE_BF16; }
+int internal_dt(int dt) { return dt == DDMI_DTYPE_F32 ? DT_F32 : DT_BF16; }
+
+int common_args(FtArgs* a, const ddmi_loss_in* in, int B, void* ws, size_t ws_bytes, const char* who) {
+  const std::string w(who);
+  DDMI_REQUIRE(in->model_out && in->second && B > 0 && in->C > 0 && in->HW > 0, w + ": null argument or empty batch");
+  DDMI_REQUIRE(dtype_ok(in->out_dtype), w + ": model_out / ref_out are fp32 or bf16");
+  DDMI_REQUIRE((in->mixing_logit == nullptr) == (in->ref_mixing_logit == nullptr) || (in->mixing_logit && !in->ref_out), w + ": both mixing logits or none");
+  DDMI_REQUIRE(!in->mixing_logit || (in->x_t && in->sqrt_1mac), w + ": mixing needs x_t and sqrt_1mac");
+  DDMI_REQUIRE((double)in->C * (double)in->HW < 1.1e12, w + ": sample too large");
+  DDMI_TRY(ft_plan(a, B, in->C, in->HW, in->mixing_logit != nullptr));
+  DDMI_REQUIRE(ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= ft_workspace_bytes(*a), w + ": workspace too small or not 16-byte aligned");
+  ft_carve(a, ws);
+  a->out = in->model_out; a->ref = in->ref_out; a->x = in->x_t; a->second = in->second; a->s1 = in->mixing_logit ? in->sqrt_1mac : nullptr;
+  a->logit = in->mixing_logit; a->ref_logit = in->ref_mixing_logit; a->weight = in->weight;
+  return DDMI_OK;
+}
+// the gradient needs neither the reference's output nor its logit (its residual is the trained network's alone)
+int pref_args(FtArgs* a, const ddmi_loss_in* in, int pairs, int noise_rows, double beta, double label_smoothing, bool grad, void* ws, size_t ws_bytes) {
+  DDMI_REQUIRE(in && (grad || in->ref_out) && pairs > 0 && pairs <= (1 << 29), "pref_loss: null argument or no pairs");
+  DDMI_REQUIRE(noise_rows == pairs || noise_rows == 2 * pairs, "pref_loss: the noise has a row for each pair or for each sample");
+  DDMI_REQUIRE(label_smoothing >= 0.0 && label_smoothing <= 1.0 && beta == beta, "pref_loss: label_smoothing in [0, 1], beta a number");
+  DDMI_TRY(common_args(a, in, 2 * pairs, ws, ws_bytes, "pref_loss"));
+  if (!in->mixing_logit) a->x = nullptr;      // not read
+  a->pairs = pairs; a->second_rows = noise_rows; a->beta = beta; a->smoothing = label_smoothing;
+  return DDMI_OK;
+}
+int policy_args(FtArgs* a, const ddmi_loss_in* in, int B, const float* transition, void* ws, size_t ws_bytes) {
+  DDMI_REQUIRE(in && transition && in->x_t, "policy_loss: null argument");
+  DDMI_TRY(common_args(a, in, B, ws, ws_bytes, "policy_loss"));
+  a->pairs = B; a->second_rows = B; a->transition = transition;
+  return DDMI_OK;
+}
+}  // namespace
+
+extern "C" {
+
+int ddmi_train_loss_workspace_bytes(int B, int C, int64_t HW, int mixed, size_t* bytes) {
+  DDMI_REQUIRE(bytes && B > 0 && C > 0 && HW > 0 && (double)C * (double)HW < 1.1e12, "train_loss_workspace_bytes: bad arguments");
+  FtArgs a{};
+  DDMI_TRY(ft_plan(&a, B, C, HW, mixed != 0));
+  *bytes = ft_workspace_bytes(a);
+  return DDMI_OK;
+}
+
+int ddmi_train_pref_loss(const ddmi_loss_in* in, int pairs, int noise_rows, double beta, double label_smoothing, void* ws, size_t ws_bytes, float* loss,
+                         float* margin, float* mse, void* stream) {
+  FtArgs a{};
+  DDMI_REQUIRE(loss && margin && mse, "pref_loss: null output");
+  DDMI_TRY(pref_args(&a, in, pairs, noise_rows, beta, label_smoothing, false, ws, ws_bytes));
+  a.loss = loss; a.row_out[0] = margin; a.row_out[1] = mse;
+  return launch_ft_sums(a, FT_PREF, internal_dt(in->out_dtype), (hipStream_t)stream);
+}
+int ddmi_train_pref_loss_bwd(const ddmi_loss_in* in, int pairs, int noise_rows, double beta, double label_smoothing, void* ws, size_t ws_bytes,
+                             const float* dloss, void* d_model_out, float* d_logit, void* stream) {
+  FtArgs a{};
+  DDMI_REQUIRE(d_model_out, "pref_loss_bwd: null output");
+  DDMI_TRY(pref_args(&a, in, pairs, noise_rows, beta, label_smoothing, true, ws, ws_bytes));
+  DDMI_REQUIRE(!d_logit || in->mixing_logit, "pref_loss_bwd: a logit's gradient without a logit");
+  a.dloss = dloss; a.d_out = d_model_out; a.d_logit = d_logit;
+  return launch_ft_grad(a, FT_PREF, internal_dt(in->out_dtype), (hipStream_t)stream);
+}
+int ddmi_train_policy_loss(const ddmi_loss_in* in, int B, const float* transition, const float* logp_old, const float* advantage, double clip_range,
+                           double kl_coef, void* ws, size_t ws_bytes, float* loss, float* logp, float* ratio, float* kl, void* stream) {
+  FtArgs a{};
+  DDMI_REQUIRE(logp, "policy_loss: null output");
+  DDMI_REQUIRE(!logp_old || (advantage && loss && ratio && kl), "policy_loss: null argument");
+  DDMI_REQUIRE(clip_range >= 0.0 && kl_coef == kl_coef, "policy_loss: clip_range >= 0, kl_coef a number");
+  DDMI_REQUIRE(kl_coef == 0.0 || (in && in->ref_out), "policy_loss: a KL term needs the reference's output");
+  DDMI_TRY(policy_args(&a, in, B, transition, ws, ws_bytes));
+  a.logp_old = logp_old; a.advantage = advantage; a.clip = clip_range; a.kl_coef = kl_coef;
+  a.loss = logp_old ? loss : nullptr; a.row_out[0] = logp; a.row_out[1] = ratio; a.row_out[2] = kl;
+  return launch_ft_sums(a, FT_POLICY, internal_dt(in->out_dtype), (hipStream_t)stream);
+}
+int ddmi_train_policy_loss_bwd(const ddmi_loss_in* in, int B, const float* transition, void* ws, size_t ws_bytes, const float* dloss, void* d_model_out,
+                               float* d_logit, void* stream) {
+  FtArgs a{};
+  DDMI_REQUIRE(d_model_out, "policy_loss_bwd: null output");
+  DDMI_TRY(policy_args(&a, in, B, transition, ws, ws_bytes));
+  DDMI_REQUIRE(!d_logit || in->mixing_logit, "policy_loss_bwd: a logit's gradient without a logit");
+  a.dloss = dloss; a.d_out = d_model_out; a.d_logit = d_logit;
+  return launch_ft_grad(a, FT_POLICY, internal_dt(in->out_dtype), (hipStream_t)stream);
+}
+
+int ddmi_train_adamw_multi(const ddmi_adamw_tensor* tensors, int n, double beta1, double beta2, double eps, double grad_scale, uint32_t seed,
+                           int param_dtype, int grad_dtype, int state_bits, void* stream) {
+  DDMI_REQUIRE(n == 0 || (tensors && n > 0), "adamw_multi: null argument");
+  DDMI_REQUIRE(dtype_ok(param_dtype) && dtype_ok(grad_dtype), "adamw_multi: parameters and gradients are fp32 or bf16");
+  DDMI_REQUIRE(state_bits == 32 || state_bits == 8, "adamw_multi: moments have 32 or 8 bits");
+  DDMI_REQUIRE(beta1 >= 0.0 && beta1 < 1.0 && beta2 >= 0.0 && beta2 < 1.0 && eps >= 0.0, "adamw_multi: betas in [0, 1), eps >= 0");
+  for (int i = 0; i < n; ++i) {
+    const ddmi_adamw_tensor& t = tensors[i];
+    DDMI_REQUIRE(t.numel >= 0 && t.step >= 1, "adamw_multi: step counts from 1");
+    if (t.numel == 0) continue;
+    DDMI_REQUIRE(t.param && t.grad && t.exp_avg && t.exp_avg_sq, "adamw_multi: null tensor");
+    DDMI_REQUIRE(state_bits == 32 || (t.exp_avg_scale && t.exp_avg_sq_scale), "adamw_multi: 8-bit moments need their scales");
+    DDMI_REQUIRE(((uintptr_t)t.param & (param_dtype == DDMI_DTYPE_F32 ? 3 : 1)) == 0 && ((uintptr_t)t.grad & (grad_dtype == DDMI_DTYPE_F32 ? 3 : 1)) == 0,
+                 "adamw_multi: tensors aligned to their values");
+  }
+  return launch_adamw_multi(tensors, n, beta1, beta2, eps, grad_scale, seed, internal_dt(param_dtype), internal_dt(grad_dtype), state_bits,
+                            (hipStream_t)stream);
+}
+
+}  // extern "C"

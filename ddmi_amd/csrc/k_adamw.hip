@@ -1,0 +1,266 @@
+// AdamW (decoupled weight decay, bias-corrected moments) over many tensors in a few launches, with the moments in 32 or in 8 bits.
+//
+//   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2,  p = p (1 - lr wd) - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+//
+// 8-bit moments: blocks of 256 consecutive values of a tensor share one fp32 scale, a power of two that puts the block's largest value
+// into (128, 256]; a value is an e4m3 code (bias 7, subnormals down to 2^-9: 2^17 below the block's largest).  m is stored as it is, v as
+// its ROOT (half the exponent range).  Both are rounded STOCHASTICALLY: a step changes v by about one part in 1 / (1 - b2) = 1000, an e4m3
+// step is one part in 8..16, so round-to-nearest would leave v where it is for ever; rounding up with the probability of the cut-off part
+// keeps the running averages unbiased.  A v that is not zero never becomes zero (its root divides).  bf16 parameters are rounded the same
+// way, for the same reason (a step of 1e-4 of the value against a spacing of 2^-8).  The random bits are a 32-bit integer mix of (seed,
+// step, tensor, block, place): nothing depends on the launch, so a step is reproducible bit for bit.
+// This file is compiled without FMA contraction: the moments that are rounded to codes are then the same on every path.
+#include <algorithm>
+#include <cmath>
+#include <vector>
+#include "kernels.h"
+#include "finetune.h"
+#include "prof.h"
+
+namespace {
+constexpr int AD_TENSORS = 48;           // tensors of one launch: their table rides in the kernel's arguments (no upload, capturable)
+constexpr int AD_UNROLL = 4;             // blocks of 256 values a wave works on at a time
+constexpr int AD_CHUNK = 4 * AD_UNROLL * ADAMW_BLOCK;   // values of a workgroup of four waves
+
+struct AdTensor {
+  void* p;
+  const void* g;
+  void* m;
+  void* v;
+  float* ms;
+  float* vs;
+  int64_t n;
+  float decay, size, inv_bc2;            // 1 - lr wd, lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
+  unsigned key;
+};
+struct AdArgs {
+  AdTensor t[AD_TENSORS];
+  unsigned first[AD_TENSORS + 1];        // workgroups before tensor i
+  int count;
+  float b1, omb1, b2, omb2, eps, gscale;
+};
+static_assert(sizeof(AdArgs) <= 4096, "kernel arguments");
+
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned short u16x4u __attribute__((ext_vector_type(4), aligned(2)));
+struct __attribute__((packed)) u32u { unsigned v; };
+
+__host__ __device__ __forceinline__ unsigned mix32(unsigned x) {
+  x ^= x >> 16;
+  x *= 0x85EBCA6Bu;
+  x ^= x >> 13;
+  x *= 0xC2B2AE35u;
+  return x ^ (x >> 16);
+}
+
+// four values at `at`, of which `left` (1..4) exist
+template <typename T> __device__ __forceinline__ void load(const void* base, int64_t at, int left, float (&v)[4]);
+template <> __device__ __forceinline__ void load<float>(const void* base, int64_t at, int left, float (&v)[4]) {
+  const float* p = (const float*)base + at;
+  if (left >= 4) { const f32x4u t = *reinterpret_cast<const f32x4u*>(p); v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w; return; }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = i < left ? p[i] : 0.f;
+}
+template <> __device__ __forceinline__ void load<bf16_t>(const void* base, int64_t at, int left, float (&v)[4]) {
+  const unsigned short* p = (const unsigned short*)base + at;
+  unsigned short u[4] = {0, 0, 0, 0};
+  if (left >= 4) { const u16x4u t = *reinterpret_cast<const u16x4u*>(p); u[0] = t.x; u[1] = t.y; u[2] = t.z; u[3] = t.w; }
+  else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) if (i < left) u[i] = p[i];
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = __uint_as_float((unsigned)u[i] << 16);
+}
+__device__ __forceinline__ void store(float* base, int64_t at, int left, const float (&v)[4]) {
+  float* p = base + at;
+  if (left >= 4) { const f32x4u t = {v[0], v[1], v[2], v[3]}; *reinterpret_cast<f32x4u*>(p) = t; return; }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) if (i < left) p[i] = v[i];
+}
+__device__ __forceinline__ void store(bf16_t* base, int64_t at, int left, const unsigned short (&u)[4]) {
+  unsigned short* p = (unsigned short*)base + at;
+  if (left >= 4) { const u16x4u t = {u[0], u[1], u[2], u[3]}; *reinterpret_cast<u16x4u*>(p) = t; return; }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) if (i < left) p[i] = u[i];
+}
+__device__ __forceinline__ unsigned load_codes(const unsigned char* p, int left) {
+  if (left >= 4) return reinterpret_cast<const u32u*>(p)->v;
+  unsigned c = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) if (i < left) c |= (unsigned)p[i] << (8 * i);
+  return c;
+}
+__device__ __forceinline__ void store_codes(unsigned char* p, int left, unsigned c) {
+  if (left >= 4) { reinterpret_cast<u32u*>(p)->v = c; return; }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) if (i < left) p[i] = (unsigned char)(c >> (8 * i));
+}
+__device__ __forceinline__ void decode(unsigned c, float scale, float (&v)[4]) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, true);
+  v[0] = lo.x * scale; v[1] = lo.y * scale; v[2] = hi.x * scale; v[3] = hi.y * scale;
+}
+// e4m3 of x (|x| <= 256 or not finite), rounded up in magnitude when the 20 random bits r reach the part that is cut off
+template <bool ROOT> __device__ __forceinline__ unsigned encode(float x, unsigned r) {
+  const unsigned bits = __float_as_uint(x) & 0x7FFFFFFFu;
+  const float a = __uint_as_float(bits);
+  const unsigned normal = ((bits + r) >> 20) - (120u << 3);                  // exponent and three fraction bits; a carry moves on to the next binade
+  const unsigned small = (unsigned)(int)floorf(a * 512.0f + (float)r * 0x1p-20f);
+  unsigned code = a < 0x1p-6f ? small : normal;
+  if (bits >= 0x7F800000u) code = 0x7Fu;                                      // NaN and infinity: the code's NaN
+  if (ROOT) return (bits != 0u && code == 0u) ? 1u : code;
+  return code | ((__float_as_uint(x) >> 24) & 0x80u);
+}
+// the largest of a wave's 64 non-negative integers, in every lane
+__device__ __forceinline__ unsigned wave_max(unsigned x) {
+  for (int st = 32; st > 0; st >>= 1) x = max(x, (unsigned)__shfl_xor((int)x, st));
+  return x;
+}
+// 2^k that puts `most` (bits of a finite non-negative float) into (128, 256], and 2^-k
+__device__ __forceinline__ void block_scale(unsigned most, float& scale, float& inv) {
+  int k = (int)(most >> 23) - 127 + ((most & 0x7FFFFFu) != 0u ? 1 : 0) - 8;
+  k = min(max(k, -120), 120);
+  scale = __uint_as_float((unsigned)(k + 127) << 23);
+  inv = __uint_as_float((unsigned)(127 - k) << 23);
+}
+
+template <typename PT, typename GT, int BITS>
+__global__ void __launch_bounds__(256) adamw_multi_kernel(AdArgs a) {
+  // the tensor this workgroup works on
+  int lo = 0, hi = a.count - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (a.first[mid] <= blockIdx.x) lo = mid; else hi = mid - 1;
+  }
+  const AdTensor& t = a.t[lo];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t blk0 = ((int64_t)(blockIdx.x - a.first[lo]) * 4 + wave) * AD_UNROLL;
+  float p[AD_UNROLL][4], g[AD_UNROLL][4], m[AD_UNROLL][4], v[AD_UNROLL][4];
+  int left[AD_UNROLL];
+#pragma unroll
+  for (int u = 0; u < AD_UNROLL; ++u) {
+    const int64_t at = (blk0 + u) * ADAMW_BLOCK + 4 * lane;
+    left[u] = at >= t.n ? 0 : (int)min((int64_t)4, t.n - at);
+    if (left[u] > 0) {
+      load<PT>(t.p, at, left[u], p[u]);
+      load<GT>(t.g, at, left[u], g[u]);
+      if (BITS == 32) {
+        load<float>(t.m, at, left[u], m[u]);
+        load<float>(t.v, at, left[u], v[u]);
+      } else {
+        decode(load_codes((const unsigned char*)t.m + at, left[u]), t.ms[blk0 + u], m[u]);
+        decode(load_codes((const unsigned char*)t.v + at, left[u]), t.vs[blk0 + u], v[u]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) p[u][i] = g[u][i] = m[u][i] = v[u][i] = 0.f;
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < AD_UNROLL; ++u) {
+    if (blk0 * ADAMW_BLOCK + (int64_t)u * ADAMW_BLOCK >= t.n) break;        // the same in every lane of the wave
+    const int64_t blk = blk0 + u, at = blk * ADAMW_BLOCK + 4 * lane;
+    unsigned rnd[4] = {0u, 0u, 0u, 0u};
+    if (BITS == 8 || sizeof(PT) == 2) {
+      const unsigned kb = mix32(t.key + (unsigned)blk * 0x9E3779B9u);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) rnd[i] = mix32(kb + (unsigned)(4 * lane + i) * 0x9E3779B9u);
+    }
+    float root[4];
+    unsigned mm = 0u, mv = 0u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float gi = g[u][i] * a.gscale;
+      const float vo = BITS == 8 ? v[u][i] * v[u][i] : v[u][i];
+      m[u][i] = m[u][i] * a.b1 + gi * a.omb1;
+      v[u][i] = vo * a.b2 + (gi * a.omb2) * gi;
+      root[i] = sqrtf(v[u][i]);
+      p[u][i] = p[u][i] * t.decay - (m[u][i] / (root[i] * t.inv_bc2 + a.eps)) * t.size;
+      if (BITS == 8 && i < left[u]) {
+        const unsigned bm = __float_as_uint(m[u][i]) & 0x7FFFFFFFu, bv = __float_as_uint(root[i]) & 0x7FFFFFFFu;
+        mm = bm < 0x7F800000u && bm > mm ? bm : mm;
+        mv = bv < 0x7F800000u && bv > mv ? bv : mv;
+      }
+    }
+    if (left[u] > 0) {
+      if (sizeof(PT) == 4) store((float*)t.p, at, left[u], p[u]);
+      else {
+        unsigned short w[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const unsigned bits = __float_as_uint(p[u][i]);
+          const bool finite = (bits & 0x7FFFFFFFu) < 0x7F800000u;
+          w[i] = (unsigned short)((finite ? bits + (mix32(rnd[i] ^ 0x68E31DA4u) & 0xFFFFu) : (p[u][i] != p[u][i] ? 0x7FC00000u : bits)) >> 16);
+        }
+        store((bf16_t*)t.p, at, left[u], w);
+      }
+    }
+    if (BITS == 32) {
+      if (left[u] > 0) {
+        store((float*)t.m, at, left[u], m[u]);
+        store((float*)t.v, at, left[u], v[u]);
+      }
+    } else {
+      float sm, im, sv, iv;
+      block_scale(wave_max(mm), sm, im);
+      block_scale(wave_max(mv), sv, iv);
+      unsigned cm = 0u, cv = 0u;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        cm |= encode<false>(m[u][i] * im, ((rnd[i] & 0xFFFu) << 8) | 0x80u) << (8 * i);
+        cv |= encode<true>(root[i] * iv, rnd[i] >> 12) << (8 * i);
+      }
+      if (left[u] > 0) {
+        store_codes((unsigned char*)t.m + at, left[u], cm);
+        store_codes((unsigned char*)t.v + at, left[u], cv);
+      }
+      if (lane == 0) { t.ms[blk] = sm; t.vs[blk] = sv; }
+    }
+  }
+}
+
+template <int BITS>
+int launch_bits(const AdArgs& a, unsigned grid, int pdt, int gdt, hipStream_t s) {
+  if (pdt == DT_F32 && gdt == DT_F32) hipLaunchKernelGGL((adamw_multi_kernel<float, float, BITS>), dim3(grid), dim3(256), 0, s, a);
+  else if (pdt == DT_F32) hipLaunchKernelGGL((adamw_multi_kernel<float, bf16_t, BITS>), dim3(grid), dim3(256), 0, s, a);
+  else if (gdt == DT_F32) hipLaunchKernelGGL((adamw_multi_kernel<bf16_t, float, BITS>), dim3(grid), dim3(256), 0, s, a);
+  else hipLaunchKernelGGL((adamw_multi_kernel<bf16_t, bf16_t, BITS>), dim3(grid), dim3(256), 0, s, a);
+  HIP_TRY(hipGetLastError());
+  return DDMI_OK;
+}
+}  // namespace
+
+int launch_adamw_multi(const ddmi_adamw_tensor* t, int n, double beta1, double beta2, double eps, double grad_scale, unsigned seed, int pdt, int gdt,
+                       int state_bits, hipStream_t s) {
+  double values = 0.0;
+  for (int i = 0; i < n; ++i) values += (double)t[i].numel;
+  PROF_SCOPE(state_bits == 8 ? "adamw8" : "adamw_multi", 0, values * (2.0 * dt_size(pdt) + dt_size(gdt) + (state_bits == 8 ? 4.0 : 16.0)), s);
+  AdArgs a;
+  a.b1 = (float)beta1; a.omb1 = (float)(1.0 - beta1); a.b2 = (float)beta2; a.omb2 = (float)(1.0 - beta2);
+  a.eps = (float)eps; a.gscale = (float)grad_scale;
+  int i = 0;
+  while (i < n) {
+    a.count = 0;
+    a.first[0] = 0;
+    while (i < n && a.count < AD_TENSORS) {
+      const ddmi_adamw_tensor& d = t[i];
+      const int64_t wgs = cdiv64(d.numel, AD_CHUNK);
+      if (wgs == 0) { ++i; continue; }
+      if (wgs > (1ll << 30)) return ddmi_fail(DDMI_ERR_INVALID, "adamw_multi: a tensor of more than 2^42 values");
+      if ((int64_t)a.first[a.count] + wgs > (1ll << 30)) break;
+      AdTensor& o = a.t[a.count];
+      o.p = d.param; o.g = d.grad; o.m = d.exp_avg; o.v = d.exp_avg_sq; o.ms = d.exp_avg_scale; o.vs = d.exp_avg_sq_scale; o.n = d.numel;
+      o.decay = (float)(1.0 - d.lr * d.weight_decay);
+      o.size = (float)(d.lr / (1.0 - std::pow(beta1, (double)d.step)));
+      o.inv_bc2 = (float)(1.0 / std::sqrt(1.0 - std::pow(beta2, (double)d.step)));
+      o.key = mix32(mix32(mix32(seed) + (unsigned)d.step * 0x9E3779B9u) + (unsigned)(d.index + 1) * 0x85EBCA77u);
+      a.first[a.count + 1] = a.first[a.count] + (unsigned)wgs;
+      ++a.count;
+      ++i;
+    }
+    if (a.count == 0) continue;
+    DDMI_TRY(state_bits == 8 ? launch_bits<8>(a, a.first[a.count], pdt, gdt, s) : launch_bits<32>(a, a.first[a.count], pdt, gdt, s));
+  }
+  return DDMI_OK;
+}

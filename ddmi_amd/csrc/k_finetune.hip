@@ -1,0 +1,398 @@
+// Fine-tuning losses of a trained latent diffusion model, each with its gradient: the preference loss (paired log ratios of denoising
+// errors against a frozen reference network) and the clipped policy loss with a KL term (log-density of a denoising transition).
+//
+// Per value, with c = sigmoid(logit[channel]) and m = sqrt(1 - abar_t) x_t (the mixed prediction; without a logit eps = o):
+//   eps = m + c (o - m),   eps - eps_ref = c (o - r) + (c - c_ref) (r - m)          (r: the reference's output; no cancellation)
+//   preference:  d = eps - noise,                  sums  (eps - eps_ref) (2 d - (eps - eps_ref)) = d^2 - d_ref^2,  d^2,  d (o - m)
+//   policy:      z = (x_prev - A x_t) - E eps,     sums  z^2,  (eps - eps_ref)^2,  z (o - m),  (eps - eps_ref) (o - m)
+// One scalar (two with KL) a sample follows from the sums over ALL of its values, and only then is the gradient known:
+//   d loss / d o = c (k z' + q far).  So: sums_kernel (reads every input once), rows_kernel (a workgroup a pair / transition: the scalar
+//   work in 64 bits, the last one to finish adds up the loss), grad_kernel (reads again what the gradient needs, writes it).
+// Factors are rounded in fp32, products and sums are held in fp64: a margin is the difference of two nearly equal errors times
+// beta ~ 10^3, and a logit's gradient a sum of either sign over the batch.  No float atomics: every sum has a fixed order.
+#include <algorithm>
+#include "kernels.h"
+#include "finetune.h"
+#include "prof.h"
+
+namespace {
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));            // rows of an odd plane start at any element
+typedef unsigned short u16x4u __attribute__((ext_vector_type(4), aligned(2)));
+
+__device__ __forceinline__ void load4(const float* p, float (&v)[4]) {
+  const f32x4u t = *reinterpret_cast<const f32x4u*>(p);
+  v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
+}
+__device__ __forceinline__ float bf16_bits(unsigned short u) { return __uint_as_float((unsigned)u << 16); }
+__device__ __forceinline__ void load4(const bf16_t* p, float (&v)[4]) {
+  const u16x4u t = *reinterpret_cast<const u16x4u*>(p);
+  v[0] = bf16_bits(t.x); v[1] = bf16_bits(t.y); v[2] = bf16_bits(t.z); v[3] = bf16_bits(t.w);
+}
+__device__ __forceinline__ void store4(float* p, const float (&v)[4]) {
+  f32x4u t = {v[0], v[1], v[2], v[3]};
+  *reinterpret_cast<f32x4u*>(p) = t;
+}
+__device__ __forceinline__ void store4(bf16_t* p, const float (&v)[4]) {   // the gradient's one rounding, to the network output's own type
+  u16x4u t;
+  t.x = __builtin_bit_cast(unsigned short, (bf16_t)v[0]); t.y = __builtin_bit_cast(unsigned short, (bf16_t)v[1]);
+  t.z = __builtin_bit_cast(unsigned short, (bf16_t)v[2]); t.w = __builtin_bit_cast(unsigned short, (bf16_t)v[3]);
+  *reinterpret_cast<u16x4u*>(p) = t;
+}
+
+// what a workgroup works on: rows [row0, row0 + rows) of sample b, values [t0, t1) of each
+struct Span {
+  int b, row0, rows, seg;
+  int64_t t0, t1;
+};
+__device__ __forceinline__ Span span_of(const FtArgs& a, int blk) {
+  Span s;
+  s.b = blk / a.wps;
+  const int j = blk - s.b * a.wps;
+  s.row0 = (j / a.nseg) * a.rows_per_wg;
+  s.seg = j - (j / a.nseg) * a.nseg;
+  s.rows = min(a.rows_per_wg, a.C - s.row0);
+  s.t0 = (int64_t)s.seg * a.seg;
+  s.t1 = s.t0 + a.seg < a.T ? s.t0 + a.seg : a.T;
+  return s;
+}
+template <int MODE>
+__device__ __forceinline__ bool takes_part(const FtArgs& a, int b) {
+  if (a.weight && !(a.weight[MODE == FT_PREF ? b % a.pairs : b] > 0.f)) return false;
+  // a transition without noise has no density
+  if (MODE == FT_POLICY && !(a.transition[3 * (int64_t)b + 2] > 0.f)) return false;
+  return true;
+}
+// c and c - c_ref of the span's rows; the difference is taken in fp64, it may be far below c
+__device__ __forceinline__ void mix_rows(const FtArgs& a, const Span& s, float2* mix) {
+  for (int r = threadIdx.x; r < s.rows; r += FT_THREADS) {
+    const double c = 1.0 / (1.0 + exp(-(double)a.logit[s.row0 + r]));
+    const double cr = a.ref_logit ? 1.0 / (1.0 + exp(-(double)a.ref_logit[s.row0 + r])) : c;
+    mix[r] = make_float2((float)c, (float)(c - cr));
+  }
+  __syncthreads();
+}
+
+struct Elem {
+  float s1, A, E, c, dc;
+};
+// the residual whose square is summed, the step away from the reference (before E), and o - m
+template <int MODE, bool MIX, bool REF>
+__device__ __forceinline__ void element(const Elem& e, float o, float r, float x, float y, float& res, float& far, float& part) {
+  const float m = MIX ? e.s1 * x : 0.f;
+  part = MIX ? o - m : 0.f;
+  const float eps = MIX ? fmaf(e.c, part, m) : o;
+  far = REF ? (MIX ? fmaf(e.c, o - r, e.dc * (r - m)) : o - r) : 0.f;
+  if (MODE == FT_PREF) res = eps - y;
+  else res = fmaf(-e.E, eps, fmaf(-e.A, x, y));
+}
+
+template <int MODE, bool MIX, bool REF>
+__device__ __forceinline__ void add_up(float res, float far, float part, double& S0, double& S1, double& S2, double& S3) {
+  const double r = res, f = far;
+  if (MODE == FT_PREF) { S0 = fma(f, 2.0 * r - f, S0); S1 = fma(r, r, S1); }
+  else { S0 = fma(r, r, S0); if (REF) S1 = fma(f, f, S1); }
+  if (MIX) { S2 = fma(r, (double)part, S2); if (MODE == FT_POLICY && REF) S3 = fma(f, (double)part, S3); }
+}
+
+template <int MODE, bool MIX, bool REF, typename T>
+__global__ void __launch_bounds__(FT_THREADS) sums_kernel(FtArgs a) {
+  __shared__ float2 mix[FT_ROWS];
+  __shared__ double red[2][FT_THREADS / 64];
+  const int tid = threadIdx.x;
+  if (blockIdx.x == 0 && tid == 0) *a.counter = 0u;   // rows_kernel counts its workgroups; stream order makes this visible to it
+  const Span s = span_of(a, blockIdx.x);
+  const int G = 1 << a.log_g, lane = tid & (G - 1), group = tid >> a.log_g, ngroups = FT_THREADS >> a.log_g;
+  const int wpg = G > 64 ? G / 64 : 1;                // waves that share a row
+  const bool used = takes_part<MODE>(a, s.b);
+  double S0 = 0.0, S1 = 0.0;
+  if (MIX && used) mix_rows(a, s, mix);
+  Elem e{a.s1 ? a.s1[s.b] : 0.f, 0.f, 1.f, 1.f, 0.f};
+  if (MODE == FT_POLICY) { e.A = a.transition[3 * (int64_t)s.b]; e.E = a.transition[3 * (int64_t)s.b + 1]; }
+  const int64_t sb = (int64_t)(s.b % a.second_rows) * a.C;
+  for (int r0 = 0; r0 < s.rows; r0 += ngroups) {      // uniform trip count: the shuffles below see whole waves
+    const int r = r0 + group;
+    double S2 = 0.0, S3 = 0.0;
+    if (used && r < s.rows) {
+      if (MIX) { const float2 c = mix[r]; e.c = c.x; e.dc = c.y; }
+      const int64_t base = ((int64_t)s.b * a.C + s.row0 + r) * a.T, base2 = (sb + s.row0 + r) * a.T;
+      const T* po = (const T*)a.out + base;
+      const T* pr = REF ? (const T*)a.ref + base : nullptr;
+      const float* px = (MIX || MODE == FT_POLICY) ? a.x + base : nullptr;
+      const float* py = a.second + base2;
+      const int64_t nvec = (s.t1 - s.t0) / 4, tail = s.t0 + 4 * nvec;
+#pragma unroll 2
+      for (int64_t v = lane; v < nvec; v += G) {
+        const int64_t t = s.t0 + 4 * v;
+        float o[4], q[4] = {0.f, 0.f, 0.f, 0.f}, x[4] = {0.f, 0.f, 0.f, 0.f}, y[4];
+        load4(po + t, o);
+        if (REF) load4(pr + t, q);
+        if (MIX || MODE == FT_POLICY) load4(px + t, x);
+        load4(py + t, y);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float res, far, part;
+          element<MODE, MIX, REF>(e, o[i], q[i], x[i], y[i], res, far, part);
+          add_up<MODE, MIX, REF>(res, far, part, S0, S1, S2, S3);
+        }
+      }
+      if (tail + lane < s.t1) {                        // at most three values, one a lane (a group of fewer lanes takes turns)
+        for (int64_t t = tail + lane; t < s.t1; t += G) {
+          float res, far, part;
+          element<MODE, MIX, REF>(e, to_f32(po[t]), REF ? to_f32(pr[t]) : 0.f, (MIX || MODE == FT_POLICY) ? px[t] : 0.f, py[t], res, far, part);
+          add_up<MODE, MIX, REF>(res, far, part, S0, S1, S2, S3);
+        }
+      }
+    }
+    if (MIX) {
+      const int w = G < 64 ? G : 64;
+      for (int st = w >> 1; st > 0; st >>= 1) { S2 += __shfl_xor(S2, st); if (MODE == FT_POLICY && REF) S3 += __shfl_xor(S3, st); }
+      if (r < s.rows && (lane & 63) == 0)
+        a.chan[(((int64_t)s.b * a.C + s.row0 + r) * a.nseg + s.seg) * wpg + (lane >> 6)] = make_double2(S2, S3);
+    }
+  }
+  for (int st = 32; st > 0; st >>= 1) { S0 += __shfl_xor(S0, st); S1 += __shfl_xor(S1, st); }
+  if ((tid & 63) == 0) { red[0][tid >> 6] = S0; red[1][tid >> 6] = S1; }
+  __syncthreads();
+  if (tid == 0) {
+    double t0 = 0.0, t1 = 0.0;
+    for (int w = 0; w < FT_THREADS / 64; ++w) { t0 += red[0][w]; t1 += red[1][w]; }
+    a.part[blockIdx.x] = make_double2(t0, t1);
+  }
+}
+
+__device__ __forceinline__ double block_sum(double v, double* red) {
+  for (int st = 32; st > 0; st >>= 1) v += __shfl_xor(v, st);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  double t = 0.0;
+  for (int w = 0; w < FT_THREADS / 64; ++w) t += red[w];
+  return t;
+}
+__device__ __forceinline__ double2 sample_sums(const FtArgs& a, int b, double* red) {
+  double u = 0.0, v = 0.0;
+  for (int j = threadIdx.x; j < a.wps; j += FT_THREADS) {
+    const double2 p = a.part[(int64_t)b * a.wps + j];
+    u += p.x; v += p.y;
+  }
+  u = block_sum(u, red);
+  v = block_sum(v, red);
+  return make_double2(u, v);
+}
+// one workgroup a pair / transition; the last one to finish adds up the loss over them, in their order
+template <int MODE>
+__global__ void __launch_bounds__(FT_THREADS) rows_kernel(FtArgs a) {
+  __shared__ double red[FT_THREADS / 64];
+  __shared__ int last;
+  const int i = blockIdx.x, rows = gridDim.x, tid = threadIdx.x;
+  const double n = (double)a.C * (double)a.T;
+  double total = 0.0;
+  for (int j = tid; j < rows; j += FT_THREADS)
+    if (takes_part<MODE>(a, j)) total += a.weight ? (double)a.weight[j] : 1.0;
+  total = block_sum(total, red);
+  const bool used = takes_part<MODE>(a, i);
+  const double w = used ? (a.weight ? (double)a.weight[i] : 1.0) / total : 0.0;
+  double term = 0.0;
+  if (MODE == FT_PREF) {
+    const double2 sw = sample_sums(a, i, red), sl = sample_sums(a, i + a.pairs, red);
+    double h = 0.0, dh = 0.0;
+    if (used) {
+      h = -0.5 * a.beta * (sw.x - sl.x) / n;
+      const double t = log1p(exp(-fabs(h))), up = 1.0 / (1.0 + exp(-h)), ls = a.smoothing;   // -log sigma(h) = t - min(h, 0)
+      term = w * ((1.0 - ls) * (t - fmin(h, 0.0)) + ls * (t + fmax(h, 0.0)));
+      dh = w * (ls * up - (1.0 - ls) / (1.0 + exp(h)));
+    }
+    if (tid == 0) {
+      a.row_out[0][i] = (float)h;
+      a.row_out[1][i] = (float)(sw.y / n);
+      a.row_out[1][i + a.pairs] = (float)(sl.y / n);
+      a.coef[i] = make_float2((float)(-dh * a.beta / n), 0.f);
+      a.coef[i + a.pairs] = make_float2((float)(dh * a.beta / n), 0.f);
+    }
+  } else {
+    const double2 s = sample_sums(a, i, red);
+    double logp = 0.0, ratio = 0.0, kl = 0.0, k = 0.0, q = 0.0;
+    if (used) {
+      const double sd = a.transition[3 * (int64_t)i + 2], var = sd * sd, E = a.transition[3 * (int64_t)i + 1];
+      logp = -s.x / n / (2.0 * var) - log(sd) - 0.91893853320467274178;
+      if (a.logp_old) {
+        const double adv = a.advantage[i];
+        ratio = exp(logp - (double)a.logp_old[i]);
+        const double lo = 1.0 - a.clip, hi = 1.0 + a.clip, held = ratio < lo ? lo : (ratio > hi ? hi : ratio);
+        kl = E * E * s.y / n / (2.0 * var);
+        const double open = -adv * ratio, bound = -adv * held;
+        term = w * ((open >= bound ? open : (bound > open ? bound : open + bound)) + a.kl_coef * kl);   // the sum: NaN stays NaN
+        k = (open >= bound) ? -adv * ratio * w / (var * n) : (bound > open ? 0.0 : open + bound);
+        q = w * a.kl_coef * E / (var * n);
+      }
+      k *= E; q *= E;
+    }
+    if (tid == 0) {
+      a.row_out[0][i] = (float)logp;
+      if (a.logp_old) { a.row_out[1][i] = (float)ratio; a.row_out[2][i] = (float)kl; a.coef[i] = make_float2((float)k, (float)q); }
+    }
+  }
+  if (!a.loss) return;
+  if (tid == 0) {
+    __hip_atomic_store(&a.term[i], term, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const unsigned done = __hip_atomic_fetch_add(a.counter, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
+    last = done == (unsigned)rows - 1u;
+  }
+  __syncthreads();
+  if (!last) return;
+  double sum = 0.0;
+  for (int j = tid; j < rows; j += FT_THREADS) sum += __hip_atomic_load(&a.term[j], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  sum = block_sum(sum, red);
+  if (tid == 0) *a.loss = (float)sum;
+}
+
+// workgroups [0, spans): the gradient of the network's output; the ones behind them: one channel's logit each
+template <int MODE, bool MIX, bool REF, typename T>
+__global__ void __launch_bounds__(FT_THREADS) grad_kernel(FtArgs a, int spans) {
+  __shared__ float2 mix[FT_ROWS];
+  __shared__ double red[FT_THREADS / 64];
+  const int tid = threadIdx.x;
+  const float up = a.dloss ? *a.dloss : 1.f;
+  if ((int)blockIdx.x >= spans) {
+    const int ch = (int)blockIdx.x - spans, per = a.nseg * (a.log_g > 6 ? 1 << (a.log_g - 6) : 1);
+    double s = 0.0;
+    for (int64_t j = tid; j < (int64_t)a.B * per; j += FT_THREADS) {
+      const int b = (int)(j / per);
+      const float2 k = a.coef[b];
+      const double2 p = a.chan[((int64_t)b * a.C + ch) * per + (j - (int64_t)b * per)];
+      s += k.x * p.x + k.y * p.y;
+    }
+    s = block_sum(s, red);
+    if (tid == 0) {
+      const double c = 1.0 / (1.0 + exp(-(double)a.logit[ch]));
+      a.d_logit[ch] = (float)(s * c * (1.0 - c) * (double)up);
+    }
+    return;
+  }
+  const Span s = span_of(a, blockIdx.x);
+  const int G = 1 << a.log_g, lane = tid & (G - 1), group = tid >> a.log_g, ngroups = FT_THREADS >> a.log_g;
+  const bool used = takes_part<MODE>(a, s.b);
+  if (MIX && used) mix_rows(a, s, mix);
+  Elem e{a.s1 ? a.s1[s.b] : 0.f, 0.f, 1.f, 1.f, 0.f};
+  if (MODE == FT_POLICY) { e.A = a.transition[3 * (int64_t)s.b]; e.E = a.transition[3 * (int64_t)s.b + 1]; }
+  float2 k = a.coef[s.b];
+  k.x *= up; k.y *= up;
+  const int64_t sb = (int64_t)(s.b % a.second_rows) * a.C;
+  for (int r = group; r < s.rows; r += ngroups) {
+    if (MIX && used) { const float2 c = mix[r]; e.c = c.x; e.dc = c.y; }
+    const float kz = MIX ? k.x * e.c : k.x, kq = MIX ? k.y * e.c : k.y;
+    const int64_t base = ((int64_t)s.b * a.C + s.row0 + r) * a.T, base2 = (sb + s.row0 + r) * a.T;
+    const T* po = (const T*)a.out + base;
+    const T* pr = REF ? (const T*)a.ref + base : nullptr;
+    const float* px = (MIX || MODE == FT_POLICY) ? a.x + base : nullptr;
+    const float* py = a.second + base2;
+    T* pg = (T*)a.d_out + base;
+    const int64_t nvec = (s.t1 - s.t0) / 4, tail = s.t0 + 4 * nvec;
+#pragma unroll 2
+    for (int64_t v = lane; v < nvec; v += G) {
+      const int64_t t = s.t0 + 4 * v;
+      float g[4] = {0.f, 0.f, 0.f, 0.f};
+      if (used) {
+        float o[4], q[4] = {0.f, 0.f, 0.f, 0.f}, x[4] = {0.f, 0.f, 0.f, 0.f}, y[4];
+        load4(po + t, o);
+        if (REF) load4(pr + t, q);
+        if (MIX || MODE == FT_POLICY) load4(px + t, x);
+        load4(py + t, y);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float res, far, part;
+          element<MODE, MIX, REF>(e, o[i], q[i], x[i], y[i], res, far, part);
+          g[i] = REF ? fmaf(kq, far, kz * res) : kz * res;
+        }
+      }
+      store4(pg + t, g);
+    }
+    for (int64_t t = tail + lane; t < s.t1; t += G) {
+      float g = 0.f;
+      if (used) {
+        float res, far, part;
+        element<MODE, MIX, REF>(e, to_f32(po[t]), REF ? to_f32(pr[t]) : 0.f, (MIX || MODE == FT_POLICY) ? px[t] : 0.f, py[t], res, far, part);
+        g = REF ? fmaf(kq, far, kz * res) : kz * res;
+      }
+      pg[t] = from_f32<T>(g);
+    }
+  }
+}
+
+template <int MODE, bool MIX, bool REF>
+int launch_sums_t(const FtArgs& a, int dt, hipStream_t s) {
+  const dim3 grid((unsigned)(a.B * a.wps));
+  if (dt == DT_F32) hipLaunchKernelGGL((sums_kernel<MODE, MIX, REF, float>), grid, dim3(FT_THREADS), 0, s, a);
+  else hipLaunchKernelGGL((sums_kernel<MODE, MIX, REF, bf16_t>), grid, dim3(FT_THREADS), 0, s, a);
+  hipLaunchKernelGGL((rows_kernel<MODE>), dim3((unsigned)(MODE == FT_PREF ? a.pairs : a.B)), dim3(FT_THREADS), 0, s, a);
+  HIP_TRY(hipGetLastError());
+  return DDMI_OK;
+}
+template <int MODE, bool MIX, bool REF>
+int launch_grad_t(const FtArgs& a, int dt, hipStream_t s) {
+  const int spans = a.B * a.wps;
+  const dim3 grid((unsigned)(spans + (MIX && a.d_logit ? a.C : 0)));
+  if (dt == DT_F32) hipLaunchKernelGGL((grad_kernel<MODE, MIX, REF, float>), grid, dim3(FT_THREADS), 0, s, a, spans);
+  else hipLaunchKernelGGL((grad_kernel<MODE, MIX, REF, bf16_t>), grid, dim3(FT_THREADS), 0, s, a, spans);
+  HIP_TRY(hipGetLastError());
+  return DDMI_OK;
+}
+}  // namespace
+
+// Rows are split so that a workgroup has about 8 192 values (16 vectors of four a thread) where there are enough of them for 1 024
+// workgroups, fewer (down to 1 024) where there are not; G lanes share a row, as many as leave each at least two vectors of it.
+int ft_plan(FtArgs* a, int B, int C, int64_t HW, bool mixed) {
+  a->B = B;
+  a->C = mixed ? C : 1;                       // without a logit nothing depends on the channel: a sample is one row
+  a->T = mixed ? HW : HW * C;
+  const double all = (double)B * C * (double)HW;
+  int64_t want = 8192;
+  while (want > 1024 && all / (double)want < 1024.0) want >>= 1;
+  if (a->T > want) {
+    a->nseg = (int)std::min<int64_t>(cdiv64(a->T, want), 1 << 20);
+    a->seg = cdiv64(cdiv64(a->T, a->nseg), 4) * 4;
+    a->nseg = (int)cdiv64(a->T, a->seg);
+    a->rows_per_wg = 1;
+  } else {
+    a->nseg = 1;
+    a->seg = cdiv64(a->T, 4) * 4;
+    a->rows_per_wg = (int)std::min<int64_t>(std::min<int64_t>(FT_ROWS, a->C), std::max<int64_t>(1, want / a->T));
+  }
+  a->log_g = 0;
+  while (a->log_g < 8 && ((int64_t)16 << a->log_g) <= std::min(a->seg, a->T)) ++a->log_g;
+  const int64_t wps = cdiv64(a->C, a->rows_per_wg) * a->nseg;
+  if (wps * B > (1ll << 30) || (int64_t)B * a->C > (1ll << 40)) return ddmi_fail(DDMI_ERR_INVALID, "fine-tuning loss: too many values in one call");
+  a->wps = (int)wps;
+  return DDMI_OK;
+}
+static size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
+size_t ft_workspace_bytes(const FtArgs& a) {
+  const int wpg = a.log_g > 6 ? 1 << (a.log_g - 6) : 1;
+  return 256 + up256((size_t)a.B * sizeof(float2)) + up256((size_t)a.B * sizeof(double)) + up256((size_t)a.B * a.wps * sizeof(double2)) +
+         up256((size_t)a.B * a.C * a.nseg * wpg * sizeof(double2));
+}
+void ft_carve(FtArgs* a, void* ws) {
+  unsigned char* p = (unsigned char*)ws;
+  a->counter = (unsigned*)p; p += 256;
+  a->coef = (float2*)p; p += up256((size_t)a->B * sizeof(float2));
+  a->term = (double*)p; p += up256((size_t)a->B * sizeof(double));
+  a->part = (double2*)p; p += up256((size_t)a->B * a->wps * sizeof(double2));
+  a->chan = (double2*)p;
+}
+static double ft_bytes(const FtArgs& a, int mode, int dt, bool grad) {
+  const double n = (double)a.B * a.C * (double)a.T;
+  return n * (dt_size(dt) * (1.0 + (a.ref ? 1 : 0) * (!grad || mode == FT_POLICY ? 1 : 0) + (grad ? 1 : 0)) + (a.x ? 4.0 : 0.0) + 4.0 * a.second_rows / a.B);
+}
+int launch_ft_sums(const FtArgs& a, int mode, int dt, hipStream_t s) {
+  PROF_SCOPE(mode == FT_PREF ? "pref_loss" : "policy_loss", 0, ft_bytes(a, mode, dt, false), s);
+  if (mode == FT_PREF) return a.logit ? launch_sums_t<FT_PREF, true, true>(a, dt, s) : launch_sums_t<FT_PREF, false, true>(a, dt, s);
+  if (a.ref) return a.logit ? launch_sums_t<FT_POLICY, true, true>(a, dt, s) : launch_sums_t<FT_POLICY, false, true>(a, dt, s);
+  return a.logit ? launch_sums_t<FT_POLICY, true, false>(a, dt, s) : launch_sums_t<FT_POLICY, false, false>(a, dt, s);
+}
+// the preference gradient does not need the reference's output: its residual is the trained network's alone
+int launch_ft_grad(const FtArgs& a, int mode, int dt, hipStream_t s) {
+  PROF_SCOPE(mode == FT_PREF ? "pref_loss_bwd" : "policy_loss_bwd", 0, ft_bytes(a, mode, dt, true), s);
+  if (mode == FT_PREF) return a.logit ? launch_grad_t<FT_PREF, true, false>(a, dt, s) : launch_grad_t<FT_PREF, false, false>(a, dt, s);
+  if (a.ref) return a.logit ? launch_grad_t<FT_POLICY, true, true>(a, dt, s) : launch_grad_t<FT_POLICY, false, true>(a, dt, s);
+  return a.logit ? launch_grad_t<FT_POLICY, true, false>(a, dt, s) : launch_grad_t<FT_POLICY, false, false>(a, dt, s);
+}

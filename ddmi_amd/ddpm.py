@@ -162,6 +162,18 @@ class DDPM:
         k.sigma = float(sigma)
         return k
 
+    def transition_coefs(self, t: int, t_next: Optional[int] = None) -> Tuple[float, float, float]:
+        """(A, E, s) of the Gaussian step x_t -> x_prev as the samplers take it: mean A x_t + E eps, deviation s, eps the (mixed) prediction.
+        Ancestral (ddpm.py:248-255) without `t_next`, else the DDIM step t -> t_next (ddpm.py:353-369; t_next < 0: x_0, s = 0)."""
+        if self.clip_denoised:
+            raise ValueError("clip_denoised: x_0 is clipped on the way, the step's mean is not linear in the prediction")
+        k = self.ancestral_coefs(t) if t_next is None else (self._base_coefs(t) if t_next < 0 else self.ddim_coefs(t, t_next))
+        if t_next is None:
+            return k.coef1 * k.sqrt_recip_ac + k.coef2, -k.coef1 * k.sqrt_recipm1_ac, k.noise_scale
+        if t_next < 0:
+            return k.sqrt_recip_ac, -k.sqrt_recipm1_ac, 0.0
+        return k.sqrt_ac_next * k.sqrt_recip_ac, k.c_dir - k.sqrt_ac_next * k.sqrt_recipm1_ac, k.sigma
+
     # ---- fused step launcher ------------------------------------------------------------------------------------
     def _logit_ptr(self, device):
         import torch

@@ -1,0 +1,270 @@
+"""Losses that fine-tune a trained latent diffusion model, beside p_losses (`train.EpsLossFn`): from preferences - pairs of a preferred and
+a rejected latent against a frozen reference network - and from rewards - denoising transitions with advantages.
+
+    out = preference_loss(model_out, ref_out, x_t, noise, sqrt_1mac, beta=2000.0)
+    out.loss.backward()
+
+Both take the network outputs of the mixed prediction (get_mixed_prediction, diffusion/ddpm.py:469-477) and differentiate through it, to
+the output and to `mixing_logit`; every value is computed in libddmi_hip (include/ddmi_hip.h "Fine-tuning"), autograd only sequences
+forward and backward.  `train.LDMTrainStep.preference_step` / `.policy_step` are the training steps made of them.
+
+Tensors live on one GPU, samples along the first axis, channels along the second, anything behind them ([B, C, H, W] latents, [B, C, L]
+clips).  model_out and ref_out are both fp32 or both bf16, everything else is fp32; strides are free (a strided tensor is copied).  The
+calls enqueue work on the tensors' device's current stream and nothing else: no synchronisation, and a forward + backward can be captured
+in a hipGraph (the workspace is a torch tensor of the call, so graphs share none).
+"""
+from __future__ import annotations
+
+import ctypes as C
+from typing import NamedTuple, Optional
+
+import torch
+
+from . import _lib
+
+_OUT_TYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
+
+
+class PreferenceLoss(NamedTuple):
+    """loss: scalar, differentiable.  margin [pairs]: beta times the implicit reward of the preferred sample over the rejected one's
+    (> 0: ranked as preferred).  mse [2 pairs]: mean((prediction - noise)^2).  Both 0 where a pair is left out."""
+    loss: torch.Tensor
+    margin: torch.Tensor
+    mse: torch.Tensor
+
+
+class PolicyLoss(NamedTuple):
+    """loss: scalar, differentiable.  logp, ratio, kl [B]: per transition, 0 where it is left out."""
+    loss: torch.Tensor
+    logp: torch.Tensor
+    ratio: torch.Tensor
+    kl: torch.Tensor
+
+
+def _p(t: Optional[torch.Tensor]):
+    return None if t is None else t.data_ptr()
+
+
+def _expect(who, name, t, shape, dtype=torch.float32):
+    if not isinstance(t, torch.Tensor):
+        raise ValueError(f"{who}: {name} is a tensor, got {type(t).__name__}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{who}: {name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if t.dtype != dtype:
+        raise ValueError(f"{who}: {name} is {t.dtype}, expected {dtype}")
+
+
+def _check_outputs(who, model_out, ref_out, x_t, sqrt_1mac, mixing_logit, ref_mixing_logit):
+    if not isinstance(model_out, torch.Tensor) or model_out.dim() < 2 or model_out.numel() == 0:
+        raise ValueError(f"{who}: model_out is a non-empty [B, C, ...] tensor")
+    if model_out.dtype not in _OUT_TYPES:
+        raise ValueError(f"{who}: model_out is fp32 or bf16, got {model_out.dtype}")
+    shape = tuple(model_out.shape)
+    if ref_out is not None:
+        _expect(who, "ref_out", ref_out, shape, model_out.dtype)
+    _expect(who, "x_t", x_t, shape)
+    _expect(who, "sqrt_1mac", sqrt_1mac, shape[:1])
+    if mixing_logit is None:
+        if ref_mixing_logit is not None:
+            raise ValueError(f"{who}: ref_mixing_logit without mixing_logit")
+    else:
+        if ref_mixing_logit is None and ref_out is not None:
+            raise ValueError(f"{who}: mixing_logit needs ref_mixing_logit, the reference network's own (frozen) one")
+        for name, t in (("mixing_logit", mixing_logit), ("ref_mixing_logit", ref_mixing_logit)):
+            if t is not None and (t.dtype != torch.float32 or t.numel() != shape[1]):
+                raise ValueError(f"{who}: {name} holds {shape[1]} fp32 values, one a channel, got {tuple(t.shape)} {t.dtype}")
+
+
+def _check_constants(who, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.requires_grad:
+            raise ValueError(f"{who}: {name} requires a gradient, but only model_out and mixing_logit get one: detach it")
+
+
+def _check_device(who, *tensors):
+    dev = tensors[0].device
+    if dev.type != "cuda":
+        raise ValueError(f"{who}: tensors live on a GPU, got {dev}")
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise ValueError(f"{who}: all tensors live on one device, got {dev} and {t.device}")
+    return dev
+
+
+class _Call:
+    """The arguments of a loss's C entry points: contiguous tensors, kept alive, and the struct that points at them."""
+
+    def __init__(self, model_out, ref_out, x_t, second, sqrt_1mac, logit, ref_logit, weight):
+        flat = lambda t: None if t is None else t.detach().contiguous()      # noqa: E731
+        self.tensors = tuple(flat(t) for t in (model_out, ref_out, x_t, second, sqrt_1mac, logit, ref_logit, weight))
+        self.B, self.C = int(model_out.shape[0]), int(model_out.shape[1])
+        self.HW = model_out.numel() // (self.B * self.C)
+        self.out_dtype = _OUT_TYPES[model_out.dtype]
+
+    def struct(self):
+        return _lib.LossIn(*[_p(t) for t in self.tensors], self.HW, self.C, self.out_dtype)
+
+    def workspace(self):
+        n = C.c_size_t(0)
+        _lib.check(_lib.lib().ddmi_train_loss_workspace_bytes(self.B, self.C, self.HW, int(self.tensors[5] is not None), C.byref(n)))
+        return torch.empty(n.value, dtype=torch.uint8, device=self.tensors[0].device)
+
+
+def _begin(dev):
+    _lib.init_device(dev.index if dev.index is not None else torch.cuda.current_device())
+
+
+class PreferenceLossFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, model_out, mixing_logit, ref_out, x_t, noise, sqrt_1mac, ref_logit, weight, beta, label_smoothing):
+        call = _Call(model_out, ref_out, x_t, noise, sqrt_1mac, mixing_logit, ref_logit, weight)
+        dev, pairs = model_out.device, model_out.shape[0] // 2
+        ws = call.workspace()
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        margin = torch.empty((pairs,), dtype=torch.float32, device=dev)
+        mse = torch.empty((2 * pairs,), dtype=torch.float32, device=dev)
+        _lib.check(_lib.lib().ddmi_train_pref_loss(C.byref(call.struct()), pairs, noise.shape[0], beta, label_smoothing, ws.data_ptr(), ws.numel(),
+                                                   loss.data_ptr(), margin.data_ptr(), mse.data_ptr(), _lib.stream_ptr()))
+        # the gradient needs neither the reference's output nor its logit
+        call.tensors = (call.tensors[0], None) + call.tensors[2:6] + (None, call.tensors[7])
+        ctx.save_for_backward(ws, *call.tensors)
+        call.tensors = None
+        ctx.call, ctx.meta = call, (pairs, int(noise.shape[0]), beta, label_smoothing)
+        ctx.logit_shape = tuple(mixing_logit.shape) if mixing_logit is not None else None
+        ctx.mark_non_differentiable(margin, mse)
+        return loss, margin, mse
+
+    @staticmethod
+    def backward(ctx, g, _margin, _mse):
+        ws, call = ctx.saved_tensors[0], ctx.call
+        call.tensors = ctx.saved_tensors[1:]
+        d_out = torch.empty_like(call.tensors[0])
+        d_logit = torch.empty(ctx.logit_shape, dtype=torch.float32, device=ws.device) if ctx.logit_shape else None
+        pairs, noise_rows, beta, smoothing = ctx.meta
+        g = g.contiguous()
+        with torch.cuda.device(ws.device):
+            _lib.check(_lib.lib().ddmi_train_pref_loss_bwd(C.byref(call.struct()), pairs, noise_rows, beta, smoothing, ws.data_ptr(), ws.numel(),
+                                                           g.data_ptr(), d_out.data_ptr(), _p(d_logit), _lib.stream_ptr()))
+        call.tensors = None
+        return (d_out, d_logit) + (None,) * 8
+
+
+class PolicyLossFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, model_out, mixing_logit, ref_out, x_t, x_prev, sqrt_1mac, ref_logit, weight, transition, logp_old, advantage, clip_range,
+                kl_coef):
+        call = _Call(model_out, ref_out, x_t, x_prev, sqrt_1mac, mixing_logit, ref_logit, weight)
+        dev, B = model_out.device, model_out.shape[0]
+        ws, transition = call.workspace(), transition.contiguous()
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        logp, ratio, kl = torch.empty((3, B), dtype=torch.float32, device=dev).unbind(0)
+        logp_old, advantage = logp_old.contiguous(), advantage.contiguous()
+        _lib.check(_lib.lib().ddmi_train_policy_loss(C.byref(call.struct()), B, transition.data_ptr(), logp_old.data_ptr(), advantage.data_ptr(),
+                                                     clip_range, kl_coef, ws.data_ptr(), ws.numel(), loss.data_ptr(), logp.data_ptr(), ratio.data_ptr(),
+                                                     kl.data_ptr(), _lib.stream_ptr()))
+        ctx.save_for_backward(ws, transition, *call.tensors)
+        call.tensors = None
+        ctx.call = call
+        ctx.logit_shape = tuple(mixing_logit.shape) if mixing_logit is not None else None
+        ctx.mark_non_differentiable(logp, ratio, kl)
+        return loss, logp, ratio, kl
+
+    @staticmethod
+    def backward(ctx, g, *_stats):
+        ws, transition, call = ctx.saved_tensors[0], ctx.saved_tensors[1], ctx.call
+        call.tensors = ctx.saved_tensors[2:]
+        d_out = torch.empty_like(call.tensors[0])
+        d_logit = torch.empty(ctx.logit_shape, dtype=torch.float32, device=ws.device) if ctx.logit_shape else None
+        g = g.contiguous()
+        with torch.cuda.device(ws.device):
+            _lib.check(_lib.lib().ddmi_train_policy_loss_bwd(C.byref(call.struct()), call.B, transition.data_ptr(), ws.data_ptr(), ws.numel(),
+                                                             g.data_ptr(), d_out.data_ptr(), _p(d_logit), _lib.stream_ptr()))
+        call.tensors = None
+        return (d_out, d_logit) + (None,) * 11
+
+
+def preference_loss(model_out, ref_out, x_t, noise, sqrt_1mac, beta, mixing_logit=None, ref_mixing_logit=None, weight=None,
+                    label_smoothing=0.0) -> PreferenceLoss:
+    """The preference loss of `pairs` pairs: rows [0, pairs) of model_out, ref_out, x_t [2 pairs, C, ...] and sqrt_1mac [2 pairs] belong to
+    the preferred latents, rows [pairs, 2 pairs) to the rejected ones.
+
+        e      = mean((prediction - noise)^2) a sample
+        margin = -beta / 2 ((e - e_ref) of the preferred - (e - e_ref) of the rejected)
+        loss   = the weighted mean over the pairs of -(1 - label_smoothing) log sigma(margin) - label_smoothing log sigma(-margin)
+
+    noise: [2 pairs, C, ...], or [pairs, C, ...] where both samples of a pair got the same noise.  weight [pairs]: a pair whose weight is not
+    > 0 is left out - nothing of it is read (it may hold NaN), its gradient is zero.  Differentiable in model_out and mixing_logit."""
+    who = "preference_loss"
+    _check_outputs(who, model_out, ref_out, x_t, sqrt_1mac, mixing_logit, ref_mixing_logit)
+    if ref_out is None:
+        raise ValueError(f"{who}: ref_out is the reference network's output")
+    if model_out.shape[0] % 2:
+        raise ValueError(f"{who}: model_out holds pairs, got {model_out.shape[0]} samples")
+    pairs = model_out.shape[0] // 2
+    if not isinstance(noise, torch.Tensor) or noise.dim() < 1 or noise.shape[0] not in (pairs, 2 * pairs):
+        raise ValueError(f"{who}: noise has {pairs} (shared by a pair) or {2 * pairs} rows")
+    _expect(who, "noise", noise, (noise.shape[0],) + tuple(model_out.shape[1:]))
+    if weight is not None:
+        _expect(who, "weight", weight, (pairs,))
+    beta, label_smoothing = float(beta), float(label_smoothing)
+    if beta != beta or not 0.0 <= label_smoothing <= 1.0:
+        raise ValueError(f"{who}: beta is a number and label_smoothing in [0, 1], got {beta}, {label_smoothing}")
+    _check_constants(who, ref_out=ref_out, x_t=x_t, noise=noise, sqrt_1mac=sqrt_1mac, ref_mixing_logit=ref_mixing_logit, weight=weight)
+    dev = _check_device(who, model_out, ref_out, x_t, noise, sqrt_1mac, mixing_logit, ref_mixing_logit, weight)
+    with torch.cuda.device(dev):
+        _begin(dev)
+        return PreferenceLoss(*PreferenceLossFn.apply(model_out, mixing_logit, ref_out, x_t, noise, sqrt_1mac, ref_mixing_logit, weight, beta,
+                                                      label_smoothing))
+
+
+def _check_transition(who, model_out, x_prev, transition, weight, **rows):
+    B = model_out.shape[0]
+    _expect(who, "x_prev", x_prev, tuple(model_out.shape))
+    _expect(who, "transition", transition, (B, 3))
+    for name, t in dict(rows, weight=weight).items():
+        if t is not None or name != "weight":
+            _expect(who, name, t, (B,))
+
+
+def policy_loss(model_out, x_t, x_prev, transition, sqrt_1mac, logp_old, advantage, clip_range, ref_out=None, kl_coef=0.0, mixing_logit=None,
+                ref_mixing_logit=None, weight=None) -> PolicyLoss:
+    """The clipped policy loss of B denoising transitions x_t -> x_prev (both [B, C, ...]) that an earlier state of the network sampled.
+
+        mu    = A x_t + E prediction, deviation s, with transition [B, 3] = (A, E, s) (DDPM.transition_coefs)
+        logp  = mean over the values of log N(x_prev; mu, s^2),   ratio = exp(logp - logp_old)
+        kl    = mean((mu - mu_ref)^2) / (2 s^2)                   (0 without ref_out)
+        loss  = the weighted mean of max(-advantage ratio, -advantage clip(ratio, 1 - clip_range, 1 + clip_range)) + kl_coef kl
+
+    logp_old [B] is what `transition_log_prob` gave when the transition was sampled.  A transition with s = 0 (a chain's last step) has no
+    density and is left out, as is one whose weight [B] is not > 0.  Differentiable in model_out and mixing_logit."""
+    who = "policy_loss"
+    _check_outputs(who, model_out, ref_out, x_t, sqrt_1mac, mixing_logit, ref_mixing_logit)
+    _check_transition(who, model_out, x_prev, transition, weight, logp_old=logp_old, advantage=advantage)
+    clip_range, kl_coef = float(clip_range), float(kl_coef)
+    if not clip_range >= 0.0 or kl_coef != kl_coef:
+        raise ValueError(f"{who}: clip_range >= 0 and kl_coef a number, got {clip_range}, {kl_coef}")
+    if kl_coef != 0.0 and ref_out is None:
+        raise ValueError(f"{who}: kl_coef without ref_out, the reference network's output")
+    _check_constants(who, ref_out=ref_out, x_t=x_t, x_prev=x_prev, transition=transition, sqrt_1mac=sqrt_1mac, logp_old=logp_old, advantage=advantage,
+                     ref_mixing_logit=ref_mixing_logit, weight=weight)
+    dev = _check_device(who, model_out, ref_out, x_t, x_prev, transition, sqrt_1mac, logp_old, advantage, mixing_logit, ref_mixing_logit, weight)
+    with torch.cuda.device(dev):
+        _begin(dev)
+        return PolicyLoss(*PolicyLossFn.apply(model_out, mixing_logit, ref_out, x_t, x_prev, sqrt_1mac, ref_mixing_logit, weight, transition, logp_old,
+                                              advantage, clip_range, kl_coef))
+
+
+def transition_log_prob(model_out, x_t, x_prev, transition, sqrt_1mac, mixing_logit=None, weight=None) -> torch.Tensor:
+    """logp [B] of `policy_loss` alone (no gradient): what a rollout records as `logp_old`."""
+    who = "transition_log_prob"
+    _check_outputs(who, model_out, None, x_t, sqrt_1mac, mixing_logit, None)
+    _check_transition(who, model_out, x_prev, transition, weight)
+    dev = _check_device(who, model_out, x_t, x_prev, transition, sqrt_1mac, mixing_logit, weight)
+    with torch.cuda.device(dev):
+        _begin(dev)
+        call = _Call(model_out, None, x_t, x_prev, sqrt_1mac, mixing_logit, None, weight)
+        ws, transition = call.workspace(), transition.detach().contiguous()
+        logp = torch.empty((call.B,), dtype=torch.float32, device=dev)
+        _lib.check(_lib.lib().ddmi_train_policy_loss(C.byref(call.struct()), call.B, transition.data_ptr(), None, None, 0.0, 0.0, ws.data_ptr(), ws.numel(),
+                                                     None, logp.data_ptr(), None, None, _lib.stream_ptr()))
+        return logp

@@ -500,6 +500,67 @@ int ddmi_train_adamw(float* param, const float* grad, float* exp_avg, float* exp
 /* ema_pytorch's parameter average (tools/ldm/image.py:64, 174): ema += (param - ema) * (1 - decay) */
 int ddmi_train_ema(float* ema, const float* param, int64_t n, float decay, void* stream);
 
+/* ---------------------------------------------------------------------------------------------------------
+ * Fine-tuning: the losses that move a trained LDM towards preferences or rewards, and the optimizer step over separately allocated
+ * tensors.  They stand beside ddmi_train_eps_loss / ddmi_train_adamw; no handle: every buffer is the caller's, the losses' workspace
+ * included (ddmi_train_loss_workspace_bytes; 16-byte aligned, contents undefined before the forward call; the backward call of a loss
+ * takes the workspace its forward call filled, any number of times).  All of them only enqueue work: capturable.
+ *
+ * Per value of sample b, channel ch:  m = sqrt_1mac[b] x_t, c = sigmoid(mixing_logit[ch]), eps = m + c (model_out - m) - the mixed
+ * prediction of diffusion/ddpm.py:469-477; eps = model_out without logits.  Samples are [C, HW], contiguous.  Sums are held in fp64.
+ * --------------------------------------------------------------------------------------------------------- */
+enum { DDMI_DTYPE_F32 = 0, DDMI_DTYPE_BF16 = 1 };
+typedef struct {
+  const void* model_out;            /* [B, C, HW] of out_dtype */
+  const void* ref_out;              /* the frozen reference network's output, same shape and type; nullable for the policy loss */
+  const float* x_t;                 /* [B, C, HW] */
+  const float* second;              /* preference: the noise [noise_rows, C, HW]; policy: the chain's next state [B, C, HW] */
+  const float* sqrt_1mac;           /* [B] sqrt(1 - abar_t); read when mixing_logit is given */
+  const float* mixing_logit;        /* [C], nullable = no mixing */
+  const float* ref_mixing_logit;    /* [C], given with mixing_logit */
+  const float* weight;              /* a pair / transition, nullable = 1.  Where it is not > 0 the row is left out: nothing of it is read, its
+                                     * gradient is zero, and the mean is taken over the others (no row left: loss 0) */
+  int64_t HW;
+  int C, out_dtype;
+} ddmi_loss_in;
+int ddmi_train_loss_workspace_bytes(int B, int C, int64_t HW, int mixed, size_t* bytes);
+/* Preference loss over `pairs` pairs: samples [0, pairs) preferred, [pairs, 2 pairs) rejected (B = 2 pairs).  e = mean((eps - noise)^2),
+ * margin = -beta / 2 ((e - e_ref) of the preferred - that of the rejected), loss = weighted mean of
+ * -(1 - label_smoothing) log sigma(margin) - label_smoothing log sigma(-margin).  noise_rows: 2 pairs, or pairs when both samples of a
+ * pair got the same noise.  margin [pairs], mse [2 pairs] = e; 0 for pairs left out. */
+int ddmi_train_pref_loss(const ddmi_loss_in* in, int pairs, int noise_rows, double beta, double label_smoothing, void* ws, size_t ws_bytes, float* loss,
+                         float* margin, float* mse, void* stream);
+/* d_model_out [B, C, HW] of out_dtype, d_logit [C] (nullable), both times *dloss (a device scalar, nullable = 1) */
+int ddmi_train_pref_loss_bwd(const ddmi_loss_in* in, int pairs, int noise_rows, double beta, double label_smoothing, void* ws, size_t ws_bytes,
+                             const float* dloss, void* d_model_out, float* d_logit, void* stream);
+/* Clipped policy loss over B denoising transitions x_t -> second: mean mu = A x_t + E eps and deviation s with transition[b] = (A, E, s);
+ * logp = mean over the values of log N(second; mu, s^2), ratio = exp(logp - logp_old), kl = mean((mu - mu_ref)^2) / (2 s^2), loss =
+ * weighted mean of max(-advantage ratio, -advantage clip(ratio, 1 -+ clip_range)) + kl_coef kl.  A transition with s = 0 has no density
+ * and is left out like one of weight 0.  logp_old = NULL: logp alone is computed (a rollout records it), the other outputs are not
+ * touched.  logp, ratio, kl [B]; 0 for transitions left out. */
+int ddmi_train_policy_loss(const ddmi_loss_in* in, int B, const float* transition, const float* logp_old, const float* advantage, double clip_range,
+                           double kl_coef, void* ws, size_t ws_bytes, float* loss, float* logp, float* ratio, float* kl, void* stream);
+int ddmi_train_policy_loss_bwd(const ddmi_loss_in* in, int B, const float* transition, void* ws, size_t ws_bytes, const float* dloss, void* d_model_out,
+                               float* d_logit, void* stream);
+/* One tensor of an AdamW step.  Moments in 32 bits: exp_avg, exp_avg_sq fp32 [numel].  In 8 bits: e4m3 codes [numel] of the first moment
+ * and of the ROOT of the second, one fp32 power-of-two scale for each 256 values (exp_avg_scale, exp_avg_sq_scale [ceil(numel / 256)]). */
+typedef struct {
+  void* param;
+  const void* grad;
+  void* exp_avg;
+  void* exp_avg_sq;
+  float* exp_avg_scale;             /* 8-bit moments only */
+  float* exp_avg_sq_scale;
+  int64_t numel;                    /* 0: skipped */
+  int64_t step;                     /* this step's number, from 1 */
+  double lr, weight_decay;
+  int64_t index;                    /* the tensor's place in the caller's list: seeds its rounding */
+} ddmi_adamw_tensor;
+/* torch.optim.AdamW over n tensors (`tensors` is HOST memory, read before the call returns), grad multiplied by grad_scale first.  8-bit
+ * moments and bf16 parameters are rounded stochastically from (seed, step, index, place): the same call gives the same bits. */
+int ddmi_train_adamw_multi(const ddmi_adamw_tensor* tensors, int n, double beta1, double beta2, double eps, double grad_scale, uint32_t seed,
+                           int param_dtype, int grad_dtype, int state_bits, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

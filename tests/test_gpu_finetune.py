@@ -1,0 +1,410 @@
+"""The fine-tuning losses and AdamW over many tensors on the GPU, against 64-bit formulas with derived bounds (finetune_ref)."""
+import math
+
+import pytest
+import torch
+
+import finetune_ref as R
+from ddmi_amd.finetune import policy_loss, preference_loss, transition_log_prob
+from ddmi_amd.optim import AdamW, adamw_step, blocks_of
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+# (B, C, T): one value; odd planes; more rows than a workgroup holds; rows of one value; several segments a row; rows shared by four waves;
+# enough values for the largest workgroups
+SHAPES = [(2, 1, 1), (2, 64, 64), (6, 5, 7), (4, 3, 1), (2, 1100, 3), (2, 2, 20001), (6, 48, 1295), (4, 7, 4096), (2, 64, 65536)]
+
+
+def call(op, d, up=None):
+    d = dict(d)
+    out = d["model_out"] = d["model_out"].detach().clone().requires_grad_()
+    logit = d["mixing_logit"]
+    if logit is not None:
+        logit = d["mixing_logit"] = logit.detach().clone().requires_grad_()
+    r = (preference_loss if op == "pref" else policy_loss)(**d)
+    leaves = [out] + ([logit] if logit is not None else [])
+    g = torch.autograd.grad(r.loss if up is None else r.loss * up, leaves)
+    return dict(r._asdict(), d_model_out=g[0], d_logit=g[1].reshape(-1) if len(g) > 1 else None)
+
+
+def reference(op, d):
+    cpu = {k: t.cpu() if isinstance(t, torch.Tensor) else t for k, t in d.items()}
+    big = cpu["model_out"].numel() > 1 << 21
+    return (R.preference if op == "pref" else R.policy)(d if big else cpu)
+
+
+@pytest.mark.parametrize("B,C,T", SHAPES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("mixed", [True, False])
+def test_preference_loss(B, C, T, dtype, mixed):
+    d = R.make("pref", B, C, T, dtype, mixed, shared=T % 2 == 1, seed=B + C + T, device=DEV)
+    R.check(call("pref", d), reference("pref", d), (B, C, T))
+
+
+@pytest.mark.parametrize("B,C,T", SHAPES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("mixed,kl", [(True, True), (True, False), (False, True), (False, False)])
+def test_policy_loss(B, C, T, dtype, mixed, kl):
+    d = R.make("policy", B, C, T, dtype, mixed, kl=kl, seed=B + C + T, device=DEV)
+    R.check(call("policy", d), reference("policy", d), (B, C, T))
+    logp = transition_log_prob(d["model_out"], d["x_t"], d["x_prev"], d["transition"], d["sqrt_1mac"], d["mixing_logit"])
+    assert torch.equal(logp, call("policy", d)["logp"])
+
+
+@pytest.mark.parametrize("op", ["pref", "policy"])
+@pytest.mark.parametrize("weight", ["some", "none_left"])
+@pytest.mark.parametrize("mixed", [True, False])
+def test_rows_left_out(op, weight, mixed):
+    """Rows of weight 0 hold NaN and infinities: none of it may show, their gradients are zeros, and the mean is over the others."""
+    d = R.make(op, 14, 5, 33, weight=weight, mixed=mixed, seed=3, device=DEV)
+    got = call(op, d)
+    R.check(got, reference(op, d), weight)
+    gone = d["weight"] == 0
+    gone = torch.cat([gone, gone]) if op == "pref" else gone
+    assert not got["d_model_out"][gone].any()
+    if weight == "none_left":
+        assert float(got["loss"]) == 0.0
+
+
+def test_transition_without_noise_is_left_out():
+    d = R.make("policy", 6, 4, 9, seed=5, device=DEV)
+    d["transition"][2, 2] = 0.0
+    got = call("policy", d)
+    R.check(got, reference("policy", d))
+    assert float(got["logp"][2]) == 0.0 and not got["d_model_out"][2].any()
+
+
+@pytest.mark.parametrize("op", ["pref", "policy"])
+def test_nan_in_a_row_that_takes_part_shows(op):
+    d = R.make(op, 6, 4, 9, seed=5, device=DEV)
+    d["model_out"][1, 2, 3] = float("nan")
+    got = call(op, d)
+    assert math.isnan(float(got["loss"]))
+    assert torch.isfinite(got["d_model_out"][[2, 5]]).all()           # rows of other pairs keep theirs
+
+
+@pytest.mark.parametrize("op", ["pref", "policy"])
+def test_strided_and_offset_inputs(op):
+    d = R.make(op, 6, 5, 31, torch.bfloat16, seed=9, device=DEV)
+    want = call(op, d)
+    odd = {}
+    for k, t in d.items():
+        if isinstance(t, torch.Tensor) and t.dim() == 3:
+            t = t.transpose(1, 2).contiguous().transpose(1, 2) if k == "x_t" else torch.cat([t.reshape(-1)[:1], t.reshape(-1)])[1:].view(t.shape)
+        elif isinstance(t, torch.Tensor) and t.dim() == 1:
+            t = torch.stack([t, t], 1)[:, 0]
+        odd[k] = t
+    got = call(op, odd)
+    for k in want:
+        assert torch.equal(want[k], got[k]), k
+
+
+@pytest.mark.parametrize("op", ["pref", "policy"])
+def test_image_shaped_and_plain_vectors(op):
+    """[B, C, H, W] is [B, C, H W]; [B, C] is [B, C, 1]."""
+    d = R.make(op, 4, 6, 12, seed=2, device=DEV)
+    shaped = {k: (t.reshape(t.shape[0], 6, 3, 4) if isinstance(t, torch.Tensor) and t.dim() == 3 and "logit" not in k else t) for k, t in d.items()}
+    a, b = call(op, d), call(op, shaped)
+    assert torch.equal(a["loss"], b["loss"]) and torch.equal(a["d_model_out"].reshape(-1), b["d_model_out"].reshape(-1))
+    d = R.make(op, 4, 6, 1, seed=2, device=DEV)
+    flat = {k: (t.reshape(t.shape[0], 6) if isinstance(t, torch.Tensor) and t.dim() == 3 and "logit" not in k else t) for k, t in d.items()}
+    assert torch.equal(call(op, d)["loss"], call(op, flat)["loss"])
+
+
+@pytest.mark.parametrize("op", ["pref", "policy"])
+def test_gradient_against_differences(op):
+    """(loss(x + s v) - loss(x - s v)) / 2 s along a random direction v.  The losses carry rounding errors within their own bounds; the
+    difference's curvature is measured by halving s (its error is of second order: a third of the change)."""
+    d = R.make(op, 4, 5, 37, seed=21, device=DEV)
+    got = call(op, d)
+    v = torch.randn(d["model_out"].shape, generator=torch.Generator().manual_seed(1)).to(DEV)
+    vl = torch.randn(d["mixing_logit"].shape, generator=torch.Generator().manual_seed(2)).to(DEV)
+    want = float((got["d_model_out"].double() * v).sum() + (got["d_logit"].double() * vl.reshape(-1)).sum())
+
+    def loss(s):
+        e = dict(d, model_out=d["model_out"] + s * v, mixing_logit=d["mixing_logit"] + s * vl)
+        return float((preference_loss if op == "pref" else policy_loss)(**e).loss)
+
+    s = 2.0 ** -9
+    wide, near = (loss(2 * s) - loss(-2 * s)) / (4 * s), (loss(s) - loss(-s)) / (2 * s)
+    e_loss = float(reference(op, d)["loss"][1]) * 4 / s + abs(float(got["loss"])) * 4 * R.U / s
+    # the shifted inputs are rounded too: half a step of values up to 8, along the gradient
+    e_in = float(got["d_model_out"].double().abs().sum()) * 8 * R.U * 2 / s
+    assert abs(near - want) <= abs(wide - near) + e_loss + e_in, (near, want)
+
+
+@pytest.mark.parametrize("op", ["pref", "policy"])
+def test_upstream_gradient_and_second_backward(op):
+    d = R.make(op, 6, 5, 33, seed=4, device=DEV)
+    one, three = call(op, d), call(op, d, 4.0)
+    assert torch.equal(one["d_model_out"] * 4, three["d_model_out"]) and torch.equal(one["d_logit"] * 4, three["d_logit"])
+    out = d["model_out"].clone().requires_grad_()
+    r = (preference_loss if op == "pref" else policy_loss)(**dict(d, model_out=out))
+    first = torch.autograd.grad(r.loss, out, retain_graph=True)[0].clone()
+    first.mul_(0)                                                       # what a caller does with its gradient does not reach the next one
+    assert torch.equal(torch.autograd.grad(r.loss, out)[0], one["d_model_out"])
+    with torch.no_grad():
+        assert torch.equal((preference_loss if op == "pref" else policy_loss)(**d).loss, one["loss"])
+
+
+@pytest.mark.parametrize("op", ["pref", "policy"])
+def test_same_bits_on_every_run_and_stream(op):
+    d = R.make(op, 8, 16, 1025, seed=6, device=DEV)
+    a = call(op, d)
+    other = torch.cuda.Stream()
+    other.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(other):
+        b = call(op, d)
+    c = call(op, d)
+    torch.cuda.synchronize()
+    for k in a:
+        assert torch.equal(a[k], b[k]) and torch.equal(a[k], c[k]), k
+
+
+@pytest.mark.parametrize("op", ["pref", "policy"])
+def test_captured_and_replayed(op):
+    """Two captured forwards + backwards of different inputs, replayed by turns with eager work between: each replay is the eager result."""
+    sets = [R.make(op, 6, 7, 131, seed=s, device=DEV) for s in (1, 2, 3, 4)]
+    want = [call(op, d) for d in sets]
+    static = [{k: t.clone() if isinstance(t, torch.Tensor) else t for k, t in sets[i].items()} for i in (0, 1)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for d in static:
+            call(op, d)
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graphs = []
+    for d in static:
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            out = call(op, d)
+        graphs.append((g, out))
+    for i in (0, 1, 2, 3, 1, 0):
+        for j in (0, 1):
+            src = sets[(i + j) % 4]
+            for k, t in static[j].items():
+                if isinstance(t, torch.Tensor):
+                    t.copy_(src[k])
+            graphs[j][0].replay()
+        call(op, sets[(i + 2) % 4])
+        torch.cuda.synchronize()
+        for j in (0, 1):
+            for k in want[0]:
+                assert torch.equal(graphs[j][1][k], want[(i + j) % 4][k]), (i, j, k)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# AdamW
+# ---------------------------------------------------------------------------------------------------------------------
+def lists(shapes, p_type, g_type, bits, seed, offset=0):
+    """Parameters, gradients and moments; `offset`: places that their storage starts off an aligned address."""
+    g = torch.Generator().manual_seed(seed)
+
+    def place(t):
+        return torch.cat([t.reshape(-1)[:1]] * offset + [t.reshape(-1)])[offset:].view(t.shape).to(DEV) if not offset else \
+            torch.cat([torch.zeros(offset, dtype=t.dtype), t.reshape(-1)]).to(DEV)[offset:].view(t.shape)
+
+    p = [place(torch.randn(s, generator=g).to(p_type)) for s in shapes]
+    gr = [place((0.1 * torch.randn(s, generator=g)).to(g_type)) for s in shapes]
+    if bits == 32:
+        return p, gr, [place(0.02 * torch.randn(s, generator=g)) for s in shapes], [place((0.1 * torch.randn(s, generator=g)) ** 2) for s in shapes], {}
+    sizes = [math.prod(s) for s in shapes]
+    codes = lambda lo, hi, n: torch.randint(lo, hi, (n,), generator=g, dtype=torch.uint8)      # noqa: E731
+    m = [place(codes(0, 0x70, n) | (codes(0, 2, n) << 7)).view(torch.float8_e4m3fn) for n in sizes]
+    v = [place(codes(0x20, 0x70, n)).view(torch.float8_e4m3fn) for n in sizes]
+    scale = lambda n: torch.exp2(torch.randint(-16, -12, (blocks_of(n),), generator=g).float()).to(DEV)      # noqa: E731
+    return p, gr, m, v, {"exp_avg_scales": [scale(n) for n in sizes], "exp_avg_sq_scales": [scale(n) for n in sizes]}
+
+
+ADAM_SHAPES = [[(1,)], [(255,), (256,), (257,)], [(3, 5, 7), (1025,), (4096,), (4097,), (2, 3)], [(k % 37 + 1,) for k in range(130)], [(3, 70001)]]
+
+
+def bits_of(t):
+    return t.view(torch.uint8) if t.dtype == torch.float8_e4m3fn else t
+
+
+@pytest.mark.parametrize("shapes", ADAM_SHAPES, ids=["one", "ends", "mixed", "many", "long"])
+@pytest.mark.parametrize("p_type,g_type", [(torch.float32, torch.float32), (torch.float32, torch.bfloat16), (torch.bfloat16, torch.float32),
+                                           (torch.bfloat16, torch.bfloat16)])
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("offset", [0, 1])
+def test_adamw_step(shapes, p_type, g_type, bits, offset):
+    p, g, m, v, scales = lists(shapes, p_type, g_type, bits, 7, offset)
+    hyper = dict(lr=2e-3, betas=(0.9, 0.99), eps=1e-7, weight_decay=0.1, grad_scale=0.5)
+    step, seed = 3, 1234
+    before = [[t.detach().clone() for t in ts] for ts in (p, g, m, v)]
+    old = {k: [t.clone() for t in ts] for k, ts in scales.items()}
+    adamw_step(p, g, m, v, step, seed=seed, **hyper, **scales)
+    for i in range(len(shapes)):
+        n = p[i].numel()
+        pb, gb, mb, vb = (ts[i].reshape(-1).cpu() for ts in before)
+        assert torch.equal(g[i].cpu().reshape(-1), gb)
+        mb, vb = mb.float().double(), vb.float().double()
+        if bits == 8:
+            mb = mb * old["exp_avg_scales"][i].cpu().double().repeat_interleave(256)[:n]
+            vb = (vb * old["exp_avg_sq_scales"][i].cpu().double().repeat_interleave(256)[:n]) ** 2
+        want = R.adamw(pb.double(), gb.double(), mb, vb, step, **hyper)
+        rnd = R.random_bits(n, seed, step, i)
+        p1, e_p = want["p"]
+        got = p[i].cpu().double().reshape(-1)
+        if p_type == torch.float32:
+            assert ((got - p1).abs() <= e_p + R.U * p1.abs()).all()
+        else:                                     # up with the probability of what is cut off: 16 random bits
+            unit = torch.exp2(torch.frexp(p1)[1].double() - 8)
+            cut = (R.mix32(rnd ^ 0x68E31DA4) & 0xFFFF).double() * 2.0 ** -16 * unit
+            lo, hi = ((p1.abs() + s * e_p).div(unit).add(cut / unit).floor() * unit for s in (-1, 1))
+            # a value whose error reaches into the next binade has another unit there: within that error of either rounding
+            assert ((got.abs() >= lo - e_p) & (got.abs() <= hi + e_p) & (got.sign() * p1.sign() >= 0)).all()
+        if bits == 32:
+            for k, t in (("m", m), ("v", v)):
+                w, e = want[k]
+                assert ((t[i].cpu().double().reshape(-1) - w).abs() <= e + R.U * w.abs()).all(), k
+            continue
+        for k, t, name, r, root in (("m", m, "exp_avg_scales", ((rnd & 0xFFF) << 8) | 0x80, False), ("root", v, "exp_avg_sq_scales", rnd >> 12, True)):
+            w, e = want[k]
+            s = scales[name][i].cpu().double()
+            # the block's largest value, in 32 bits, is within its error of the one in 64: next to a power of two it may lie on the other
+            # side (sqrt(0.01 (0.5 * 0.3125)^2 + 1e-11) is 2^-6 (1 + 2.6e-8), less than half a step of fp32 above 2^-6)
+            assert ((s >= R.block_scales((w.abs() - e).clamp_min(0))) & (s <= R.block_scales(w.abs() + e))).all(), name
+            lo, hi = R.codes_allowed(w, e, s, r, root)
+            code = t[i].cpu().float().double().reshape(-1)
+            assert ((code.abs() >= lo) & (code.abs() <= hi)).all(), k
+            assert float((lo != hi).double().mean()) < 0.01          # the allowance is the exception
+            assert ((code * w >= 0) | (code == 0)).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_is_reproducible_and_independent_of_the_list(bits):
+    """Twice the same bits, on another stream too; a tensor's result depends on its own place in the list, not on its neighbours."""
+    shapes = [(40, 70), (9,), (1000,)]
+    results = []
+    for k in range(3):
+        p, g, m, v, scales = lists(shapes, torch.bfloat16, torch.float32, bits, 5)
+        st = torch.cuda.Stream() if k == 1 else torch.cuda.current_stream()
+        st.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(st):
+            if k == 2:        # the same places, other neighbours
+                p[1], g[1] = p[1] * 3, g[1] * 5
+            adamw_step(p, g, m, v, [2, 2, 9], lr=[1e-3, 1e-2, 1e-4], weight_decay=[0.0, 0.1, 0.2], seed=3, **scales)
+        torch.cuda.synchronize()
+        results.append((p, m, v, *scales.values()))
+    for ts in zip(*results):
+        for i in range(3):
+            assert torch.equal(bits_of(ts[0][i]), bits_of(ts[1][i]))
+            if i != 1:
+                assert torch.equal(bits_of(ts[0][i]), bits_of(ts[2][i]))
+
+
+def test_adamw_writes_nothing_behind_a_tensor():
+    n = 300
+    slab = {k: torch.full((4096,), 77, dtype=torch.uint8, device=DEV) for k in ("p", "m", "v")}
+    sc = [torch.full((8,), 3.0, device=DEV) for _ in range(2)]
+    p = slab["p"][:4 * n].view(torch.float32)
+    p.fill_(1.0)
+    m, v = (slab[k][:n].view(torch.float8_e4m3fn) for k in "mv")
+    adamw_step([p], [torch.ones(n, device=DEV)], [m], [v], 1, lr=0.1, exp_avg_scales=[sc[0][:2]], exp_avg_sq_scales=[sc[1][:2]])
+    assert (slab["p"][4 * n:] == 77).all() and (slab["m"][n:] == 77).all() and (slab["v"][n:] == 77).all()
+    assert (sc[0][2:] == 3).all() and (sc[1][2:] == 3).all() and (sc[0][:2] != 3).all()
+
+
+def test_adamw_refuses_shared_memory_and_captures():
+    p = [torch.zeros(8, device=DEV)]
+    s = lambda: [torch.zeros(8, device=DEV), torch.zeros(8, device=DEV)]      # noqa: E731
+    with pytest.raises(ValueError, match="share memory"):
+        adamw_step(p * 2, s(), s(), s(), 1, lr=0.1)
+    big = torch.zeros(12, device=DEV)
+    with pytest.raises(ValueError, match="share memory"):
+        adamw_step([big[:8], big[4:]], s(), s(), s(), 1, lr=0.1)
+    g, a, b = s()[:1], s()[:1], s()[:1]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(RuntimeError, match="graph capture"):
+            adamw_step(p, g, a, b, 1, lr=0.1)
+        big.add_(1)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert not p[0].any()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_nan_gradient_stays_with_its_value(bits):
+    p, g, m, v, scales = lists([(600,)], torch.float32, torch.float32, bits, 5)
+    clean = lists([(600,)], torch.float32, torch.float32, bits, 5)
+    g[0][300], g[0][301] = float("nan"), float("inf")
+    adamw_step(p, g, m, v, 2, lr=1e-3, **scales)
+    adamw_step(*clean[:4], 2, lr=1e-3, **clean[4])
+    other = torch.ones(600, dtype=torch.bool, device=DEV)
+    other[300:302] = False
+    assert torch.isnan(p[0][~other]).all() and torch.equal(p[0][other], clean[0][0][other])
+    assert torch.isnan(m[0].float()[300]) and not torch.isfinite(m[0].float()[301])
+    if bits == 32:
+        assert torch.equal(m[0][other], clean[2][0][other])
+    else:                # the block's scale is that of its finite values; the outliers were not its largest before
+        far = other.clone()
+        far[256:512] = False
+        assert torch.equal(bits_of(m[0])[far], bits_of(clean[2][0])[far])
+        assert torch.isfinite(m[0].float()[other]).all()
+
+
+def test_rounding_of_8_bit_moments_is_unbiased():
+    """Over 4096 equal values the mean of a moment is its exact value within six standard deviations of a rounding (of at most a step's
+    half each, independent): round-to-nearest would leave every one where it is."""
+    n = 4096
+    p, g = [torch.zeros(n, device=DEV)], [torch.full((n,), 1.0, device=DEV)]
+    m, v = ([torch.full((n,), c, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn)] for c in (0x70, 0x70))      # 128
+    scales = [[torch.full((16,), 2.0 ** -7, device=DEV)] for _ in range(2)]                                                  # the value is 1
+    g[0].fill_(1.1)
+    adamw_step(p, g, m, v, 5, lr=1e-3, betas=(0.9, 0.999), exp_avg_scales=scales[0], exp_avg_sq_scales=scales[1])
+    for codes, scale, want in ((m, scales[0], 0.9 + 0.1 * 1.1), (v, scales[1], math.sqrt(0.999 + 0.001 * 1.21))):
+        val = codes[0].float() * scale[0].repeat_interleave(256)
+        step = 2.0 ** -3
+        assert len(set(val.tolist())) == 2
+        assert abs(float(val.double().mean()) - want) <= 6 * 0.5 * step / math.sqrt(n) + step * 2.0 ** -12, (float(val.mean()), want)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_class_steps_groups_and_checkpoints(bits):
+    g = torch.Generator().manual_seed(2)
+    make = lambda: [torch.nn.Parameter(torch.randn(s, generator=g.manual_seed(2)).to(DEV)) for s in ((33, 9), (300,), (5,))]      # noqa: E731
+    ps, qs = make(), make()
+    groups = lambda v: [{"params": v[:2], "weight_decay": 0.1}, {"params": v[2:], "lr": 1e-2}]      # noqa: E731
+    a, b = AdamW(groups(ps), lr=1e-3, state_bits=bits, seed=9), AdamW(groups(qs), lr=1e-3, state_bits=bits, seed=9)
+    t = torch.optim.AdamW([{"params": [p.detach().clone().requires_grad_() for p in v["params"]], **{k: x for k, x in v.items() if k != "params"}}
+                           for v in groups(ps)], lr=1e-3, weight_decay=0.0)
+    tp = [p for gr in t.param_groups for p in gr["params"]]
+    for k in range(4):
+        for p, q in zip(ps, tp):
+            grad = torch.randn(p.shape, generator=g).to(DEV)
+            p.grad, q.grad = grad, grad.clone()
+        if k == 2:
+            ps[1].grad = tp[1].grad = None        # sits this step out
+        a.step()
+        t.step()
+        if k == 1:
+            sd = a.state_dict()
+            for p, q in zip(ps, qs):
+                q.data.copy_(p.data)
+            b.load_state_dict(sd)
+        elif k > 1:
+            for p, q in zip(ps, qs):
+                q.grad = p.grad
+            b.step()
+    assert a.steps == [4, 3, 4] == b.steps
+    for p, q in zip(ps, qs):
+        assert torch.equal(p, q)                  # resumed from the state dict: the same bits
+    if bits == 32:
+        t2 = torch.optim.AdamW([{"params": [x]} for x in tp])
+        for p, q in zip(ps, tp):                  # four steps of at most lr each; both in 32 bits
+            assert float((p - q).abs().max()) <= 4 * (1e-2 * 40 + 8) * R.U * float(1 + p.abs().max())
+        del t2
+        for i, st in a.state_dict()["state"].items():
+            ref = t.state[tp[i]]
+            assert float(st["step"]) == float(ref["step"])
+            assert torch.allclose(st["exp_avg"], ref["exp_avg"], rtol=32 * R.U, atol=32 * R.U)
+            assert torch.allclose(st["exp_avg_sq"], ref["exp_avg_sq"], rtol=64 * R.U, atol=0)
+    a.zero_grad(set_to_none=True)
+    assert all(p.grad is None for p in ps)
+    before = [p.detach().clone() for p in ps]
+    a.step()
+    assert all(torch.equal(x, p) for x, p in zip(before, ps)) and a.steps == [4, 3, 4]
