@@ -101,21 +101,17 @@ __device__ __forceinline__ void decode(unsigned c, float scale, float (&v)[4]) {
   const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, true);
   v[0] = lo.x * scale; v[1] = lo.y * scale; v[2] = hi.x * scale; v[3] = hi.y * scale;
 }
-// e4m3 of x (|x| <= 256 or not finite), rounded up in magnitude when the 20 random bits r reach the part that is cut off
-template <bool ROOT> __device__ __forceinline__ unsigned encode(float x, unsigned r) {
-  const unsigned bits = __float_as_uint(x) & 0x7FFFFFFFu;
-  const float a = __uint_as_float(bits);
-  const unsigned normal = ((bits + r) >> 20) - (120u << 3);                  // exponent and three fraction bits; a carry moves on to the next binade
-  const unsigned small = (unsigned)(int)floorf(a * 512.0f + (float)r * 0x1p-20f);
-  unsigned code = a < 0x1p-6f ? small : normal;
-  if (bits >= 0x7F800000u) code = 0x7Fu;                                      // NaN and infinity: the code's NaN
-  if (ROOT) return (bits != 0u && code == 0u) ? 1u : code;
-  return code | ((__float_as_uint(x) >> 24) & 0x80u);
+// the largest of a wave's 64 values of v, as bits; the lane shifts need no LDS
+template <int CTRL> __device__ __forceinline__ unsigned max_with(unsigned x) {
+  return max(x, (unsigned)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xF, 0xF, false));
 }
-// the largest of a wave's 64 non-negative integers, in every lane
-__device__ __forceinline__ unsigned wave_max(unsigned x) {
-  for (int st = 32; st > 0; st >>= 1) x = max(x, (unsigned)__shfl_xor((int)x, st));
-  return x;
+// (two at a time: a lane shift waits for the instruction before it)
+__device__ __forceinline__ void wave_max(unsigned& x, unsigned& y) {
+  x = max_with<0x111>(x); y = max_with<0x111>(y); x = max_with<0x112>(x); y = max_with<0x112>(y);      // within a row of 16 lanes
+  x = max_with<0x114>(x); y = max_with<0x114>(y); x = max_with<0x118>(x); y = max_with<0x118>(y);
+  x = max_with<0x142>(x); y = max_with<0x142>(y); x = max_with<0x143>(x); y = max_with<0x143>(y);      // over the rows
+  x = (unsigned)__builtin_amdgcn_readlane((int)x, 63);
+  y = (unsigned)__builtin_amdgcn_readlane((int)y, 63);
 }
 // 2^k that puts `most` (bits of a finite non-negative float) into (128, 256], and 2^-k
 __device__ __forceinline__ void block_scale(unsigned most, float& scale, float& inv) {
@@ -124,7 +120,110 @@ __device__ __forceinline__ void block_scale(unsigned most, float& scale, float& 
   scale = __uint_as_float((unsigned)(k + 127) << 23);
   inv = __uint_as_float((unsigned)(127 - k) << 23);
 }
+// Four e4m3 codes.  v_cvt_sr_fp8_f32 adds the upper 20 of its 32 random bits to what is cut off below the three fraction bits (a
+// subnormal: below 2^-9) and truncates: up with the probability of the cut-off part.  The first moment takes the 12 low bits of a value's
+// random word (centred), the root the 20 high ones.  NaN becomes the code's NaN; an infinity is not given to it.
+template <bool ROOT> __device__ __forceinline__ unsigned encode4(const float (&x)[4], float inv, const unsigned (&rnd)[4]) {
+  float y[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    y[i] = x[i] * inv;
+    if (ROOT) y[i] = y[i] > 0.f ? fmaxf(y[i], 0x1p-9f) : y[i];            // no root but zero becomes zero: at least the least code
+  }
+  int c = 0;
+  c = __builtin_amdgcn_cvt_sr_fp8_f32(y[0], (int)(ROOT ? rnd[0] : (rnd[0] << 20) | 0x80000u), c, 0);
+  c = __builtin_amdgcn_cvt_sr_fp8_f32(y[1], (int)(ROOT ? rnd[1] : (rnd[1] << 20) | 0x80000u), c, 1);
+  c = __builtin_amdgcn_cvt_sr_fp8_f32(y[2], (int)(ROOT ? rnd[2] : (rnd[2] << 20) | 0x80000u), c, 2);
+  c = __builtin_amdgcn_cvt_sr_fp8_f32(y[3], (int)(ROOT ? rnd[3] : (rnd[3] << 20) | 0x80000u), c, 3);
+  return (unsigned)c;
+}
 
+// One step of four values.  v: the second moment, or its root (8 bits).  The root is correctly rounded - r = x - s^2 is exact in an FMA, so
+// one correction of s = x rsq(x) is enough (checked on every fraction) - at half the instructions of sqrtf; the quotient by the hardware's
+// reciprocal is within 1.5 ulp, of a change that is a small part of the parameter.
+template <int BITS>
+__device__ __forceinline__ void step4(const AdArgs& a, const AdTensor& t, float (&p)[4], const float (&g)[4], float (&m)[4], float (&v)[4],
+                                      float (&root)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float gi = g[i] * a.gscale;
+    const float vo = BITS == 8 ? v[i] * v[i] : v[i];
+    m[i] = m[i] * a.b1 + gi * a.omb1;
+    v[i] = vo * a.b2 + (gi * a.omb2) * gi;
+    const float y = __builtin_amdgcn_rsqf(v[i]), s = v[i] * y;
+    root[i] = fmaf(fmaf(-s, s, v[i]), 0.5f * y, s);
+  }
+  const float least = fminf(fminf(v[0], v[1]), fminf(v[2], v[3])), most = fmaxf(fmaxf(v[0], v[1]), fmaxf(v[2], v[3]));
+  if (!(least >= 0x1p-90f && most < 0x1p126f)) {                            // zero, next to it, or not finite
+#pragma unroll
+    for (int i = 0; i < 4; ++i) root[i] = sqrtf(v[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) p[i] = p[i] * t.decay - (m[i] * __builtin_amdgcn_rcpf(root[i] * t.inv_bc2 + a.eps)) * t.size;
+}
+__device__ __forceinline__ void random4(unsigned key, int64_t blk, int lane, unsigned (&rnd)[4]) {
+  const unsigned kb = mix32(key + (unsigned)blk * 0x9E3779B9u);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) rnd[i] = mix32(kb + (unsigned)(4 * lane + i) * 0x9E3779B9u);
+}
+__device__ __forceinline__ void round_bf16(const float (&p)[4], const unsigned (&rnd)[4], unsigned short (&w)[4]) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const unsigned bits = __float_as_uint(p[i]);
+    const bool finite = (bits & 0x7FFFFFFFu) < 0x7F800000u;
+    w[i] = (unsigned short)((finite ? bits + (mix32(rnd[i] ^ 0x68E31DA4u) & 0xFFFFu) : (p[i] != p[i] ? 0x7FC00000u : bits)) >> 16);
+  }
+}
+// what is left to do of one block when its values are there: `left` (0..4) of the lane's four exist
+template <typename PT, int BITS>
+__device__ __forceinline__ void finish_block(const AdArgs& a, const AdTensor& t, int64_t blk, int lane, int left, float (&p)[4], const float (&g)[4],
+                                             float (&m)[4], float (&v)[4]) {
+  const int64_t at = blk * ADAMW_BLOCK + 4 * lane;
+  unsigned rnd[4] = {0u, 0u, 0u, 0u};
+  float root[4];
+  if (BITS == 8 || sizeof(PT) == 2) random4(t.key, blk, lane, rnd);
+  step4<BITS>(a, t, p, g, m, v, root);
+  if (left > 0) {
+    if constexpr (sizeof(PT) == 4) store((float*)t.p, at, left, p);
+    else {
+      unsigned short w[4];
+      round_bf16(p, rnd, w);
+      store((bf16_t*)t.p, at, left, w);
+    }
+  }
+  if constexpr (BITS == 32) {
+    if (left > 0) {
+      store((float*)t.m, at, left, m);
+      store((float*)t.v, at, left, v);
+    }
+  } else {
+    unsigned mm = 0u, mv = 0u;                                                // values that do not exist are zeros
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { mm = max(mm, __float_as_uint(m[i]) & 0x7FFFFFFFu); mv = max(mv, __float_as_uint(root[i]) & 0x7FFFFFFFu); }
+    wave_max(mm, mv);
+    if (mm >= 0x7F800000u || mv >= 0x7F800000u) {                             // the same in every lane: the scale is that of the finite values, the others are NaN
+      mm = mv = 0u;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const unsigned bm = __float_as_uint(m[i]) & 0x7FFFFFFFu, bv = __float_as_uint(root[i]) & 0x7FFFFFFFu;
+        if (bm < 0x7F800000u) mm = max(mm, bm); else m[i] = __builtin_nanf("");
+        if (bv < 0x7F800000u) mv = max(mv, bv); else root[i] = __builtin_nanf("");
+      }
+      wave_max(mm, mv);
+    }
+    float sm, im, sv, iv;
+    block_scale(mm, sm, im);
+    block_scale(mv, sv, iv);
+    const unsigned cm = encode4<false>(m, im, rnd), cv = encode4<true>(root, iv, rnd);
+    if (left > 0) {
+      store_codes((unsigned char*)t.m + at, left, cm);
+      store_codes((unsigned char*)t.v + at, left, cv);
+    }
+    if (lane == 0) { t.ms[blk] = sm; t.vs[blk] = sv; }
+  }
+}
+
+// A wave takes AD_UNROLL blocks: all their loads are issued before the first is worked on.
 template <typename PT, typename GT, int BITS>
 __global__ void __launch_bounds__(256) adamw_multi_kernel(AdArgs a) {
   // the tensor this workgroup works on
@@ -134,89 +233,51 @@ __global__ void __launch_bounds__(256) adamw_multi_kernel(AdArgs a) {
     if (a.first[mid] <= blockIdx.x) lo = mid; else hi = mid - 1;
   }
   const AdTensor& t = a.t[lo];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t blk0 = ((int64_t)(blockIdx.x - a.first[lo]) * 4 + wave) * AD_UNROLL;
-  float p[AD_UNROLL][4], g[AD_UNROLL][4], m[AD_UNROLL][4], v[AD_UNROLL][4];
-  int left[AD_UNROLL];
+  if ((blk0 + AD_UNROLL) * ADAMW_BLOCK <= t.n) {
+    float p[AD_UNROLL][4], g[AD_UNROLL][4], m[AD_UNROLL][4], v[AD_UNROLL][4];
+    unsigned cm[AD_UNROLL], cv[AD_UNROLL];
 #pragma unroll
-  for (int u = 0; u < AD_UNROLL; ++u) {
-    const int64_t at = (blk0 + u) * ADAMW_BLOCK + 4 * lane;
-    left[u] = at >= t.n ? 0 : (int)min((int64_t)4, t.n - at);
-    if (left[u] > 0) {
-      load<PT>(t.p, at, left[u], p[u]);
-      load<GT>(t.g, at, left[u], g[u]);
+    for (int u = 0; u < AD_UNROLL; ++u) {
+      const int64_t at = (blk0 + u) * ADAMW_BLOCK + 4 * lane;
+      load<PT>(t.p, at, 4, p[u]);
+      load<GT>(t.g, at, 4, g[u]);
       if (BITS == 32) {
-        load<float>(t.m, at, left[u], m[u]);
-        load<float>(t.v, at, left[u], v[u]);
+        load<float>(t.m, at, 4, m[u]);
+        load<float>(t.v, at, 4, v[u]);
       } else {
-        decode(load_codes((const unsigned char*)t.m + at, left[u]), t.ms[blk0 + u], m[u]);
-        decode(load_codes((const unsigned char*)t.v + at, left[u]), t.vs[blk0 + u], v[u]);
+        cm[u] = load_codes((const unsigned char*)t.m + at, 4);
+        cv[u] = load_codes((const unsigned char*)t.v + at, 4);
       }
-    } else {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) p[u][i] = g[u][i] = m[u][i] = v[u][i] = 0.f;
     }
+#pragma unroll
+    for (int u = 0; u < AD_UNROLL; ++u) {
+      if (BITS == 8) {
+        decode(cm[u], t.ms[blk0 + u], m[u]);
+        decode(cv[u], t.vs[blk0 + u], v[u]);
+      }
+      finish_block<PT, BITS>(a, t, blk0 + u, lane, 4, p[u], g[u], m[u], v[u]);
+    }
+    return;
   }
-#pragma unroll
-  for (int u = 0; u < AD_UNROLL; ++u) {
-    if (blk0 * ADAMW_BLOCK + (int64_t)u * ADAMW_BLOCK >= t.n) break;        // the same in every lane of the wave
-    const int64_t blk = blk0 + u, at = blk * ADAMW_BLOCK + 4 * lane;
-    unsigned rnd[4] = {0u, 0u, 0u, 0u};
-    if (BITS == 8 || sizeof(PT) == 2) {
-      const unsigned kb = mix32(t.key + (unsigned)blk * 0x9E3779B9u);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) rnd[i] = mix32(kb + (unsigned)(4 * lane + i) * 0x9E3779B9u);
-    }
-    float root[4];
-    unsigned mm = 0u, mv = 0u;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float gi = g[u][i] * a.gscale;
-      const float vo = BITS == 8 ? v[u][i] * v[u][i] : v[u][i];
-      m[u][i] = m[u][i] * a.b1 + gi * a.omb1;
-      v[u][i] = vo * a.b2 + (gi * a.omb2) * gi;
-      root[i] = sqrtf(v[u][i]);
-      p[u][i] = p[u][i] * t.decay - (m[u][i] / (root[i] * t.inv_bc2 + a.eps)) * t.size;
-      if (BITS == 8 && i < left[u]) {
-        const unsigned bm = __float_as_uint(m[u][i]) & 0x7FFFFFFFu, bv = __float_as_uint(root[i]) & 0x7FFFFFFFu;
-        mm = bm < 0x7F800000u && bm > mm ? bm : mm;
-        mv = bv < 0x7F800000u && bv > mv ? bv : mv;
+#pragma unroll 1
+  for (int64_t blk = blk0; blk < blk0 + AD_UNROLL && blk * ADAMW_BLOCK < t.n; ++blk) {
+    const int64_t at = blk * ADAMW_BLOCK + 4 * lane;
+    const int left = at >= t.n ? 0 : (int)min((int64_t)4, t.n - at);
+    float p[4] = {0.f, 0.f, 0.f, 0.f}, g[4] = {0.f, 0.f, 0.f, 0.f}, m[4] = {0.f, 0.f, 0.f, 0.f}, v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (left > 0) {
+      load<PT>(t.p, at, left, p);
+      load<GT>(t.g, at, left, g);
+      if (BITS == 32) {
+        load<float>(t.m, at, left, m);
+        load<float>(t.v, at, left, v);
+      } else {
+        decode(load_codes((const unsigned char*)t.m + at, left), t.ms[blk], m);
+        decode(load_codes((const unsigned char*)t.v + at, left), t.vs[blk], v);
       }
     }
-    if (left[u] > 0) {
-      if (sizeof(PT) == 4) store((float*)t.p, at, left[u], p[u]);
-      else {
-        unsigned short w[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const unsigned bits = __float_as_uint(p[u][i]);
-          const bool finite = (bits & 0x7FFFFFFFu) < 0x7F800000u;
-          w[i] = (unsigned short)((finite ? bits + (mix32(rnd[i] ^ 0x68E31DA4u) & 0xFFFFu) : (p[u][i] != p[u][i] ? 0x7FC00000u : bits)) >> 16);
-        }
-        store((bf16_t*)t.p, at, left[u], w);
-      }
-    }
-    if (BITS == 32) {
-      if (left[u] > 0) {
-        store((float*)t.m, at, left[u], m[u]);
-        store((float*)t.v, at, left[u], v[u]);
-      }
-    } else {
-      float sm, im, sv, iv;
-      block_scale(wave_max(mm), sm, im);
-      block_scale(wave_max(mv), sv, iv);
-      unsigned cm = 0u, cv = 0u;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        cm |= encode<false>(m[u][i] * im, ((rnd[i] & 0xFFFu) << 8) | 0x80u) << (8 * i);
-        cv |= encode<true>(root[i] * iv, rnd[i] >> 12) << (8 * i);
-      }
-      if (left[u] > 0) {
-        store_codes((unsigned char*)t.m + at, left[u], cm);
-        store_codes((unsigned char*)t.v + at, left[u], cv);
-      }
-      if (lane == 0) { t.ms[blk] = sm; t.vs[blk] = sv; }
-    }
+    finish_block<PT, BITS>(a, t, blk, lane, left, p, g, m, v);
   }
 }
 

@@ -244,7 +244,8 @@ def adamw(p, g, m, v, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=
     change = lr / (1 - b1 ** step) * m1 / denom
     e_denom = e_root / math.sqrt(1 - b2 ** step) + 4 * U * denom
     low = (denom - e_denom).clamp_min(1e-300)
-    e_change = lr / (1 - b1 ** step) * (e_m / low + m1.abs() * e_denom / (denom * low)) + 4 * U * change.abs()
+    # the quotient is m times the hardware's reciprocal (within one ulp: 2 U), rounded (U), times the step size (itself rounded: U), rounded (U)
+    e_change = lr / (1 - b1 ** step) * (e_m / low + m1.abs() * e_denom / (denom * low)) + 5.01 * U * change.abs()
     p1 = p * (1 - lr * weight_decay) - change
     e_p = e_change + 2 * U * p.abs() + 2 * U * (p1.abs() + e_change)
     return {"p": (p1, e_p), "m": (m1, e_m), "v": (v1, e_v), "root": (root, e_root)}
