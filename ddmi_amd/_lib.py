@@ -267,6 +267,29 @@ def stream_ptr() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
+def raw_stream(device_index: int) -> int:
+    """The handle of a device's current stream, without making a torch.cuda.Stream of it."""
+    import torch
+    return torch._C._cuda_getCurrentRawStream(device_index)
+
+
+class on_device:
+    """`with torch.cuda.device(index)`, entered only where it is not the current device already (the common case costs a comparison)."""
+    __slots__ = ("guard",)
+
+    def __init__(self, index: int):
+        import torch
+        self.guard = None if torch._C._cuda_getDevice() == index else torch.cuda.device(index)
+
+    def __enter__(self):
+        if self.guard is not None:
+            self.guard.__enter__()
+
+    def __exit__(self, *exc):
+        if self.guard is not None:
+            self.guard.__exit__(*exc)
+
+
 def load_weights(load_fn, handle, state, prefix_strip: str = "", only_prefixes=None) -> int:
     """Hands every fp32 tensor of a state-dict-like mapping to `load_fn(handle, key, ptr, shape, ndim)`."""
     import numpy as np

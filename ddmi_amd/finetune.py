@@ -16,6 +16,7 @@ in a hipGraph (the workspace is a torch tensor of the call, so graphs share none
 from __future__ import annotations
 
 import ctypes as C
+import functools
 from typing import NamedTuple, Optional
 
 import torch
@@ -48,7 +49,7 @@ def _p(t: Optional[torch.Tensor]):
 def _expect(who, name, t, shape, dtype=torch.float32):
     if not isinstance(t, torch.Tensor):
         raise ValueError(f"{who}: {name} is a tensor, got {type(t).__name__}")
-    if tuple(t.shape) != tuple(shape):
+    if t.shape != shape:
         raise ValueError(f"{who}: {name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
     if t.dtype != dtype:
         raise ValueError(f"{who}: {name} is {t.dtype}, expected {dtype}")
@@ -59,7 +60,7 @@ def _check_outputs(who, model_out, ref_out, x_t, sqrt_1mac, mixing_logit, ref_mi
         raise ValueError(f"{who}: model_out is a non-empty [B, C, ...] tensor")
     if model_out.dtype not in _OUT_TYPES:
         raise ValueError(f"{who}: model_out is fp32 or bf16, got {model_out.dtype}")
-    shape = tuple(model_out.shape)
+    shape = model_out.shape
     if ref_out is not None:
         _expect(who, "ref_out", ref_out, shape, model_out.dtype)
     _expect(who, "x_t", x_t, shape)
@@ -81,37 +82,43 @@ def _check_constants(who, **tensors):
             raise ValueError(f"{who}: {name} requires a gradient, but only model_out and mixing_logit get one: detach it")
 
 
-def _check_device(who, *tensors):
-    dev = tensors[0].device
-    if dev.type != "cuda":
-        raise ValueError(f"{who}: tensors live on a GPU, got {dev}")
+def _check_device(who, *tensors) -> int:
+    index = tensors[0].get_device()
+    if index < 0 or not tensors[0].is_cuda:
+        raise ValueError(f"{who}: tensors live on a GPU, got {tensors[0].device}")
     for t in tensors:
-        if t is not None and t.device != dev:
-            raise ValueError(f"{who}: all tensors live on one device, got {dev} and {t.device}")
-    return dev
+        if t is not None and t.get_device() != index:
+            raise ValueError(f"{who}: all tensors live on one device, got {tensors[0].device} and {t.device}")
+    return index
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(B: int, Cc: int, HW: int, mixed: bool) -> int:
+    n = C.c_size_t(0)
+    _lib.check(_lib.lib().ddmi_train_loss_workspace_bytes(B, Cc, HW, int(mixed), C.byref(n)))
+    return n.value
+
+
+def _flat(t):
+    return None if t is None else (t.detach() if t.requires_grad else t).contiguous()
 
 
 class _Call:
     """The arguments of a loss's C entry points: contiguous tensors, kept alive, and the struct that points at them."""
+    __slots__ = ("tensors", "B", "C", "HW", "out_dtype", "index")
 
-    def __init__(self, model_out, ref_out, x_t, second, sqrt_1mac, logit, ref_logit, weight):
-        flat = lambda t: None if t is None else t.detach().contiguous()      # noqa: E731
-        self.tensors = tuple(flat(t) for t in (model_out, ref_out, x_t, second, sqrt_1mac, logit, ref_logit, weight))
-        self.B, self.C = int(model_out.shape[0]), int(model_out.shape[1])
-        self.HW = model_out.numel() // (self.B * self.C)
-        self.out_dtype = _OUT_TYPES[model_out.dtype]
+    def __init__(self, *tensors):      # model_out, ref_out, x_t, noise / x_prev, sqrt_1mac, mixing_logit, ref_mixing_logit, weight
+        self.tensors = tuple(map(_flat, tensors))
+        out = tensors[0]
+        self.B, self.C = out.shape[0], out.shape[1]
+        self.HW = out.numel() // (self.B * self.C)
+        self.out_dtype, self.index = _OUT_TYPES[out.dtype], out.get_device()
 
     def struct(self):
-        return _lib.LossIn(*[_p(t) for t in self.tensors], self.HW, self.C, self.out_dtype)
+        return _lib.LossIn(*map(_p, self.tensors), self.HW, self.C, self.out_dtype)
 
     def workspace(self):
-        n = C.c_size_t(0)
-        _lib.check(_lib.lib().ddmi_train_loss_workspace_bytes(self.B, self.C, self.HW, int(self.tensors[5] is not None), C.byref(n)))
-        return torch.empty(n.value, dtype=torch.uint8, device=self.tensors[0].device)
-
-
-def _begin(dev):
-    _lib.init_device(dev.index if dev.index is not None else torch.cuda.current_device())
+        return torch.empty(_workspace_bytes(self.B, self.C, self.HW, self.tensors[5] is not None), dtype=torch.uint8, device=self.tensors[0].device)
 
 
 class PreferenceLossFn(torch.autograd.Function):
@@ -124,7 +131,7 @@ class PreferenceLossFn(torch.autograd.Function):
         margin = torch.empty((pairs,), dtype=torch.float32, device=dev)
         mse = torch.empty((2 * pairs,), dtype=torch.float32, device=dev)
         _lib.check(_lib.lib().ddmi_train_pref_loss(C.byref(call.struct()), pairs, noise.shape[0], beta, label_smoothing, ws.data_ptr(), ws.numel(),
-                                                   loss.data_ptr(), margin.data_ptr(), mse.data_ptr(), _lib.stream_ptr()))
+                                                   loss.data_ptr(), margin.data_ptr(), mse.data_ptr(), _lib.raw_stream(call.index)))
         # the gradient needs neither the reference's output nor its logit
         call.tensors = (call.tensors[0], None) + call.tensors[2:6] + (None, call.tensors[7])
         ctx.save_for_backward(ws, *call.tensors)
@@ -142,9 +149,9 @@ class PreferenceLossFn(torch.autograd.Function):
         d_logit = torch.empty(ctx.logit_shape, dtype=torch.float32, device=ws.device) if ctx.logit_shape else None
         pairs, noise_rows, beta, smoothing = ctx.meta
         g = g.contiguous()
-        with torch.cuda.device(ws.device):
+        with _lib.on_device(call.index):
             _lib.check(_lib.lib().ddmi_train_pref_loss_bwd(C.byref(call.struct()), pairs, noise_rows, beta, smoothing, ws.data_ptr(), ws.numel(),
-                                                           g.data_ptr(), d_out.data_ptr(), _p(d_logit), _lib.stream_ptr()))
+                                                           g.data_ptr(), d_out.data_ptr(), _p(d_logit), _lib.raw_stream(call.index)))
         call.tensors = None
         return (d_out, d_logit) + (None,) * 8
 
@@ -161,7 +168,7 @@ class PolicyLossFn(torch.autograd.Function):
         logp_old, advantage = logp_old.contiguous(), advantage.contiguous()
         _lib.check(_lib.lib().ddmi_train_policy_loss(C.byref(call.struct()), B, transition.data_ptr(), logp_old.data_ptr(), advantage.data_ptr(),
                                                      clip_range, kl_coef, ws.data_ptr(), ws.numel(), loss.data_ptr(), logp.data_ptr(), ratio.data_ptr(),
-                                                     kl.data_ptr(), _lib.stream_ptr()))
+                                                     kl.data_ptr(), _lib.raw_stream(call.index)))
         ctx.save_for_backward(ws, transition, *call.tensors)
         call.tensors = None
         ctx.call = call
@@ -176,9 +183,9 @@ class PolicyLossFn(torch.autograd.Function):
         d_out = torch.empty_like(call.tensors[0])
         d_logit = torch.empty(ctx.logit_shape, dtype=torch.float32, device=ws.device) if ctx.logit_shape else None
         g = g.contiguous()
-        with torch.cuda.device(ws.device):
+        with _lib.on_device(call.index):
             _lib.check(_lib.lib().ddmi_train_policy_loss_bwd(C.byref(call.struct()), call.B, transition.data_ptr(), ws.data_ptr(), ws.numel(),
-                                                             g.data_ptr(), d_out.data_ptr(), _p(d_logit), _lib.stream_ptr()))
+                                                             g.data_ptr(), d_out.data_ptr(), _p(d_logit), _lib.raw_stream(call.index)))
         call.tensors = None
         return (d_out, d_logit) + (None,) * 11
 
@@ -211,8 +218,8 @@ def preference_loss(model_out, ref_out, x_t, noise, sqrt_1mac, beta, mixing_logi
         raise ValueError(f"{who}: beta is a number and label_smoothing in [0, 1], got {beta}, {label_smoothing}")
     _check_constants(who, ref_out=ref_out, x_t=x_t, noise=noise, sqrt_1mac=sqrt_1mac, ref_mixing_logit=ref_mixing_logit, weight=weight)
     dev = _check_device(who, model_out, ref_out, x_t, noise, sqrt_1mac, mixing_logit, ref_mixing_logit, weight)
-    with torch.cuda.device(dev):
-        _begin(dev)
+    with _lib.on_device(dev):
+        _lib.init_device(dev)
         return PreferenceLoss(*PreferenceLossFn.apply(model_out, mixing_logit, ref_out, x_t, noise, sqrt_1mac, ref_mixing_logit, weight, beta,
                                                       label_smoothing))
 
@@ -248,8 +255,8 @@ def policy_loss(model_out, x_t, x_prev, transition, sqrt_1mac, logp_old, advanta
     _check_constants(who, ref_out=ref_out, x_t=x_t, x_prev=x_prev, transition=transition, sqrt_1mac=sqrt_1mac, logp_old=logp_old, advantage=advantage,
                      ref_mixing_logit=ref_mixing_logit, weight=weight)
     dev = _check_device(who, model_out, ref_out, x_t, x_prev, transition, sqrt_1mac, logp_old, advantage, mixing_logit, ref_mixing_logit, weight)
-    with torch.cuda.device(dev):
-        _begin(dev)
+    with _lib.on_device(dev):
+        _lib.init_device(dev)
         return PolicyLoss(*PolicyLossFn.apply(model_out, mixing_logit, ref_out, x_t, x_prev, sqrt_1mac, ref_mixing_logit, weight, transition, logp_old,
                                               advantage, clip_range, kl_coef))
 
@@ -260,11 +267,11 @@ def transition_log_prob(model_out, x_t, x_prev, transition, sqrt_1mac, mixing_lo
     _check_outputs(who, model_out, None, x_t, sqrt_1mac, mixing_logit, None)
     _check_transition(who, model_out, x_prev, transition, weight)
     dev = _check_device(who, model_out, x_t, x_prev, transition, sqrt_1mac, mixing_logit, weight)
-    with torch.cuda.device(dev):
-        _begin(dev)
+    with _lib.on_device(dev):
+        _lib.init_device(dev)
         call = _Call(model_out, None, x_t, x_prev, sqrt_1mac, mixing_logit, None, weight)
         ws, transition = call.workspace(), transition.detach().contiguous()
-        logp = torch.empty((call.B,), dtype=torch.float32, device=dev)
+        logp = torch.empty((call.B,), dtype=torch.float32, device=model_out.device)
         _lib.check(_lib.lib().ddmi_train_policy_loss(C.byref(call.struct()), call.B, transition.data_ptr(), None, None, 0.0, 0.0, ws.data_ptr(), ws.numel(),
-                                                     None, logp.data_ptr(), None, None, _lib.stream_ptr()))
+                                                     None, logp.data_ptr(), None, None, _lib.raw_stream(call.index)))
         return logp

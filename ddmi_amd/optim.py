@@ -22,6 +22,9 @@ _ENTRY = np.dtype([("param", "u8"), ("grad", "u8"), ("exp_avg", "u8"), ("exp_avg
                    ("numel", "i8"), ("step", "i8"), ("lr", "f8"), ("weight_decay", "f8"), ("index", "i8")])
 
 
+_NUMEL, _CONTIGUOUS, _POINTER, _DEVICE = torch.Tensor.numel, torch.Tensor.is_contiguous, torch.Tensor.data_ptr, torch.Tensor.get_device
+
+
 def blocks_of(n: int) -> int:
     """Scales of a tensor of n values."""
     return -(-n // BLOCK)
@@ -29,7 +32,7 @@ def blocks_of(n: int) -> int:
 
 def _overlap(ptrs, nbytes) -> bool:
     at = np.argsort(ptrs, kind="stable")
-    p, n = ptrs[at], nbytes[at]
+    p, n = ptrs[at].astype(np.int64), nbytes[at]
     return bool(np.any(p[:-1] + n[:-1] > p[1:]))
 
 
@@ -68,23 +71,25 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     else:
         raise ValueError(f"{who}: moments are all fp32 or all float8_e4m3fn, got {sorted(map(str, kinds))}")
     p_types, g_types = [t.dtype for t in params], [t.dtype for t in grads]
-    bad = (set(p_types) | set(g_types)) - set(_TYPES)
+    kinds = set(zip(p_types, g_types))
+    bad = {k for kind in kinds for k in kind} - set(_TYPES)
     if bad:
         raise ValueError(f"{who}: parameters and gradients are fp32 or bf16, got {sorted(map(str, bad))}")
     e = np.zeros(n, dtype=_ENTRY)
-    e["numel"] = numel = np.array([t.numel() for t in params], dtype=np.int64)
+    sizes = list(map(_NUMEL, params))
     for name, ts in (("gradient", grads), ("exp_avg", exp_avgs), ("exp_avg_sq", exp_avg_sqs)):
-        if [t.numel() for t in ts] != numel.tolist():
+        if list(map(_NUMEL, ts)) != sizes:
             raise ValueError(f"{who}: a tensor's {name} has another number of values than the parameter")
     if [t.shape for t in grads] != [t.shape for t in params]:
         raise ValueError(f"{who}: a gradient has another shape than its parameter")
+    e["numel"] = numel = np.array(sizes, dtype=np.int64)
     blocks = -(-numel // BLOCK)
     if bits == 8:
         for ts in scales:
-            if [t.numel() for t in ts] != blocks.tolist() or {t.dtype for t in ts} != {torch.float32}:
+            if list(map(_NUMEL, ts)) != blocks.tolist() or {t.dtype for t in ts} != {torch.float32}:
                 raise ValueError(f"{who}: scales are fp32, one for each {BLOCK} values of a tensor")
     for ts in lists:
-        if not all(t.is_contiguous() for t in ts):
+        if not all(map(_CONTIGUOUS, ts)):
             raise ValueError(f"{who}: tensors are contiguous")
     e["step"], e["lr"], e["weight_decay"], e["index"] = step, lr, weight_decay, np.arange(n)
     if e["step"].min() < 1:
@@ -92,27 +97,26 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     b1, b2 = float(betas[0]), float(betas[1])
     if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and eps >= 0.0):
         raise ValueError(f"{who}: betas in [0, 1) and eps >= 0, got {betas}, {eps}")
-    devices = {t.device for ts in lists for t in ts}
-    if len(devices) > 1 or next(iter(devices)).type != "cuda":
-        raise ValueError(f"{who}: all tensors live on one GPU, got {sorted(map(str, devices))}")
+    dev = params[0].get_device()
+    if dev < 0 or not params[0].is_cuda or any(set(map(_DEVICE, ts)) != {dev} for ts in lists):
+        raise ValueError(f"{who}: all tensors live on one GPU, got {sorted({str(t.device) for ts in lists for t in ts})}")
     for name, ts in zip(("param", "grad", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale"), lists):
-        e[name] = [t.data_ptr() for t in ts]
-    p_bytes = numel * np.array([t.itemsize for t in p_types], dtype=np.int64)
-    written = [("parameters", "param", p_bytes)] + [(k, k, numel * (4 if bits == 32 else 1)) for k in ("exp_avg", "exp_avg_sq")]
-    written += [(k, k, 4 * blocks) for k in ("exp_avg_scale", "exp_avg_sq_scale")] if bits == 8 else []
-    for name, key, size in written:
-        if _overlap(e[key].astype(np.int64)[numel > 0], size[numel > 0]):
-            raise ValueError(f"{who}: two of the {name} share memory (the same tensor twice?)")
-    dev = next(iter(devices))
-    with torch.cuda.device(dev):
+        e[name] = list(map(_POINTER, ts))
+    p_bytes = numel * (4 if p_types.count(torch.float32) == n else np.array([t.itemsize for t in p_types], dtype=np.int64))
+    state = [("exp_avg", 4 * numel if bits == 32 else numel), ("exp_avg_sq", 4 * numel if bits == 32 else numel)]
+    state += [("exp_avg_scale", 4 * blocks), ("exp_avg_sq_scale", 4 * blocks)] if bits == 8 else []
+    used = numel > 0
+    if _overlap(np.concatenate([e[k][used] for k in ("param", *(k for k, _ in state))]), np.concatenate([p_bytes[used], *(v[used] for _, v in state)])):
+        raise ValueError(f"{who}: two of the tensors that are written share memory (the same one twice?)")
+    with _lib.on_device(dev):
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError(f"{who}: not inside a graph capture: the step number is an argument and would be frozen")
-        _lib.init_device(dev.index if dev.index is not None else torch.cuda.current_device())
-        kinds = list(zip(p_types, g_types))
-        for kind in dict.fromkeys(kinds):
-            part = e if all(k == kind for k in kinds) else np.ascontiguousarray(e[[k == kind for k in kinds]])
+        _lib.init_device(dev)
+        of = list(zip(p_types, g_types)) if len(kinds) > 1 else None
+        for kind in kinds if of is None else dict.fromkeys(of):
+            part = e if of is None else np.ascontiguousarray(e[[k == kind for k in of]])
             _lib.check(_lib.lib().ddmi_train_adamw_multi(part.ctypes.data, len(part), b1, b2, float(eps), float(grad_scale), int(seed) & 0xFFFFFFFF,
-                                                         _TYPES[kind[0]], _TYPES[kind[1]], bits, _lib.stream_ptr()))
+                                                         _TYPES[kind[0]], _TYPES[kind[1]], bits, _lib.raw_stream(dev)))
 
 
 def encode_moment(x: torch.Tensor, root: bool):
