@@ -4,6 +4,8 @@
 
 enum { FT_PREF = 0, FT_POLICY = 1 };
 #define FT_THREADS 256
+#define FT_VECS 16       // vectors of four residuals that a thread of the one-pass kernel keeps in registers
+#define FT_FUSED_LEAST (1ll << 21)   // values from which on one pass over the inputs is taken
 #define FT_ROWS 512      // most rows (sample, channel) of one workgroup: their mixing coefficients sit in LDS
 
 struct FtArgs {
@@ -30,17 +32,21 @@ struct FtArgs {
   // plan
   int B, C, pairs;
   int64_t T, seg;
-  int wps, rows_per_wg, nseg, log_g;
+  int wps, rows_per_wg, nseg, log_g, fused, polls;
   // workspace
   unsigned* counter;
+  double* total;             // one pass: sum of the weights
+  int* done;                 // one pass: whether a span's gradient is written
   float2* coef;              // a sample: factors of the residual and of the step away from the reference
   double* term;
   double2* part;             // a workgroup of sums_kernel
   double2* chan;             // a (sample, channel, segment, wave): sums the mixing logit's gradient needs
 };
-int ft_plan(FtArgs* a, int B, int C, int64_t HW, bool mixed);
+// rows_of: samples whose sums meet (2: a pair); keep: vectors a thread may keep for one pass over the inputs, 0: two passes
+int ft_plan(FtArgs* a, int B, int C, int64_t HW, bool mixed, int rows_of, int keep);
 size_t ft_workspace_bytes(const FtArgs& a);
 void ft_carve(FtArgs* a, void* ws);
+void ft_set_polls(int n);
 int launch_ft_sums(const FtArgs& a, int mode, int dt, hipStream_t s);
 int launch_ft_grad(const FtArgs& a, int mode, int dt, hipStream_t s);
 

@@ -1,19 +1,20 @@
 // C ABI of the fine-tuning operators (include/ddmi_hip.h, "Fine-tuning"): no handle, no state; the caller owns every buffer, the losses'
 // workspace among them (so two captured graphs, or two streams, that use workspaces of their own share nothing).
+#include <algorithm>
 #include "finetune.h"
 
 namespace {
 bool dtype_ok(int dt) { return dt == DDMI_DTYPE_F32 || dt == DDMI_DTYPE_BF16; }
 int internal_dt(int dt) { return dt == DDMI_DTYPE_F32 ? DT_F32 : DT_BF16; }
 
-int common_args(FtArgs* a, const ddmi_loss_in* in, int B, void* ws, size_t ws_bytes, const char* who) {
+int common_args(FtArgs* a, const ddmi_loss_in* in, int B, int rows_of, int keep, void* ws, size_t ws_bytes, const char* who) {
   const std::string w(who);
   DDMI_REQUIRE(in->model_out && in->second && B > 0 && in->C > 0 && in->HW > 0, w + ": null argument or empty batch");
   DDMI_REQUIRE(dtype_ok(in->out_dtype), w + ": model_out / ref_out are fp32 or bf16");
   DDMI_REQUIRE((in->mixing_logit == nullptr) == (in->ref_mixing_logit == nullptr) || (in->mixing_logit && !in->ref_out), w + ": both mixing logits or none");
   DDMI_REQUIRE(!in->mixing_logit || (in->x_t && in->sqrt_1mac), w + ": mixing needs x_t and sqrt_1mac");
   DDMI_REQUIRE((double)in->C * (double)in->HW < 1.1e12, w + ": sample too large");
-  DDMI_TRY(ft_plan(a, B, in->C, in->HW, in->mixing_logit != nullptr));
+  DDMI_TRY(ft_plan(a, B, in->C, in->HW, in->mixing_logit != nullptr, rows_of, keep));
   DDMI_REQUIRE(ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= ft_workspace_bytes(*a), w + ": workspace too small or not 16-byte aligned");
   ft_carve(a, ws);
   a->out = in->model_out; a->ref = in->ref_out; a->x = in->x_t; a->second = in->second; a->s1 = in->mixing_logit ? in->sqrt_1mac : nullptr;
@@ -21,18 +22,18 @@ int common_args(FtArgs* a, const ddmi_loss_in* in, int B, void* ws, size_t ws_by
   return DDMI_OK;
 }
 // the gradient needs neither the reference's output nor its logit (its residual is the trained network's alone)
-int pref_args(FtArgs* a, const ddmi_loss_in* in, int pairs, int noise_rows, double beta, double label_smoothing, bool grad, void* ws, size_t ws_bytes) {
+int pref_args(FtArgs* a, const ddmi_loss_in* in, int pairs, int noise_rows, double beta, double label_smoothing, bool grad, bool kept, void* ws, size_t ws_bytes) {
   DDMI_REQUIRE(in && (grad || in->ref_out) && pairs > 0 && pairs <= (1 << 29), "pref_loss: null argument or no pairs");
   DDMI_REQUIRE(noise_rows == pairs || noise_rows == 2 * pairs, "pref_loss: the noise has a row for each pair or for each sample");
   DDMI_REQUIRE(label_smoothing >= 0.0 && label_smoothing <= 1.0 && beta == beta, "pref_loss: label_smoothing in [0, 1], beta a number");
-  DDMI_TRY(common_args(a, in, 2 * pairs, ws, ws_bytes, "pref_loss"));
+  DDMI_TRY(common_args(a, in, 2 * pairs, 2, kept ? FT_VECS : 0, ws, ws_bytes, "pref_loss"));
   if (!in->mixing_logit) a->x = nullptr;      // not read
   a->pairs = pairs; a->second_rows = noise_rows; a->beta = beta; a->smoothing = label_smoothing;
   return DDMI_OK;
 }
-int policy_args(FtArgs* a, const ddmi_loss_in* in, int B, const float* transition, void* ws, size_t ws_bytes) {
+int policy_args(FtArgs* a, const ddmi_loss_in* in, int B, const float* transition, bool kept, void* ws, size_t ws_bytes) {
   DDMI_REQUIRE(in && transition && in->x_t, "policy_loss: null argument");
-  DDMI_TRY(common_args(a, in, B, ws, ws_bytes, "policy_loss"));
+  DDMI_TRY(common_args(a, in, B, 1, kept ? (in->ref_out ? FT_VECS / 2 : FT_VECS) : 0, ws, ws_bytes, "policy_loss"));
   a->pairs = B; a->second_rows = B; a->transition = transition;
   return DDMI_OK;
 }
@@ -42,49 +43,65 @@ extern "C" {
 
 int ddmi_train_loss_workspace_bytes(int B, int C, int64_t HW, int mixed, size_t* bytes) {
   DDMI_REQUIRE(bytes && B > 0 && C > 0 && HW > 0 && (double)C * (double)HW < 1.1e12, "train_loss_workspace_bytes: bad arguments");
-  FtArgs a{};
-  DDMI_TRY(ft_plan(&a, B, C, HW, mixed != 0));
-  *bytes = ft_workspace_bytes(a);
+  *bytes = 0;
+  for (int rows_of = 1; rows_of <= 2; ++rows_of)
+    for (int keep : {0, FT_VECS / 2, FT_VECS}) {      // whichever loss the call is, with or without its gradient
+      FtArgs a{};
+      DDMI_TRY(ft_plan(&a, B, C, HW, mixed != 0, rows_of, keep));
+      *bytes = std::max(*bytes, ft_workspace_bytes(a));
+    }
   return DDMI_OK;
 }
 
 int ddmi_train_pref_loss(const ddmi_loss_in* in, int pairs, int noise_rows, double beta, double label_smoothing, void* ws, size_t ws_bytes, float* loss,
-                         float* margin, float* mse, void* stream) {
+                         float* margin, float* mse, void* d_model_out, void* stream) {
   FtArgs a{};
   DDMI_REQUIRE(loss && margin && mse, "pref_loss: null output");
-  DDMI_TRY(pref_args(&a, in, pairs, noise_rows, beta, label_smoothing, false, ws, ws_bytes));
+  DDMI_TRY(pref_args(&a, in, pairs, noise_rows, beta, label_smoothing, false, d_model_out != nullptr, ws, ws_bytes));
+  a.d_out = d_model_out;
   a.loss = loss; a.row_out[0] = margin; a.row_out[1] = mse;
   return launch_ft_sums(a, FT_PREF, internal_dt(in->out_dtype), (hipStream_t)stream);
 }
 int ddmi_train_pref_loss_bwd(const ddmi_loss_in* in, int pairs, int noise_rows, double beta, double label_smoothing, void* ws, size_t ws_bytes,
-                             const float* dloss, void* d_model_out, float* d_logit, void* stream) {
+                             const float* dloss, int state, void* d_model_out, float* d_logit, void* stream) {
   FtArgs a{};
-  DDMI_REQUIRE(d_model_out, "pref_loss_bwd: null output");
-  DDMI_TRY(pref_args(&a, in, pairs, noise_rows, beta, label_smoothing, true, ws, ws_bytes));
+  DDMI_REQUIRE(d_model_out && state >= DDMI_GRAD_NONE && state <= DDMI_GRAD_THIS, "pref_loss_bwd: null output or bad state");
+  DDMI_TRY(pref_args(&a, in, pairs, noise_rows, beta, label_smoothing, true, state != DDMI_GRAD_NONE, ws, ws_bytes));
+  if (!a.fused || state != DDMI_GRAD_THIS) a.done = nullptr;
   DDMI_REQUIRE(!d_logit || in->mixing_logit, "pref_loss_bwd: a logit's gradient without a logit");
   a.dloss = dloss; a.d_out = d_model_out; a.d_logit = d_logit;
   return launch_ft_grad(a, FT_PREF, internal_dt(in->out_dtype), (hipStream_t)stream);
 }
 int ddmi_train_policy_loss(const ddmi_loss_in* in, int B, const float* transition, const float* logp_old, const float* advantage, double clip_range,
-                           double kl_coef, void* ws, size_t ws_bytes, float* loss, float* logp, float* ratio, float* kl, void* stream) {
+                           double kl_coef, void* ws, size_t ws_bytes, float* loss, float* logp, float* ratio, float* kl, void* d_model_out,
+                           void* stream) {
   FtArgs a{};
   DDMI_REQUIRE(logp, "policy_loss: null output");
   DDMI_REQUIRE(!logp_old || (advantage && loss && ratio && kl), "policy_loss: null argument");
   DDMI_REQUIRE(clip_range >= 0.0 && kl_coef == kl_coef, "policy_loss: clip_range >= 0, kl_coef a number");
   DDMI_REQUIRE(kl_coef == 0.0 || (in && in->ref_out), "policy_loss: a KL term needs the reference's output");
-  DDMI_TRY(policy_args(&a, in, B, transition, ws, ws_bytes));
+  DDMI_REQUIRE(logp_old || !d_model_out, "policy_loss: a gradient of the log-density alone is not offered");
+  DDMI_TRY(policy_args(&a, in, B, transition, d_model_out != nullptr, ws, ws_bytes));
+  a.d_out = d_model_out;
   a.logp_old = logp_old; a.advantage = advantage; a.clip = clip_range; a.kl_coef = kl_coef;
   a.loss = logp_old ? loss : nullptr; a.row_out[0] = logp; a.row_out[1] = ratio; a.row_out[2] = kl;
   return launch_ft_sums(a, FT_POLICY, internal_dt(in->out_dtype), (hipStream_t)stream);
 }
-int ddmi_train_policy_loss_bwd(const ddmi_loss_in* in, int B, const float* transition, void* ws, size_t ws_bytes, const float* dloss, void* d_model_out,
-                               float* d_logit, void* stream) {
+int ddmi_train_policy_loss_bwd(const ddmi_loss_in* in, int B, const float* transition, void* ws, size_t ws_bytes, const float* dloss, int state,
+                               void* d_model_out, float* d_logit, void* stream) {
   FtArgs a{};
-  DDMI_REQUIRE(d_model_out, "policy_loss_bwd: null output");
-  DDMI_TRY(policy_args(&a, in, B, transition, ws, ws_bytes));
+  DDMI_REQUIRE(d_model_out && state >= DDMI_GRAD_NONE && state <= DDMI_GRAD_THIS, "policy_loss_bwd: null output or bad state");
+  DDMI_TRY(policy_args(&a, in, B, transition, state != DDMI_GRAD_NONE, ws, ws_bytes));
+  if (!a.fused || state != DDMI_GRAD_THIS) a.done = nullptr;
   DDMI_REQUIRE(!d_logit || in->mixing_logit, "policy_loss_bwd: a logit's gradient without a logit");
   a.dloss = dloss; a.d_out = d_model_out; a.d_logit = d_logit;
   return launch_ft_grad(a, FT_POLICY, internal_dt(in->out_dtype), (hipStream_t)stream);
+}
+
+int ddmi_debug_loss_polls(int n) {
+  DDMI_REQUIRE(n >= 0, "debug_loss_polls: not negative");
+  ft_set_polls(n);
+  return DDMI_OK;
 }
 
 int ddmi_train_adamw_multi(const ddmi_adamw_tensor* tensors, int n, double beta1, double beta2, double eps, double grad_scale, uint32_t seed,

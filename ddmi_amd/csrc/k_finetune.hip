@@ -44,10 +44,12 @@ struct Span {
   int b, row0, rows, seg;
   int64_t t0, t1;
 };
+// spans [0, wps) are those of the first sample, and so on; of the preference loss: of the first pair's preferred sample, its rejected one ...
+template <int MODE>
 __device__ __forceinline__ Span span_of(const FtArgs& a, int blk) {
   Span s;
-  s.b = blk / a.wps;
-  const int j = blk - s.b * a.wps;
+  const int i = blk / a.wps, j = blk - i * a.wps;
+  s.b = MODE == FT_PREF ? (i >> 1) + (i & 1) * a.pairs : i;
   s.row0 = (j / a.nseg) * a.rows_per_wg;
   s.seg = j - (j / a.nseg) * a.nseg;
   s.rows = min(a.rows_per_wg, a.C - s.row0);
@@ -100,7 +102,7 @@ __global__ void __launch_bounds__(FT_THREADS) sums_kernel(FtArgs a) {
   __shared__ double red[2][FT_THREADS / 64];
   const int tid = threadIdx.x;
   if (blockIdx.x == 0 && tid == 0) *a.counter = 0u;   // rows_kernel counts its workgroups; stream order makes this visible to it
-  const Span s = span_of(a, blockIdx.x);
+  const Span s = span_of<MODE>(a, blockIdx.x);
   const int G = 1 << a.log_g, lane = tid & (G - 1), group = tid >> a.log_g, ngroups = FT_THREADS >> a.log_g;
   const int wpg = G > 64 ? G / 64 : 1;                // waves that share a row
   const bool used = takes_part<MODE>(a, s.b);
@@ -169,10 +171,53 @@ __device__ __forceinline__ double block_sum(double v, double* red) {
   for (int w = 0; w < FT_THREADS / 64; ++w) t += red[w];
   return t;
 }
-__device__ __forceinline__ double2 sample_sums(const FtArgs& a, int b, double* red) {
+// the scalar work of one pair / transition, from its sums
+struct RowOut {
+  double term, stat[3];       // weighted loss; margin, mse, mse | logp, ratio, kl
+  float2 coef[2];             // factors of the residual and of the step from the reference: preferred, rejected | transition
+};
+__device__ __forceinline__ RowOut pref_row(const FtArgs& a, bool used, double w, double2 sw, double2 sl) {
+  RowOut o{};
+  const double n = (double)a.C * (double)a.T;
+  double h = 0.0, dh = 0.0;
+  if (used) {
+    h = -0.5 * a.beta * (sw.x - sl.x) / n;
+    const double t = log1p(exp(-fabs(h))), ls = a.smoothing;              // -log sigma(h) = t - min(h, 0)
+    o.term = w * ((1.0 - ls) * (t - fmin(h, 0.0)) + ls * (t + fmax(h, 0.0)));
+    dh = w * (ls / (1.0 + exp(-h)) - (1.0 - ls) / (1.0 + exp(h)));
+  }
+  o.stat[0] = h; o.stat[1] = sw.y / n; o.stat[2] = sl.y / n;
+  o.coef[0] = make_float2((float)(-dh * a.beta / n), 0.f);
+  o.coef[1] = make_float2((float)(dh * a.beta / n), 0.f);
+  return o;
+}
+__device__ __forceinline__ RowOut policy_row(const FtArgs& a, bool used, double w, int i, double2 s) {
+  RowOut o{};
+  const double n = (double)a.C * (double)a.T;
+  if (!used) return o;
+  const double sd = a.transition[3 * (int64_t)i + 2], var = sd * sd, E = a.transition[3 * (int64_t)i + 1];
+  o.stat[0] = -s.x / n / (2.0 * var) - log(sd) - 0.91893853320467274178;
+  if (!a.logp_old) return o;
+  const double adv = a.advantage[i], ratio = exp(o.stat[0] - (double)a.logp_old[i]);
+  const double lo = 1.0 - a.clip, hi = 1.0 + a.clip, held = ratio < lo ? lo : (ratio > hi ? hi : ratio);
+  const double kl = E * E * s.y / n / (2.0 * var), open = -adv * ratio, bound = -adv * held;
+  const bool free = open >= bound, clipped = bound > open;                 // neither: a NaN, which shows in the sum
+  o.term = w * ((free ? open : (clipped ? bound : open + bound)) + a.kl_coef * kl);
+  o.stat[1] = ratio; o.stat[2] = kl;
+  o.coef[0] = make_float2((float)((free ? open * w / (var * n) : (clipped ? 0.0 : open + bound)) * E), (float)(w * a.kl_coef * E * E / (var * n)));
+  return o;
+}
+template <int MODE>
+__device__ __forceinline__ double total_weight(const FtArgs& a, int rows, double* red) {
+  double total = 0.0;
+  for (int j = threadIdx.x; j < rows; j += FT_THREADS)
+    if (takes_part<MODE>(a, j)) total += a.weight ? (double)a.weight[j] : 1.0;
+  return block_sum(total, red);
+}
+__device__ __forceinline__ double2 sample_sums(const FtArgs& a, int sample, double* red) {
   double u = 0.0, v = 0.0;
   for (int j = threadIdx.x; j < a.wps; j += FT_THREADS) {
-    const double2 p = a.part[(int64_t)b * a.wps + j];
+    const double2 p = a.part[(int64_t)sample * a.wps + j];
     u += p.x; v += p.y;
   }
   u = block_sum(u, red);
@@ -185,56 +230,32 @@ __global__ void __launch_bounds__(FT_THREADS) rows_kernel(FtArgs a) {
   __shared__ double red[FT_THREADS / 64];
   __shared__ int last;
   const int i = blockIdx.x, rows = gridDim.x, tid = threadIdx.x;
-  const double n = (double)a.C * (double)a.T;
-  double total = 0.0;
-  for (int j = tid; j < rows; j += FT_THREADS)
-    if (takes_part<MODE>(a, j)) total += a.weight ? (double)a.weight[j] : 1.0;
-  total = block_sum(total, red);
+  const double total = total_weight<MODE>(a, rows, red);
   const bool used = takes_part<MODE>(a, i);
   const double w = used ? (a.weight ? (double)a.weight[i] : 1.0) / total : 0.0;
-  double term = 0.0;
+  RowOut o;
   if (MODE == FT_PREF) {
-    const double2 sw = sample_sums(a, i, red), sl = sample_sums(a, i + a.pairs, red);
-    double h = 0.0, dh = 0.0;
-    if (used) {
-      h = -0.5 * a.beta * (sw.x - sl.x) / n;
-      const double t = log1p(exp(-fabs(h))), up = 1.0 / (1.0 + exp(-h)), ls = a.smoothing;   // -log sigma(h) = t - min(h, 0)
-      term = w * ((1.0 - ls) * (t - fmin(h, 0.0)) + ls * (t + fmax(h, 0.0)));
-      dh = w * (ls * up - (1.0 - ls) / (1.0 + exp(h)));
-    }
-    if (tid == 0) {
-      a.row_out[0][i] = (float)h;
-      a.row_out[1][i] = (float)(sw.y / n);
-      a.row_out[1][i + a.pairs] = (float)(sl.y / n);
-      a.coef[i] = make_float2((float)(-dh * a.beta / n), 0.f);
-      a.coef[i + a.pairs] = make_float2((float)(dh * a.beta / n), 0.f);
-    }
+    const double2 sw = sample_sums(a, 2 * i, red), sl = sample_sums(a, 2 * i + 1, red);
+    o = pref_row(a, used, w, sw, sl);
   } else {
-    const double2 s = sample_sums(a, i, red);
-    double logp = 0.0, ratio = 0.0, kl = 0.0, k = 0.0, q = 0.0;
-    if (used) {
-      const double sd = a.transition[3 * (int64_t)i + 2], var = sd * sd, E = a.transition[3 * (int64_t)i + 1];
-      logp = -s.x / n / (2.0 * var) - log(sd) - 0.91893853320467274178;
-      if (a.logp_old) {
-        const double adv = a.advantage[i];
-        ratio = exp(logp - (double)a.logp_old[i]);
-        const double lo = 1.0 - a.clip, hi = 1.0 + a.clip, held = ratio < lo ? lo : (ratio > hi ? hi : ratio);
-        kl = E * E * s.y / n / (2.0 * var);
-        const double open = -adv * ratio, bound = -adv * held;
-        term = w * ((open >= bound ? open : (bound > open ? bound : open + bound)) + a.kl_coef * kl);   // the sum: NaN stays NaN
-        k = (open >= bound) ? -adv * ratio * w / (var * n) : (bound > open ? 0.0 : open + bound);
-        q = w * a.kl_coef * E / (var * n);
-      }
-      k *= E; q *= E;
-    }
-    if (tid == 0) {
-      a.row_out[0][i] = (float)logp;
-      if (a.logp_old) { a.row_out[1][i] = (float)ratio; a.row_out[2][i] = (float)kl; a.coef[i] = make_float2((float)k, (float)q); }
+    o = policy_row(a, used, w, i, sample_sums(a, i, red));
+  }
+  if (tid == 0) {
+    a.row_out[0][i] = (float)o.stat[0];
+    if (MODE == FT_PREF) {
+      a.row_out[1][i] = (float)o.stat[1];
+      a.row_out[1][i + a.pairs] = (float)o.stat[2];
+      a.coef[i] = o.coef[0];
+      a.coef[i + a.pairs] = o.coef[1];
+    } else if (a.logp_old) {
+      a.row_out[1][i] = (float)o.stat[1];
+      a.row_out[2][i] = (float)o.stat[2];
+      a.coef[i] = o.coef[0];
     }
   }
   if (!a.loss) return;
   if (tid == 0) {
-    __hip_atomic_store(&a.term[i], term, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __hip_atomic_store(&a.term[i], o.term, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     const unsigned done = __hip_atomic_fetch_add(a.counter, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
     last = done == (unsigned)rows - 1u;
   }
@@ -246,9 +267,180 @@ __global__ void __launch_bounds__(FT_THREADS) rows_kernel(FtArgs a) {
   if (tid == 0) *a.loss = (float)sum;
 }
 
+// ---- one pass: the residuals wait in registers for their sample's sums ----------------------------------------------------------
+// A workgroup reads its span, adds up, publishes its two sums, waits for those of the pair's (transition's) other spans and writes the
+// gradient from the residuals in its registers: every input is read once.  The sums' own bits are the signal - open_kernel fills their
+// places with a NaN that no sum is stored as - so publishing is two relaxed agent-scope stores, with no fence and no counter.  The wait is
+// bounded: a workgroup whose neighbours do not show up (other kernels hold the compute units) leaves its span undone, and grad_kernel,
+// which runs after it in any case, computes what is not done.
+constexpr unsigned long long FT_OPEN = 0xFFFFFFFFFFFFFFFFull;
+int g_polls = 1 << 12;                  // some milliseconds; the spans of a row start within microseconds of each other
+
+template <int MODE>
+__global__ void __launch_bounds__(FT_THREADS) open_kernel(FtArgs a, int64_t places, int rows) {
+  __shared__ double red[FT_THREADS / 64];
+  unsigned long long* p = reinterpret_cast<unsigned long long*>(a.part);
+  for (int64_t i = (int64_t)blockIdx.x * FT_THREADS + threadIdx.x; i < places; i += (int64_t)gridDim.x * FT_THREADS) p[i] = FT_OPEN;
+  if (blockIdx.x == 0) {
+    const double total = total_weight<MODE>(a, rows, red);
+    if (threadIdx.x == 0) { *a.counter = 0u; *a.total = total; }
+  }
+}
+__device__ __forceinline__ void publish(double* place, double v) {
+  const unsigned long long bits = v != v ? 0x7FF8000000000000ull : (unsigned long long)__double_as_longlong(v);
+  __hip_atomic_store(reinterpret_cast<unsigned long long*>(place), bits, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// the sums of one sample, by one wave: lane i adds those of spans i, i + 64 ...; false when one did not show up
+__device__ __forceinline__ bool await_sums(const FtArgs& a, int64_t first, int lane, int& polls, double2& out) {
+  unsigned long long* p = reinterpret_cast<unsigned long long*>(a.part + first);
+  double u = 0.0, v = 0.0;
+  for (int j0 = 0; j0 < a.wps; j0 += 64) {
+    const int j = j0 + lane;
+    unsigned long long x = 0, y = 0;
+    for (;;) {
+      if (j < a.wps) {
+        x = __hip_atomic_load(p + 2 * j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        y = __hip_atomic_load(p + 2 * j + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
+      if (__all(x != FT_OPEN && y != FT_OPEN)) break;
+      if (--polls < 0) return false;
+      __builtin_amdgcn_s_sleep(8);
+    }
+    u += __longlong_as_double((long long)x);
+    v += __longlong_as_double((long long)y);
+  }
+  for (int st = 32; st > 0; st >>= 1) { u += __shfl_xor(u, st); v += __shfl_xor(v, st); }
+  out = make_double2(u, v);
+  return true;
+}
+template <typename T> __device__ __forceinline__ void load_some(const T* p, int left, float (&v)[4]) {
+  if (left == 4) { load4(p, v); return; }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) v[i] = i < left ? to_f32(p[i]) : 0.f;
+}
+template <typename T> __device__ __forceinline__ void store_some(T* p, int left, const float (&v)[4]) {
+  if (left == 4) { store4(p, v); return; }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) if (i < left) p[i] = from_f32<T>(v[i]);
+}
+
+// NV vectors of four values a thread; a row's vectors lie on its G lanes in turn, `turns` to a lane
+template <int MODE, bool MIX, bool REF, typename T, int NV>
+__global__ void __launch_bounds__(FT_THREADS, 2) fused_kernel(FtArgs a) {
+  constexpr bool TWO = MODE == FT_POLICY && REF;
+  __shared__ float2 mix[FT_ROWS];
+  __shared__ double red[2][FT_THREADS / 64];
+  __shared__ float2 factor;
+  __shared__ int whole;
+  const int tid = threadIdx.x;
+  const Span s = span_of<MODE>(a, blockIdx.x);
+  const int G = 1 << a.log_g, lane = tid & (G - 1), group = tid >> a.log_g, ngroups = FT_THREADS >> a.log_g;
+  const int wpg = G > 64 ? G / 64 : 1;
+  const int len = (int)(s.t1 - s.t0), turns = cdiv(cdiv(len, 4), G), row_turns = cdiv(s.rows, ngroups);
+  const bool used = takes_part<MODE>(a, s.b);
+  T* pg = (T*)a.d_out + ((int64_t)s.b * a.C + s.row0) * a.T + s.t0;
+  if (!used) {                                                             // its partner's spans still read their places
+    if (tid == 0) { publish(&a.part[blockIdx.x].x, 0.0); publish(&a.part[blockIdx.x].y, 0.0); a.done[blockIdx.x] = 1; }
+    if (MIX)
+      for (int i = tid; i < s.rows * wpg; i += FT_THREADS)
+        a.chan[(((int64_t)s.b * a.C + s.row0 + i / wpg) * a.nseg + s.seg) * wpg + i % wpg] = make_double2(0.0, 0.0);
+    const float zero[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int r = group; r < s.rows; r += ngroups)
+      for (int t = 4 * lane; t < len; t += 4 * G) store_some(pg + (int64_t)r * a.T + t, min(4, len - t), zero);
+    return;
+  }
+  if (MIX) mix_rows(a, s, mix);
+  Elem e{a.s1 ? a.s1[s.b] : 0.f, 0.f, 1.f, 1.f, 0.f};
+  if (MODE == FT_POLICY) { e.A = a.transition[3 * (int64_t)s.b]; e.E = a.transition[3 * (int64_t)s.b + 1]; }
+  const int64_t base = ((int64_t)s.b * a.C + s.row0) * a.T + s.t0, base2 = ((int64_t)(s.b % a.second_rows) * a.C + s.row0) * a.T + s.t0;
+  const T* po = (const T*)a.out + base;
+  const T* pr = REF ? (const T*)a.ref + base : nullptr;
+  const float* px = (MIX || MODE == FT_POLICY) ? a.x + base : nullptr;
+  const float* py = a.second + base2;
+  float res[NV][4], far[TWO ? NV : 1][4];
+  double S0 = 0.0, S1 = 0.0, S2 = 0.0, S3 = 0.0;
+  int rt = 0, turn = 0;                                                    // the same in every lane
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    if (rt < row_turns) {
+      const int r = rt * ngroups + group, t = 4 * (turn * G + lane);
+      const int left = r < s.rows ? min(4, len - t) : 0;
+      float o[4] = {0.f, 0.f, 0.f, 0.f}, q[4] = {0.f, 0.f, 0.f, 0.f}, x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
+      if (left > 0) {
+        const int64_t at = (int64_t)r * a.T + t;
+        load_some(po + at, left, o);
+        if (REF) load_some(pr + at, left, q);
+        if (MIX || MODE == FT_POLICY) load_some(px + at, left, x);
+        load_some(py + at, left, y);
+        if (MIX) { const float2 c = mix[r]; e.c = c.x; e.dc = c.y; }
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float f, part;
+          element<MODE, MIX, REF>(e, o[i], q[i], x[i], y[i], res[j][i], f, part);
+          if (i < left) add_up<MODE, MIX, REF>(res[j][i], f, part, S0, S1, S2, S3);
+          if (TWO) far[j][i] = f;
+        }
+      }
+      if (++turn == turns) {                                               // the row is complete
+        turn = 0;
+        ++rt;
+        if (MIX) {
+          for (int st = (G < 64 ? G : 64) >> 1; st > 0; st >>= 1) { S2 += __shfl_xor(S2, st); if (TWO) S3 += __shfl_xor(S3, st); }
+          if (r < s.rows && (lane & 63) == 0)
+            a.chan[(((int64_t)s.b * a.C + s.row0 + r) * a.nseg + s.seg) * wpg + (lane >> 6)] = make_double2(S2, S3);
+          S2 = S3 = 0.0;
+        }
+      }
+    }
+  }
+  for (int st = 32; st > 0; st >>= 1) { S0 += __shfl_xor(S0, st); S1 += __shfl_xor(S1, st); }
+  if ((tid & 63) == 0) { red[0][tid >> 6] = S0; red[1][tid >> 6] = S1; }
+  __syncthreads();
+  if (tid < 64) {
+    if (tid == 0) {
+      double t0 = 0.0, t1 = 0.0;
+      for (int w = 0; w < FT_THREADS / 64; ++w) { t0 += red[0][w]; t1 += red[1][w]; }
+      publish(&a.part[blockIdx.x].x, t0);
+      publish(&a.part[blockIdx.x].y, t1);
+    }
+    const int row = MODE == FT_PREF ? s.b % a.pairs : s.b;
+    const double w = (a.weight ? (double)a.weight[row] : 1.0) / *a.total;
+    int polls = a.polls;
+    double2 s0 = make_double2(0.0, 0.0), s1 = make_double2(0.0, 0.0);
+    const int64_t first = (int64_t)(MODE == FT_PREF ? 2 * row : row) * a.wps;
+    bool ok = await_sums(a, first, tid, polls, s0);
+    if (MODE == FT_PREF && ok) ok = await_sums(a, first + a.wps, tid, polls, s1);
+    const RowOut o = MODE == FT_PREF ? pref_row(a, true, w, s0, s1) : policy_row(a, true, w, row, s0);
+    if (tid == 0) {
+      factor = MODE == FT_PREF && s.b >= a.pairs ? o.coef[1] : o.coef[0];
+      whole = ok;
+      a.done[blockIdx.x] = ok;
+    }
+  }
+  __syncthreads();
+  if (!whole) return;
+  const float2 k = factor;
+  rt = turn = 0;
+#pragma unroll
+  for (int j = 0; j < NV; ++j) {
+    if (rt < row_turns) {
+      const int r = rt * ngroups + group, t = 4 * (turn * G + lane);
+      const int left = r < s.rows ? min(4, len - t) : 0;
+      if (left > 0) {
+        const float c = MIX ? mix[r].x : 1.f, kz = k.x * c, kq = k.y * c;
+        float g[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) g[i] = TWO ? fmaf(kq, far[TWO ? j : 0][i], kz * res[j][i]) : kz * res[j][i];
+        store_some(pg + (int64_t)r * a.T + t, left, g);
+      }
+      if (++turn == turns) { turn = 0; ++rt; }
+    }
+  }
+}
+
 // workgroups [0, spans): the gradient of the network's output; the ones behind them: one channel's logit each
 template <int MODE, bool MIX, bool REF, typename T>
-__global__ void __launch_bounds__(FT_THREADS) grad_kernel(FtArgs a, int spans) {
+__global__ void __launch_bounds__(FT_THREADS) grad_kernel(FtArgs a, int spans) {   // a.done: spans that are in d_out already, for dloss = 1
   __shared__ float2 mix[FT_ROWS];
   __shared__ double red[FT_THREADS / 64];
   const int tid = threadIdx.x;
@@ -269,7 +461,8 @@ __global__ void __launch_bounds__(FT_THREADS) grad_kernel(FtArgs a, int spans) {
     }
     return;
   }
-  const Span s = span_of(a, blockIdx.x);
+  if (a.done && up == 1.f && a.done[blockIdx.x]) return;
+  const Span s = span_of<MODE>(a, blockIdx.x);
   const int G = 1 << a.log_g, lane = tid & (G - 1), group = tid >> a.log_g, ngroups = FT_THREADS >> a.log_g;
   const bool used = takes_part<MODE>(a, s.b);
   if (MIX && used) mix_rows(a, s, mix);
@@ -322,9 +515,22 @@ __global__ void __launch_bounds__(FT_THREADS) grad_kernel(FtArgs a, int spans) {
 template <int MODE, bool MIX, bool REF>
 int launch_sums_t(const FtArgs& a, int dt, hipStream_t s) {
   const dim3 grid((unsigned)(a.B * a.wps));
+  const int rows = MODE == FT_PREF ? a.pairs : a.B;
+  if (a.fused) {
+    constexpr int NV = (MODE == FT_POLICY && REF) ? FT_VECS / 2 : FT_VECS;
+    const int64_t places = 2ll * a.B * a.wps;
+    FtArgs f = a;
+    f.polls = g_polls;
+    hipLaunchKernelGGL((open_kernel<MODE>), dim3((unsigned)std::min<int64_t>(cdiv64(places, FT_THREADS), 256)), dim3(FT_THREADS), 0, s, a, places, rows);
+    if (dt == DT_F32) hipLaunchKernelGGL((fused_kernel<MODE, MIX, REF, float, NV>), grid, dim3(FT_THREADS), 0, s, f);
+    else hipLaunchKernelGGL((fused_kernel<MODE, MIX, REF, bf16_t, NV>), grid, dim3(FT_THREADS), 0, s, f);
+    hipLaunchKernelGGL((rows_kernel<MODE>), dim3((unsigned)rows), dim3(FT_THREADS), 0, s, a);
+    HIP_TRY(hipGetLastError());
+    return DDMI_OK;
+  }
   if (dt == DT_F32) hipLaunchKernelGGL((sums_kernel<MODE, MIX, REF, float>), grid, dim3(FT_THREADS), 0, s, a);
   else hipLaunchKernelGGL((sums_kernel<MODE, MIX, REF, bf16_t>), grid, dim3(FT_THREADS), 0, s, a);
-  hipLaunchKernelGGL((rows_kernel<MODE>), dim3((unsigned)(MODE == FT_PREF ? a.pairs : a.B)), dim3(FT_THREADS), 0, s, a);
+  hipLaunchKernelGGL((rows_kernel<MODE>), dim3((unsigned)rows), dim3(FT_THREADS), 0, s, a);
   HIP_TRY(hipGetLastError());
   return DDMI_OK;
 }
@@ -339,15 +545,10 @@ int launch_grad_t(const FtArgs& a, int dt, hipStream_t s) {
 }
 }  // namespace
 
-// Rows are split so that a workgroup has about 8 192 values (16 vectors of four a thread) where there are enough of them for 1 024
-// workgroups, fewer (down to 1 024) where there are not; G lanes share a row, as many as leave each at least two vectors of it.
-int ft_plan(FtArgs* a, int B, int C, int64_t HW, bool mixed) {
-  a->B = B;
-  a->C = mixed ? C : 1;                       // without a logit nothing depends on the channel: a sample is one row
-  a->T = mixed ? HW : HW * C;
-  const double all = (double)B * C * (double)HW;
-  int64_t want = 8192;
-  while (want > 1024 && all / (double)want < 1024.0) want >>= 1;
+// Two passes: rows are split so that a workgroup has about 8 192 values (16 vectors of four a thread) where there are enough of them for
+// 1 024 workgroups, fewer (down to 1 024) where there are not; G lanes share a row, as many as leave each at least two vectors of it.
+// One pass (`keep` vectors a thread stay in registers): a workgroup takes what fills them.
+static void ft_split(FtArgs* a, int64_t want) {
   if (a->T > want) {
     a->nseg = (int)std::min<int64_t>(cdiv64(a->T, want), 1 << 20);
     a->seg = cdiv64(cdiv64(a->T, a->nseg), 4) * 4;
@@ -360,23 +561,49 @@ int ft_plan(FtArgs* a, int B, int C, int64_t HW, bool mixed) {
   }
   a->log_g = 0;
   while (a->log_g < 8 && ((int64_t)16 << a->log_g) <= std::min(a->seg, a->T)) ++a->log_g;
+}
+int ft_plan(FtArgs* a, int B, int C, int64_t HW, bool mixed, int rows_of, int keep) {
+  a->B = B;
+  a->C = mixed ? C : 1;                       // without a logit nothing depends on the channel: a sample is one row
+  a->T = mixed ? HW : HW * C;
+  const int64_t all = (int64_t)B * C * HW;
+  a->fused = 0;
+  if (keep > 0 && all >= FT_FUSED_LEAST) {
+    // whole turns of the groups over the rows, whole turns of the lanes over a row
+    ft_split(a, 1024ll * keep);
+    const int64_t turns = cdiv64(cdiv64(std::min(a->seg, a->T), 4), 1ll << a->log_g), groups = FT_THREADS >> a->log_g;
+    a->rows_per_wg = (int)std::max<int64_t>(1, std::min<int64_t>(a->rows_per_wg, keep / std::max<int64_t>(turns, 1) * groups));
+    const int64_t wps = cdiv64(a->C, a->rows_per_wg) * a->nseg;
+    // the spans that wait for each other are resident together with room to spare (two workgroups a compute unit), and the threads'
+    // registers are mostly in use
+    const double filled = (double)a->rows_per_wg * (double)std::min(a->seg, a->T) / (1024.0 * keep);
+    a->fused = wps * rows_of <= 256 && turns <= keep && filled >= 0.5;
+  }
+  if (!a->fused) {
+    int64_t want = 8192;
+    while (want > 1024 && (double)all / (double)want < 1024.0) want >>= 1;
+    ft_split(a, want);
+  }
   const int64_t wps = cdiv64(a->C, a->rows_per_wg) * a->nseg;
   if (wps * B > (1ll << 30) || (int64_t)B * a->C > (1ll << 40)) return ddmi_fail(DDMI_ERR_INVALID, "fine-tuning loss: too many values in one call");
   a->wps = (int)wps;
   return DDMI_OK;
 }
+void ft_set_polls(int n) { g_polls = n; }
 static size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
 size_t ft_workspace_bytes(const FtArgs& a) {
   const int wpg = a.log_g > 6 ? 1 << (a.log_g - 6) : 1;
   return 256 + up256((size_t)a.B * sizeof(float2)) + up256((size_t)a.B * sizeof(double)) + up256((size_t)a.B * a.wps * sizeof(double2)) +
-         up256((size_t)a.B * a.C * a.nseg * wpg * sizeof(double2));
+         up256((size_t)a.B * a.wps * sizeof(int)) + up256((size_t)a.B * a.C * a.nseg * wpg * sizeof(double2));
 }
 void ft_carve(FtArgs* a, void* ws) {
   unsigned char* p = (unsigned char*)ws;
-  a->counter = (unsigned*)p; p += 256;
+  a->counter = (unsigned*)p;
+  a->total = (double*)(p + 64); p += 256;
   a->coef = (float2*)p; p += up256((size_t)a->B * sizeof(float2));
   a->term = (double*)p; p += up256((size_t)a->B * sizeof(double));
   a->part = (double2*)p; p += up256((size_t)a->B * a->wps * sizeof(double2));
+  a->done = (int*)p; p += up256((size_t)a->B * a->wps * sizeof(int));
   a->chan = (double2*)p;
 }
 static double ft_bytes(const FtArgs& a, int mode, int dt, bool grad) {

@@ -121,6 +121,17 @@ class _Call:
         return torch.empty(_workspace_bytes(self.B, self.C, self.HW, self.tensors[5] is not None), dtype=torch.uint8, device=self.tensors[0].device)
 
 
+def _gradient_buffer(ctx, call):
+    """Where the forward call may leave the gradient for an upstream gradient of 1 (large batches: the inputs are then read once)."""
+    return torch.empty_like(call.tensors[0]) if ctx.needs_input_grad[0] or ctx.needs_input_grad[1] else None
+
+
+def _take_buffer(ctx, call):
+    """That buffer, for the first backward: it is the caller's afterwards, so a second one gets its own."""
+    d_out, ctx.d_out = ctx.d_out, None
+    return (d_out, _lib.GRAD_THIS) if d_out is not None else (torch.empty_like(call.tensors[0]), _lib.GRAD_OTHER)
+
+
 class PreferenceLossFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, model_out, mixing_logit, ref_out, x_t, noise, sqrt_1mac, ref_logit, weight, beta, label_smoothing):
@@ -130,8 +141,9 @@ class PreferenceLossFn(torch.autograd.Function):
         loss = torch.empty((), dtype=torch.float32, device=dev)
         margin = torch.empty((pairs,), dtype=torch.float32, device=dev)
         mse = torch.empty((2 * pairs,), dtype=torch.float32, device=dev)
+        d_out = ctx.d_out = _gradient_buffer(ctx, call)
         _lib.check(_lib.lib().ddmi_train_pref_loss(C.byref(call.struct()), pairs, noise.shape[0], beta, label_smoothing, ws.data_ptr(), ws.numel(),
-                                                   loss.data_ptr(), margin.data_ptr(), mse.data_ptr(), _lib.raw_stream(call.index)))
+                                                   loss.data_ptr(), margin.data_ptr(), mse.data_ptr(), _p(d_out), _lib.raw_stream(call.index)))
         # the gradient needs neither the reference's output nor its logit
         call.tensors = (call.tensors[0], None) + call.tensors[2:6] + (None, call.tensors[7])
         ctx.save_for_backward(ws, *call.tensors)
@@ -145,13 +157,13 @@ class PreferenceLossFn(torch.autograd.Function):
     def backward(ctx, g, _margin, _mse):
         ws, call = ctx.saved_tensors[0], ctx.call
         call.tensors = ctx.saved_tensors[1:]
-        d_out = torch.empty_like(call.tensors[0])
+        d_out, state = _take_buffer(ctx, call)
         d_logit = torch.empty(ctx.logit_shape, dtype=torch.float32, device=ws.device) if ctx.logit_shape else None
         pairs, noise_rows, beta, smoothing = ctx.meta
         g = g.contiguous()
         with _lib.on_device(call.index):
             _lib.check(_lib.lib().ddmi_train_pref_loss_bwd(C.byref(call.struct()), pairs, noise_rows, beta, smoothing, ws.data_ptr(), ws.numel(),
-                                                           g.data_ptr(), d_out.data_ptr(), _p(d_logit), _lib.raw_stream(call.index)))
+                                                           g.data_ptr(), state, d_out.data_ptr(), _p(d_logit), _lib.raw_stream(call.index)))
         call.tensors = None
         return (d_out, d_logit) + (None,) * 8
 
@@ -166,9 +178,10 @@ class PolicyLossFn(torch.autograd.Function):
         loss = torch.empty((), dtype=torch.float32, device=dev)
         logp, ratio, kl = torch.empty((3, B), dtype=torch.float32, device=dev).unbind(0)
         logp_old, advantage = logp_old.contiguous(), advantage.contiguous()
+        d_out = ctx.d_out = _gradient_buffer(ctx, call)
         _lib.check(_lib.lib().ddmi_train_policy_loss(C.byref(call.struct()), B, transition.data_ptr(), logp_old.data_ptr(), advantage.data_ptr(),
                                                      clip_range, kl_coef, ws.data_ptr(), ws.numel(), loss.data_ptr(), logp.data_ptr(), ratio.data_ptr(),
-                                                     kl.data_ptr(), _lib.raw_stream(call.index)))
+                                                     kl.data_ptr(), _p(d_out), _lib.raw_stream(call.index)))
         ctx.save_for_backward(ws, transition, *call.tensors)
         call.tensors = None
         ctx.call = call
@@ -180,12 +193,12 @@ class PolicyLossFn(torch.autograd.Function):
     def backward(ctx, g, *_stats):
         ws, transition, call = ctx.saved_tensors[0], ctx.saved_tensors[1], ctx.call
         call.tensors = ctx.saved_tensors[2:]
-        d_out = torch.empty_like(call.tensors[0])
+        d_out, state = _take_buffer(ctx, call)
         d_logit = torch.empty(ctx.logit_shape, dtype=torch.float32, device=ws.device) if ctx.logit_shape else None
         g = g.contiguous()
         with _lib.on_device(call.index):
             _lib.check(_lib.lib().ddmi_train_policy_loss_bwd(C.byref(call.struct()), call.B, transition.data_ptr(), ws.data_ptr(), ws.numel(),
-                                                             g.data_ptr(), d_out.data_ptr(), _p(d_logit), _lib.raw_stream(call.index)))
+                                                             g.data_ptr(), state, d_out.data_ptr(), _p(d_logit), _lib.raw_stream(call.index)))
         call.tensors = None
         return (d_out, d_logit) + (None,) * 11
 
@@ -273,5 +286,5 @@ def transition_log_prob(model_out, x_t, x_prev, transition, sqrt_1mac, mixing_lo
         ws, transition = call.workspace(), transition.detach().contiguous()
         logp = torch.empty((call.B,), dtype=torch.float32, device=model_out.device)
         _lib.check(_lib.lib().ddmi_train_policy_loss(C.byref(call.struct()), call.B, transition.data_ptr(), None, None, 0.0, 0.0, ws.data_ptr(), ws.numel(),
-                                                     None, logp.data_ptr(), None, None, _lib.raw_stream(call.index)))
+                                                     None, logp.data_ptr(), None, None, None, _lib.raw_stream(call.index)))
         return logp
