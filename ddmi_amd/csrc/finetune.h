@@ -5,7 +5,7 @@
 enum { FT_PREF = 0, FT_POLICY = 1 };
 #define FT_THREADS 256
 #define FT_VECS 16       // vectors of four residuals that a thread of the one-pass kernel keeps in registers
-#define FT_FUSED_LEAST (1ll << 21)   // values from which on one pass over the inputs is taken
+#define FT_CACHE_BYTES 268435456.0   // the last-level cache: an optimizer step that touches more goes past it
 #define FT_ROWS 512      // most rows (sample, channel) of one workgroup: their mixing coefficients sit in LDS
 
 struct FtArgs {

@@ -19,24 +19,38 @@ namespace {
 typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));            // rows of an odd plane start at any element
 typedef unsigned short u16x4u __attribute__((ext_vector_type(4), aligned(2)));
 
-__device__ __forceinline__ void load4(const float* p, float (&v)[4]) {
-  const f32x4u t = *reinterpret_cast<const f32x4u*>(p);
+// NT: past the caches.  One pass over a large batch leaves nothing in them that anyone finds again, and the memory runs faster without
+// (256 pairs of 64 x 64 x 64: 508 -> 473 us; 16 pairs: 62 -> 53)
+// (overloads, not a template: a deduced type would lose its alignment)
+#define FT_GET_PUT(V)                                                                                   \
+  template <bool NT> __device__ __forceinline__ V get(const V* p) {                                     \
+    if constexpr (NT) return __builtin_nontemporal_load(p);                                             \
+    else return *p;                                                                                     \
+  }                                                                                                     \
+  template <bool NT> __device__ __forceinline__ void put(V* p, V v) {                                   \
+    if constexpr (NT) __builtin_nontemporal_store(v, p);                                                \
+    else *p = v;                                                                                        \
+  }
+FT_GET_PUT(f32x4u)
+FT_GET_PUT(u16x4u)
+template <bool NT = false> __device__ __forceinline__ void load4(const float* p, float (&v)[4]) {
+  const f32x4u t = get<NT>(reinterpret_cast<const f32x4u*>(p));
   v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
 }
 __device__ __forceinline__ float bf16_bits(unsigned short u) { return __uint_as_float((unsigned)u << 16); }
-__device__ __forceinline__ void load4(const bf16_t* p, float (&v)[4]) {
-  const u16x4u t = *reinterpret_cast<const u16x4u*>(p);
+template <bool NT = false> __device__ __forceinline__ void load4(const bf16_t* p, float (&v)[4]) {
+  const u16x4u t = get<NT>(reinterpret_cast<const u16x4u*>(p));
   v[0] = bf16_bits(t.x); v[1] = bf16_bits(t.y); v[2] = bf16_bits(t.z); v[3] = bf16_bits(t.w);
 }
-__device__ __forceinline__ void store4(float* p, const float (&v)[4]) {
-  f32x4u t = {v[0], v[1], v[2], v[3]};
-  *reinterpret_cast<f32x4u*>(p) = t;
+template <bool NT = false> __device__ __forceinline__ void store4(float* p, const float (&v)[4]) {
+  const f32x4u t = {v[0], v[1], v[2], v[3]};
+  put<NT>(reinterpret_cast<f32x4u*>(p), t);
 }
-__device__ __forceinline__ void store4(bf16_t* p, const float (&v)[4]) {   // the gradient's one rounding, to the network output's own type
+template <bool NT = false> __device__ __forceinline__ void store4(bf16_t* p, const float (&v)[4]) {   // the gradient's one rounding, to the network output's own type
   u16x4u t;
   t.x = __builtin_bit_cast(unsigned short, (bf16_t)v[0]); t.y = __builtin_bit_cast(unsigned short, (bf16_t)v[1]);
   t.z = __builtin_bit_cast(unsigned short, (bf16_t)v[2]); t.w = __builtin_bit_cast(unsigned short, (bf16_t)v[3]);
-  *reinterpret_cast<u16x4u*>(p) = t;
+  put<NT>(reinterpret_cast<u16x4u*>(p), t);
 }
 
 // what a workgroup works on: rows [row0, row0 + rows) of sample b, values [t0, t1) of each
@@ -230,7 +244,7 @@ __global__ void __launch_bounds__(FT_THREADS) rows_kernel(FtArgs a) {
   __shared__ double red[FT_THREADS / 64];
   __shared__ int last;
   const int i = blockIdx.x, rows = gridDim.x, tid = threadIdx.x;
-  const double total = total_weight<MODE>(a, rows, red);
+  const double total = a.fused ? *a.total : total_weight<MODE>(a, rows, red);
   const bool used = takes_part<MODE>(a, i);
   const double w = used ? (a.weight ? (double)a.weight[i] : 1.0) / total : 0.0;
   RowOut o;
@@ -314,12 +328,12 @@ __device__ __forceinline__ bool await_sums(const FtArgs& a, int64_t first, int l
   return true;
 }
 template <typename T> __device__ __forceinline__ void load_some(const T* p, int left, float (&v)[4]) {
-  if (left == 4) { load4(p, v); return; }
+  if (left == 4) { load4<true>(p, v); return; }
 #pragma unroll
   for (int i = 0; i < 4; ++i) v[i] = i < left ? to_f32(p[i]) : 0.f;
 }
 template <typename T> __device__ __forceinline__ void store_some(T* p, int left, const float (&v)[4]) {
-  if (left == 4) { store4(p, v); return; }
+  if (left == 4) { store4<true>(p, v); return; }
 #pragma unroll
   for (int i = 0; i < 4; ++i) if (i < left) p[i] = from_f32<T>(v[i]);
 }
@@ -438,31 +452,11 @@ __global__ void __launch_bounds__(FT_THREADS, 2) fused_kernel(FtArgs a) {
   }
 }
 
-// workgroups [0, spans): the gradient of the network's output; the ones behind them: one channel's logit each
+// the gradient of one span, from the inputs
 template <int MODE, bool MIX, bool REF, typename T>
-__global__ void __launch_bounds__(FT_THREADS) grad_kernel(FtArgs a, int spans) {   // a.done: spans that are in d_out already, for dloss = 1
-  __shared__ float2 mix[FT_ROWS];
-  __shared__ double red[FT_THREADS / 64];
+__device__ __forceinline__ void grad_span(const FtArgs& a, int blk, float up, float2* mix) {
   const int tid = threadIdx.x;
-  const float up = a.dloss ? *a.dloss : 1.f;
-  if ((int)blockIdx.x >= spans) {
-    const int ch = (int)blockIdx.x - spans, per = a.nseg * (a.log_g > 6 ? 1 << (a.log_g - 6) : 1);
-    double s = 0.0;
-    for (int64_t j = tid; j < (int64_t)a.B * per; j += FT_THREADS) {
-      const int b = (int)(j / per);
-      const float2 k = a.coef[b];
-      const double2 p = a.chan[((int64_t)b * a.C + ch) * per + (j - (int64_t)b * per)];
-      s += k.x * p.x + k.y * p.y;
-    }
-    s = block_sum(s, red);
-    if (tid == 0) {
-      const double c = 1.0 / (1.0 + exp(-(double)a.logit[ch]));
-      a.d_logit[ch] = (float)(s * c * (1.0 - c) * (double)up);
-    }
-    return;
-  }
-  if (a.done && up == 1.f && a.done[blockIdx.x]) return;
-  const Span s = span_of<MODE>(a, blockIdx.x);
+  const Span s = span_of<MODE>(a, blk);
   const int G = 1 << a.log_g, lane = tid & (G - 1), group = tid >> a.log_g, ngroups = FT_THREADS >> a.log_g;
   const bool used = takes_part<MODE>(a, s.b);
   if (MIX && used) mix_rows(a, s, mix);
@@ -512,6 +506,37 @@ __global__ void __launch_bounds__(FT_THREADS) grad_kernel(FtArgs a, int spans) {
   }
 }
 
+// Workgroups [0, channels): one channel's logit each; the others take spans in turn.  a.done: which spans are in d_out already, for an
+// upstream gradient of 1.
+template <int MODE, bool MIX, bool REF, typename T>
+__global__ void __launch_bounds__(FT_THREADS) grad_kernel(FtArgs a, int spans, int channels) {
+  __shared__ float2 mix[FT_ROWS];
+  __shared__ double red[FT_THREADS / 64];
+  const int tid = threadIdx.x;
+  const float up = a.dloss ? *a.dloss : 1.f;
+  if ((int)blockIdx.x < channels) {
+    const int ch = (int)blockIdx.x, per = a.nseg * (a.log_g > 6 ? 1 << (a.log_g - 6) : 1);
+    double s = 0.0;
+    for (int64_t j = tid; j < (int64_t)a.B * per; j += FT_THREADS) {
+      const int b = (int)(j / per);
+      const float2 k = a.coef[b];
+      const double2 p = a.chan[((int64_t)b * a.C + ch) * per + (j - (int64_t)b * per)];
+      s += k.x * p.x + k.y * p.y;
+    }
+    s = block_sum(s, red);
+    if (tid == 0) {
+      const double c = 1.0 / (1.0 + exp(-(double)a.logit[ch]));
+      a.d_logit[ch] = (float)(s * c * (1.0 - c) * (double)up);
+    }
+    return;
+  }
+  for (int blk = (int)blockIdx.x - channels; blk < spans; blk += (int)gridDim.x - channels) {
+    if (a.done && up == 1.f && a.done[blk]) continue;
+    grad_span<MODE, MIX, REF, T>(a, blk, up, mix);
+    __syncthreads();                                    // the next span's coefficients take this one's place
+  }
+}
+
 template <int MODE, bool MIX, bool REF>
 int launch_sums_t(const FtArgs& a, int dt, hipStream_t s) {
   const dim3 grid((unsigned)(a.B * a.wps));
@@ -536,10 +561,10 @@ int launch_sums_t(const FtArgs& a, int dt, hipStream_t s) {
 }
 template <int MODE, bool MIX, bool REF>
 int launch_grad_t(const FtArgs& a, int dt, hipStream_t s) {
-  const int spans = a.B * a.wps;
-  const dim3 grid((unsigned)(spans + (MIX && a.d_logit ? a.C : 0)));
-  if (dt == DT_F32) hipLaunchKernelGGL((grad_kernel<MODE, MIX, REF, float>), grid, dim3(FT_THREADS), 0, s, a, spans);
-  else hipLaunchKernelGGL((grad_kernel<MODE, MIX, REF, bf16_t>), grid, dim3(FT_THREADS), 0, s, a, spans);
+  const int spans = a.B * a.wps, channels = MIX && a.d_logit ? a.C : 0;
+  const dim3 grid((unsigned)(channels + (a.done ? std::min(spans, 1024) : spans)));   // 1 024 look through what is most often done
+  if (dt == DT_F32) hipLaunchKernelGGL((grad_kernel<MODE, MIX, REF, float>), grid, dim3(FT_THREADS), 0, s, a, spans, channels);
+  else hipLaunchKernelGGL((grad_kernel<MODE, MIX, REF, bf16_t>), grid, dim3(FT_THREADS), 0, s, a, spans, channels);
   HIP_TRY(hipGetLastError());
   return DDMI_OK;
 }
@@ -568,16 +593,17 @@ int ft_plan(FtArgs* a, int B, int C, int64_t HW, bool mixed, int rows_of, int ke
   a->T = mixed ? HW : HW * C;
   const int64_t all = (int64_t)B * C * HW;
   a->fused = 0;
-  if (keep > 0 && all >= FT_FUSED_LEAST) {
+  if (keep > 0) {
     // whole turns of the groups over the rows, whole turns of the lanes over a row
     ft_split(a, 1024ll * keep);
     const int64_t turns = cdiv64(cdiv64(std::min(a->seg, a->T), 4), 1ll << a->log_g), groups = FT_THREADS >> a->log_g;
     a->rows_per_wg = (int)std::max<int64_t>(1, std::min<int64_t>(a->rows_per_wg, keep / std::max<int64_t>(turns, 1) * groups));
     const int64_t wps = cdiv64(a->C, a->rows_per_wg) * a->nseg;
-    // the spans that wait for each other are resident together with room to spare (two workgroups a compute unit), and the threads'
-    // registers are mostly in use
+    // One pass pays from 384 workgroups on, one and a half for each compute unit (64 x 64 x 64 latents, two passes | one: 8 pairs 40 | 48 us,
+    // 12: 52 | 50, 16: 65 | 53, 256: 680 | 477; transitions with KL 8: 33 | 39, 12: 43 | 41, 512: 894 | 533).  The spans that wait for each
+    // other are resident together with room to spare (two workgroups a compute unit), and the threads' registers are mostly in use.
     const double filled = (double)a->rows_per_wg * (double)std::min(a->seg, a->T) / (1024.0 * keep);
-    a->fused = wps * rows_of <= 256 && turns <= keep && filled >= 0.5;
+    a->fused = wps * B >= 384 && wps * rows_of <= 256 && turns <= keep && filled >= 0.5;
   }
   if (!a->fused) {
     int64_t want = 8192;

@@ -14,8 +14,8 @@ DEV = "cuda:0"
 # (B, C, T): one value; odd planes; more rows than a workgroup holds; rows of one value; several segments a row; rows shared by four waves;
 # enough values for the largest workgroups
 SHAPES = [(2, 1, 1), (2, 64, 64), (6, 5, 7), (4, 3, 1), (2, 1100, 3), (2, 2, 20001), (6, 48, 1295), (4, 7, 4096), (2, 64, 65536)]
-# the residuals kept in registers (at least 2^21 values): whole turns; odd planes; short rows; segments of long odd rows
-LARGE = [(16, 64, 2048), (40, 33, 1601), (150, 190, 77), (22, 3, 33001), (8, 64, 4100)]
+# the residuals kept in registers (from 384 workgroups on): whole turns; odd planes; short rows; segments of long odd rows
+LARGE = [(48, 64, 2048), (80, 33, 2501), (500, 190, 77), (140, 3, 33001), (36, 64, 4100)]
 SHAPES += LARGE
 
 
@@ -58,7 +58,7 @@ def test_policy_loss(B, C, T, dtype, mixed, kl):
 @pytest.mark.parametrize("op", ["pref", "policy"])
 @pytest.mark.parametrize("weight", ["some", "none_left"])
 @pytest.mark.parametrize("mixed", [True, False])
-@pytest.mark.parametrize("B,C,T", [(14, 5, 33), (26, 50, 1701)])
+@pytest.mark.parametrize("B,C,T", [(14, 5, 33), (80, 50, 1701)])
 def test_rows_left_out(op, weight, mixed, B, C, T):
     """Rows of weight 0 hold NaN and infinities: none of it may show, their gradients are zeros, and the mean is over the others."""
     d = R.make(op, B, C, T, weight=weight, mixed=mixed, seed=3, device=DEV)
@@ -154,7 +154,7 @@ def test_gradient_against_differences(op):
 
 
 @pytest.mark.parametrize("op", ["pref", "policy"])
-@pytest.mark.parametrize("B,C,T", [(6, 5, 33), (16, 64, 2051)])
+@pytest.mark.parametrize("B,C,T", [(6, 5, 33), (50, 64, 2051)])
 def test_upstream_gradient_and_second_backward(op, B, C, T):
     d = R.make(op, B, C, T, seed=4, device=DEV)
     one, three = call(op, d), call(op, d, 4.0)
@@ -170,7 +170,7 @@ def test_upstream_gradient_and_second_backward(op, B, C, T):
 
 
 @pytest.mark.parametrize("op", ["pref", "policy"])
-@pytest.mark.parametrize("B,C,T", [(8, 16, 1025), (40, 33, 1601)])
+@pytest.mark.parametrize("B,C,T", [(8, 16, 1025), (80, 33, 2501)])
 def test_same_bits_on_every_run_and_stream(op, B, C, T):
     d = R.make(op, B, C, T, seed=6, device=DEV)
     a = call(op, d)
@@ -185,7 +185,7 @@ def test_same_bits_on_every_run_and_stream(op, B, C, T):
 
 
 @pytest.mark.parametrize("op", ["pref", "policy"])
-@pytest.mark.parametrize("B,C,T", [(6, 7, 131), (40, 33, 1601)])
+@pytest.mark.parametrize("B,C,T", [(6, 7, 131), (80, 33, 2501)])
 def test_captured_and_replayed(op, B, C, T):
     """Two captured forwards + backwards of different inputs, replayed by turns with eager work between: each replay is the eager result."""
     sets = [R.make(op, B, C, T, seed=s, device=DEV) for s in (1, 2, 3, 4)]
