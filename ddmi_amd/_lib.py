@@ -68,7 +68,6 @@ class StepCoefs(C.Structure):
 
 
 DTYPE_F32, DTYPE_BF16 = 0, 1
-GRAD_NONE, GRAD_OTHER, GRAD_THIS = 0, 1, 2
 
 
 class LossIn(C.Structure):
@@ -194,10 +193,9 @@ SYMBOLS = {
     "ddmi_train_ema": (_I, [_VP, _VP, C.c_int64, _F, _VP]),
     # fine-tuning (include/ddmi_hip.h "Fine-tuning")
     "ddmi_train_loss_workspace_bytes": (_I, [_I, _I, C.c_int64, _I, C.POINTER(C.c_size_t)]),
-    "ddmi_train_pref_loss": (_I, [C.POINTER(LossIn), _I, _I, C.c_double, C.c_double, _VP, C.c_size_t, _VP, _VP, _VP, _VP, _VP]),
-    "ddmi_train_pref_loss_bwd": (_I, [C.POINTER(LossIn), _I, _I, C.c_double, C.c_double, _VP, C.c_size_t, _VP, _I, _VP, _VP, _VP]),
-    "ddmi_train_policy_loss": (_I, [C.POINTER(LossIn), _I, _VP, _VP, _VP, C.c_double, C.c_double, _VP, C.c_size_t, _VP, _VP, _VP, _VP, _VP, _VP]),
-    "ddmi_train_policy_loss_bwd": (_I, [C.POINTER(LossIn), _I, _VP, _VP, C.c_size_t, _VP, _I, _VP, _VP, _VP]),
+    "ddmi_train_pref_loss": (_I, [C.POINTER(LossIn), _I, _I, C.c_double, C.c_double, _VP, _VP, C.c_size_t] + [_VP] * 6),
+    "ddmi_train_policy_loss": (_I, [C.POINTER(LossIn), _I, _VP, _VP, _VP, C.c_double, C.c_double, _VP, _VP, C.c_size_t] + [_VP] * 7),
+    "ddmi_train_loss_scale": (_I, [_VP, _VP, _I, C.c_int64, _VP, _I, _VP]),
     "ddmi_debug_loss_polls": (_I, [_I]),
     "ddmi_train_adamw_multi": (_I, [_VP, _I, C.c_double, C.c_double, C.c_double, C.c_double, C.c_uint32, _I, _I, _I, _VP]),
 }

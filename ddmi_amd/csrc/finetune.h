@@ -26,7 +26,7 @@ struct FtArgs {
   // outputs
   float* loss;
   float* row_out[3];         // margin, mse | logp, ratio, kl
-  const float* dloss;        // upstream gradient, a device scalar
+  const float* dloss;        // upstream gradient, a device scalar (null: 1)
   void* d_out;
   float* d_logit;
   // plan
@@ -48,6 +48,7 @@ size_t ft_workspace_bytes(const FtArgs& a);
 void ft_carve(FtArgs* a, void* ws);
 void ft_set_polls(int n);
 int launch_ft_sums(const FtArgs& a, int mode, int dt, hipStream_t s);
+int launch_ft_scale(const float* dloss, void* g, int dt, int64_t n, float* d_logit, int C, hipStream_t s);
 int launch_ft_grad(const FtArgs& a, int mode, int dt, hipStream_t s);
 
 #define ADAMW_BLOCK 256      // values of a tensor that share one scale of the 8-bit moments

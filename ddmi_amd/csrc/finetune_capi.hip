@@ -21,21 +21,9 @@ int common_args(FtArgs* a, const ddmi_loss_in* in, int B, int rows_of, int keep,
   a->logit = in->mixing_logit; a->ref_logit = in->ref_mixing_logit; a->weight = in->weight;
   return DDMI_OK;
 }
-// the gradient needs neither the reference's output nor its logit (its residual is the trained network's alone)
-int pref_args(FtArgs* a, const ddmi_loss_in* in, int pairs, int noise_rows, double beta, double label_smoothing, bool grad, bool kept, void* ws, size_t ws_bytes) {
-  DDMI_REQUIRE(in && (grad || in->ref_out) && pairs > 0 && pairs <= (1 << 29), "pref_loss: null argument or no pairs");
-  DDMI_REQUIRE(noise_rows == pairs || noise_rows == 2 * pairs, "pref_loss: the noise has a row for each pair or for each sample");
-  DDMI_REQUIRE(label_smoothing >= 0.0 && label_smoothing <= 1.0 && beta == beta, "pref_loss: label_smoothing in [0, 1], beta a number");
-  DDMI_TRY(common_args(a, in, 2 * pairs, 2, kept ? FT_VECS : 0, ws, ws_bytes, "pref_loss"));
-  if (!in->mixing_logit) a->x = nullptr;      // not read
-  a->pairs = pairs; a->second_rows = noise_rows; a->beta = beta; a->smoothing = label_smoothing;
-  return DDMI_OK;
-}
-int policy_args(FtArgs* a, const ddmi_loss_in* in, int B, const float* transition, bool kept, void* ws, size_t ws_bytes) {
-  DDMI_REQUIRE(in && transition && in->x_t, "policy_loss: null argument");
-  DDMI_TRY(common_args(a, in, B, 1, kept ? (in->ref_out ? FT_VECS / 2 : FT_VECS) : 0, ws, ws_bytes, "policy_loss"));
-  a->pairs = B; a->second_rows = B; a->transition = transition;
-  return DDMI_OK;
+int run(FtArgs* a, int mode, int out_dtype, hipStream_t s) {
+  DDMI_TRY(launch_ft_sums(*a, mode, internal_dt(out_dtype), s));
+  return a->d_out ? launch_ft_grad(*a, mode, internal_dt(out_dtype), s) : DDMI_OK;
 }
 }  // namespace
 
@@ -53,51 +41,41 @@ int ddmi_train_loss_workspace_bytes(int B, int C, int64_t HW, int mixed, size_t*
   return DDMI_OK;
 }
 
-int ddmi_train_pref_loss(const ddmi_loss_in* in, int pairs, int noise_rows, double beta, double label_smoothing, void* ws, size_t ws_bytes, float* loss,
-                         float* margin, float* mse, void* d_model_out, void* stream) {
+int ddmi_train_pref_loss(const ddmi_loss_in* in, int pairs, int noise_rows, double beta, double label_smoothing, const float* dloss, void* ws,
+                         size_t ws_bytes, float* loss, float* margin, float* mse, void* d_model_out, float* d_logit, void* stream) {
   FtArgs a{};
+  DDMI_REQUIRE(in && in->ref_out && pairs > 0 && pairs <= (1 << 29), "pref_loss: null argument or no pairs");
   DDMI_REQUIRE(loss && margin && mse, "pref_loss: null output");
-  DDMI_TRY(pref_args(&a, in, pairs, noise_rows, beta, label_smoothing, false, d_model_out != nullptr, ws, ws_bytes));
-  a.d_out = d_model_out;
-  a.loss = loss; a.row_out[0] = margin; a.row_out[1] = mse;
-  return launch_ft_sums(a, FT_PREF, internal_dt(in->out_dtype), (hipStream_t)stream);
-}
-int ddmi_train_pref_loss_bwd(const ddmi_loss_in* in, int pairs, int noise_rows, double beta, double label_smoothing, void* ws, size_t ws_bytes,
-                             const float* dloss, int state, void* d_model_out, float* d_logit, void* stream) {
-  FtArgs a{};
-  DDMI_REQUIRE(d_model_out && state >= DDMI_GRAD_NONE && state <= DDMI_GRAD_THIS, "pref_loss_bwd: null output or bad state");
-  DDMI_TRY(pref_args(&a, in, pairs, noise_rows, beta, label_smoothing, true, state != DDMI_GRAD_NONE, ws, ws_bytes));
-  if (!a.fused || state != DDMI_GRAD_THIS) a.done = nullptr;
-  DDMI_REQUIRE(!d_logit || in->mixing_logit, "pref_loss_bwd: a logit's gradient without a logit");
-  a.dloss = dloss; a.d_out = d_model_out; a.d_logit = d_logit;
-  return launch_ft_grad(a, FT_PREF, internal_dt(in->out_dtype), (hipStream_t)stream);
+  DDMI_REQUIRE(noise_rows == pairs || noise_rows == 2 * pairs, "pref_loss: the noise has a row for each pair or for each sample");
+  DDMI_REQUIRE(label_smoothing >= 0.0 && label_smoothing <= 1.0 && beta == beta, "pref_loss: label_smoothing in [0, 1], beta a number");
+  DDMI_REQUIRE(!d_logit || (in->mixing_logit && d_model_out), "pref_loss: d_logit goes with mixing_logit and d_model_out");
+  DDMI_TRY(common_args(&a, in, 2 * pairs, 2, d_model_out ? FT_VECS : 0, ws, ws_bytes, "pref_loss"));
+  if (!in->mixing_logit) a.x = nullptr;      // not read
+  a.pairs = pairs; a.second_rows = noise_rows; a.beta = beta; a.smoothing = label_smoothing;
+  a.loss = loss; a.row_out[0] = margin; a.row_out[1] = mse; a.dloss = dloss; a.d_out = d_model_out; a.d_logit = d_logit;
+  return run(&a, FT_PREF, in->out_dtype, (hipStream_t)stream);
 }
 int ddmi_train_policy_loss(const ddmi_loss_in* in, int B, const float* transition, const float* logp_old, const float* advantage, double clip_range,
-                           double kl_coef, void* ws, size_t ws_bytes, float* loss, float* logp, float* ratio, float* kl, void* d_model_out,
-                           void* stream) {
+                           double kl_coef, const float* dloss, void* ws, size_t ws_bytes, float* loss, float* logp, float* ratio, float* kl,
+                           void* d_model_out, float* d_logit, void* stream) {
   FtArgs a{};
-  DDMI_REQUIRE(logp, "policy_loss: null output");
+  DDMI_REQUIRE(in && transition && in->x_t && logp, "policy_loss: null argument");
   DDMI_REQUIRE(!logp_old || (advantage && loss && ratio && kl), "policy_loss: null argument");
   DDMI_REQUIRE(clip_range >= 0.0 && kl_coef == kl_coef, "policy_loss: clip_range >= 0, kl_coef a number");
-  DDMI_REQUIRE(kl_coef == 0.0 || (in && in->ref_out), "policy_loss: a KL term needs the reference's output");
+  DDMI_REQUIRE(kl_coef == 0.0 || in->ref_out, "policy_loss: a KL term needs the reference's output");
   DDMI_REQUIRE(logp_old || !d_model_out, "policy_loss: a gradient of the log-density alone is not offered");
-  DDMI_TRY(policy_args(&a, in, B, transition, d_model_out != nullptr, ws, ws_bytes));
-  a.d_out = d_model_out;
+  DDMI_REQUIRE(!d_logit || (in->mixing_logit && d_model_out), "policy_loss: d_logit goes with mixing_logit and d_model_out");
+  DDMI_TRY(common_args(&a, in, B, 1, d_model_out ? (in->ref_out ? FT_VECS / 2 : FT_VECS) : 0, ws, ws_bytes, "policy_loss"));
+  a.pairs = B; a.second_rows = B; a.transition = transition;
   a.logp_old = logp_old; a.advantage = advantage; a.clip = clip_range; a.kl_coef = kl_coef;
   a.loss = logp_old ? loss : nullptr; a.row_out[0] = logp; a.row_out[1] = ratio; a.row_out[2] = kl;
-  return launch_ft_sums(a, FT_POLICY, internal_dt(in->out_dtype), (hipStream_t)stream);
-}
-int ddmi_train_policy_loss_bwd(const ddmi_loss_in* in, int B, const float* transition, void* ws, size_t ws_bytes, const float* dloss, int state,
-                               void* d_model_out, float* d_logit, void* stream) {
-  FtArgs a{};
-  DDMI_REQUIRE(d_model_out && state >= DDMI_GRAD_NONE && state <= DDMI_GRAD_THIS, "policy_loss_bwd: null output or bad state");
-  DDMI_TRY(policy_args(&a, in, B, transition, state != DDMI_GRAD_NONE, ws, ws_bytes));
-  if (!a.fused || state != DDMI_GRAD_THIS) a.done = nullptr;
-  DDMI_REQUIRE(!d_logit || in->mixing_logit, "policy_loss_bwd: a logit's gradient without a logit");
   a.dloss = dloss; a.d_out = d_model_out; a.d_logit = d_logit;
-  return launch_ft_grad(a, FT_POLICY, internal_dt(in->out_dtype), (hipStream_t)stream);
+  return run(&a, FT_POLICY, in->out_dtype, (hipStream_t)stream);
 }
-
+int ddmi_train_loss_scale(const float* dloss, void* d_model_out, int out_dtype, int64_t n, float* d_logit, int C, void* stream) {
+  DDMI_REQUIRE(dloss && d_model_out && n > 0 && dtype_ok(out_dtype) && (!d_logit || C > 0), "loss_scale: bad arguments");
+  return launch_ft_scale(dloss, d_model_out, internal_dt(out_dtype), n, d_logit, C, (hipStream_t)stream);
+}
 int ddmi_debug_loss_polls(int n) {
   DDMI_REQUIRE(n >= 0, "debug_loss_polls: not negative");
   ft_set_polls(n);

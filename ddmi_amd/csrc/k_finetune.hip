@@ -7,7 +7,8 @@
 //   policy:      z = (x_prev - A x_t) - E eps,     sums  z^2,  (eps - eps_ref)^2,  z (o - m),  (eps - eps_ref) (o - m)
 // One scalar (two with KL) a sample follows from the sums over ALL of its values, and only then is the gradient known:
 //   d loss / d o = c (k z' + q far).  So: sums_kernel (reads every input once), rows_kernel (a workgroup a pair / transition: the scalar
-//   work in 64 bits, the last one to finish adds up the loss), grad_kernel (reads again what the gradient needs, writes it).
+//   work in 64 bits, the last one to finish adds up the loss), grad_kernel (reads again what the gradient needs, writes it).  A large
+//   batch is read once: fused_kernel below.
 // Factors are rounded in fp32, products and sums are held in fp64: a margin is the difference of two nearly equal errors times
 // beta ~ 10^3, and a logit's gradient a sum of either sign over the batch.  No float atomics: every sum has a fixed order.
 #include <algorithm>
@@ -286,7 +287,7 @@ __global__ void __launch_bounds__(FT_THREADS) rows_kernel(FtArgs a) {
 // gradient from the residuals in its registers: every input is read once.  The sums' own bits are the signal - open_kernel fills their
 // places with a NaN that no sum is stored as - so publishing is two relaxed agent-scope stores, with no fence and no counter.  The wait is
 // bounded: a workgroup whose neighbours do not show up (other kernels hold the compute units) leaves its span undone, and grad_kernel,
-// which runs after it in any case, computes what is not done.
+// which runs after it in any case (the logits' gradients need every sample's factors), computes what is not done.
 constexpr unsigned long long FT_OPEN = 0xFFFFFFFFFFFFFFFFull;
 int g_polls = 1 << 12;                  // some milliseconds; the spans of a row start within microseconds of each other
 
@@ -426,7 +427,9 @@ __global__ void __launch_bounds__(FT_THREADS, 2) fused_kernel(FtArgs a) {
     if (MODE == FT_PREF && ok) ok = await_sums(a, first + a.wps, tid, polls, s1);
     const RowOut o = MODE == FT_PREF ? pref_row(a, true, w, s0, s1) : policy_row(a, true, w, row, s0);
     if (tid == 0) {
-      factor = MODE == FT_PREF && s.b >= a.pairs ? o.coef[1] : o.coef[0];
+      const float up = a.dloss ? *a.dloss : 1.f;
+      const float2 k = MODE == FT_PREF && s.b >= a.pairs ? o.coef[1] : o.coef[0];
+      factor = make_float2(k.x * up, k.y * up);
       whole = ok;
       a.done[blockIdx.x] = ok;
     }
@@ -506,8 +509,7 @@ __device__ __forceinline__ void grad_span(const FtArgs& a, int blk, float up, fl
   }
 }
 
-// Workgroups [0, channels): one channel's logit each; the others take spans in turn.  a.done: which spans are in d_out already, for an
-// upstream gradient of 1.
+// Workgroups [0, channels): one channel's logit each; the others take spans in turn, but for those that are in d_out already.
 template <int MODE, bool MIX, bool REF, typename T>
 __global__ void __launch_bounds__(FT_THREADS) grad_kernel(FtArgs a, int spans, int channels) {
   __shared__ float2 mix[FT_ROWS];
@@ -531,7 +533,7 @@ __global__ void __launch_bounds__(FT_THREADS) grad_kernel(FtArgs a, int spans, i
     return;
   }
   for (int blk = (int)blockIdx.x - channels; blk < spans; blk += (int)gridDim.x - channels) {
-    if (a.done && up == 1.f && a.done[blk]) continue;
+    if (a.fused && a.done[blk]) continue;
     grad_span<MODE, MIX, REF, T>(a, blk, up, mix);
     __syncthreads();                                    // the next span's coefficients take this one's place
   }
@@ -562,11 +564,28 @@ int launch_sums_t(const FtArgs& a, int dt, hipStream_t s) {
 template <int MODE, bool MIX, bool REF>
 int launch_grad_t(const FtArgs& a, int dt, hipStream_t s) {
   const int spans = a.B * a.wps, channels = MIX && a.d_logit ? a.C : 0;
-  const dim3 grid((unsigned)(channels + (a.done ? std::min(spans, 1024) : spans)));   // 1 024 look through what is most often done
+  const dim3 grid((unsigned)(channels + (a.fused ? std::min(spans, 1024) : spans)));   // 1 024 look through what is most often done
   if (dt == DT_F32) hipLaunchKernelGGL((grad_kernel<MODE, MIX, REF, float>), grid, dim3(FT_THREADS), 0, s, a, spans, channels);
   else hipLaunchKernelGGL((grad_kernel<MODE, MIX, REF, bf16_t>), grid, dim3(FT_THREADS), 0, s, a, spans, channels);
   HIP_TRY(hipGetLastError());
   return DDMI_OK;
+}
+// the gradients times an upstream gradient that is not 1
+template <typename T>
+__global__ void __launch_bounds__(FT_THREADS) scale_kernel(const float* __restrict__ dloss, T* __restrict__ g, int64_t n, float* __restrict__ d_logit, int C) {
+  const float up = *dloss;
+  if (up == 1.f) return;
+  const int64_t first = (int64_t)blockIdx.x * FT_THREADS + threadIdx.x, step = (int64_t)gridDim.x * FT_THREADS;
+  for (int64_t v = first; v < n / 4; v += step) {
+    float x[4];
+    load4(g + 4 * v, x);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x[i] *= up;
+    store4(g + 4 * v, x);
+  }
+  for (int64_t i = n / 4 * 4 + first; i < n; i += step) g[i] = from_f32<T>(to_f32(g[i]) * up);
+  if (d_logit)
+    for (int64_t i = first; i < C; i += step) d_logit[i] *= up;
 }
 }  // namespace
 
@@ -641,6 +660,13 @@ int launch_ft_sums(const FtArgs& a, int mode, int dt, hipStream_t s) {
   if (mode == FT_PREF) return a.logit ? launch_sums_t<FT_PREF, true, true>(a, dt, s) : launch_sums_t<FT_PREF, false, true>(a, dt, s);
   if (a.ref) return a.logit ? launch_sums_t<FT_POLICY, true, true>(a, dt, s) : launch_sums_t<FT_POLICY, false, true>(a, dt, s);
   return a.logit ? launch_sums_t<FT_POLICY, true, false>(a, dt, s) : launch_sums_t<FT_POLICY, false, false>(a, dt, s);
+}
+int launch_ft_scale(const float* dloss, void* g, int dt, int64_t n, float* d_logit, int C, hipStream_t s) {
+  const dim3 grid((unsigned)std::min<int64_t>(cdiv64(n, 4 * FT_THREADS), 2048));
+  if (dt == DT_F32) hipLaunchKernelGGL((scale_kernel<float>), grid, dim3(FT_THREADS), 0, s, dloss, (float*)g, n, d_logit, C);
+  else hipLaunchKernelGGL((scale_kernel<bf16_t>), grid, dim3(FT_THREADS), 0, s, dloss, (bf16_t*)g, n, d_logit, C);
+  HIP_TRY(hipGetLastError());
+  return DDMI_OK;
 }
 // the preference gradient does not need the reference's output: its residual is the trained network's alone
 int launch_ft_grad(const FtArgs& a, int mode, int dt, hipStream_t s) {

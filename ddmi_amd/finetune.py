@@ -121,86 +121,85 @@ class _Call:
         return torch.empty(_workspace_bytes(self.B, self.C, self.HW, self.tensors[5] is not None), dtype=torch.uint8, device=self.tensors[0].device)
 
 
-def _gradient_buffer(ctx, call):
-    """Where the forward call may leave the gradient for an upstream gradient of 1 (large batches: the inputs are then read once)."""
-    return torch.empty_like(call.tensors[0]) if ctx.needs_input_grad[0] or ctx.needs_input_grad[1] else None
+class _LossFn(torch.autograd.Function):
+    """What the two losses share: `launch` computes loss, statistics and, along with them, the gradients for an upstream gradient of 1.  The
+    first backward hands those out - multiplied in place when the upstream gradient, which only the device knows, is another - and a later
+    one (retain_graph) computes them again from the saved inputs."""
+
+    @classmethod
+    def _forward(cls, ctx, call, extra, args):
+        ctx.mixed = call.tensors[5] is not None and ctx.needs_input_grad[1]
+        grads = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
+        outs, ctx.grads = cls.launch(call, extra, args, None, grads, ctx.mixed)
+        if grads:
+            ctx.save_for_backward(*call.tensors, *extra)
+            ctx.args, ctx.index = args, call.index
+        ctx.mark_non_differentiable(*outs[1:])
+        return outs
+
+    @classmethod
+    def _backward(cls, ctx, g):
+        if g.dtype != torch.float32 or not g.is_contiguous():
+            g = g.float().contiguous()
+        with _lib.on_device(ctx.index):
+            if ctx.grads is not None:
+                (d_out, d_logit), ctx.grads = ctx.grads, None
+                _lib.check(_lib.lib().ddmi_train_loss_scale(g.data_ptr(), d_out.data_ptr(), _OUT_TYPES[d_out.dtype], d_out.numel(), _p(d_logit),
+                                                            0 if d_logit is None else d_logit.numel(), _lib.raw_stream(ctx.index)))
+            else:
+                saved = ctx.saved_tensors
+                d_out, d_logit = cls.launch(_Call(*saved[:8]), saved[8:], ctx.args, g, True, ctx.mixed)[1]
+        return d_out, d_logit
+
+    @staticmethod
+    def buffers(call, grads, mixed):
+        d_out = torch.empty_like(call.tensors[0]) if grads else None
+        return d_out, torch.empty_like(call.tensors[5]) if mixed else None
 
 
-def _take_buffer(ctx, call):
-    """That buffer, for the first backward: it is the caller's afterwards, so a second one gets its own."""
-    d_out, ctx.d_out = ctx.d_out, None
-    return (d_out, _lib.GRAD_THIS) if d_out is not None else (torch.empty_like(call.tensors[0]), _lib.GRAD_OTHER)
-
-
-class PreferenceLossFn(torch.autograd.Function):
+class PreferenceLossFn(_LossFn):
     @staticmethod
     def forward(ctx, model_out, mixing_logit, ref_out, x_t, noise, sqrt_1mac, ref_logit, weight, beta, label_smoothing):
         call = _Call(model_out, ref_out, x_t, noise, sqrt_1mac, mixing_logit, ref_logit, weight)
-        dev, pairs = model_out.device, model_out.shape[0] // 2
-        ws = call.workspace()
+        return PreferenceLossFn._forward(ctx, call, (), (beta, label_smoothing))
+
+    @staticmethod
+    def launch(call, extra, args, g, grads, mixed):
+        dev, pairs, ws = call.tensors[0].device, call.B // 2, call.workspace()
         loss = torch.empty((), dtype=torch.float32, device=dev)
         margin = torch.empty((pairs,), dtype=torch.float32, device=dev)
         mse = torch.empty((2 * pairs,), dtype=torch.float32, device=dev)
-        d_out = ctx.d_out = _gradient_buffer(ctx, call)
-        _lib.check(_lib.lib().ddmi_train_pref_loss(C.byref(call.struct()), pairs, noise.shape[0], beta, label_smoothing, ws.data_ptr(), ws.numel(),
-                                                   loss.data_ptr(), margin.data_ptr(), mse.data_ptr(), _p(d_out), _lib.raw_stream(call.index)))
-        # the gradient needs neither the reference's output nor its logit
-        call.tensors = (call.tensors[0], None) + call.tensors[2:6] + (None, call.tensors[7])
-        ctx.save_for_backward(ws, *call.tensors)
-        call.tensors = None
-        ctx.call, ctx.meta = call, (pairs, int(noise.shape[0]), beta, label_smoothing)
-        ctx.logit_shape = tuple(mixing_logit.shape) if mixing_logit is not None else None
-        ctx.mark_non_differentiable(margin, mse)
-        return loss, margin, mse
+        d_out, d_logit = PreferenceLossFn.buffers(call, grads, mixed)
+        _lib.check(_lib.lib().ddmi_train_pref_loss(C.byref(call.struct()), pairs, call.tensors[3].shape[0], *args, _p(g), ws.data_ptr(), ws.numel(),
+                                                   loss.data_ptr(), margin.data_ptr(), mse.data_ptr(), _p(d_out), _p(d_logit), _lib.raw_stream(call.index)))
+        return (loss, margin, mse), (d_out, d_logit)
 
     @staticmethod
     def backward(ctx, g, _margin, _mse):
-        ws, call = ctx.saved_tensors[0], ctx.call
-        call.tensors = ctx.saved_tensors[1:]
-        d_out, state = _take_buffer(ctx, call)
-        d_logit = torch.empty(ctx.logit_shape, dtype=torch.float32, device=ws.device) if ctx.logit_shape else None
-        pairs, noise_rows, beta, smoothing = ctx.meta
-        g = g.contiguous()
-        with _lib.on_device(call.index):
-            _lib.check(_lib.lib().ddmi_train_pref_loss_bwd(C.byref(call.struct()), pairs, noise_rows, beta, smoothing, ws.data_ptr(), ws.numel(),
-                                                           g.data_ptr(), state, d_out.data_ptr(), _p(d_logit), _lib.raw_stream(call.index)))
-        call.tensors = None
-        return (d_out, d_logit) + (None,) * 8
+        return PreferenceLossFn._backward(ctx, g) + (None,) * 8
 
 
-class PolicyLossFn(torch.autograd.Function):
+class PolicyLossFn(_LossFn):
     @staticmethod
     def forward(ctx, model_out, mixing_logit, ref_out, x_t, x_prev, sqrt_1mac, ref_logit, weight, transition, logp_old, advantage, clip_range,
                 kl_coef):
         call = _Call(model_out, ref_out, x_t, x_prev, sqrt_1mac, mixing_logit, ref_logit, weight)
-        dev, B = model_out.device, model_out.shape[0]
-        ws, transition = call.workspace(), transition.contiguous()
+        return PolicyLossFn._forward(ctx, call, (transition.contiguous(), logp_old.contiguous(), advantage.contiguous()), (clip_range, kl_coef))
+
+    @staticmethod
+    def launch(call, extra, args, g, grads, mixed):
+        dev, ws = call.tensors[0].device, call.workspace()
         loss = torch.empty((), dtype=torch.float32, device=dev)
-        logp, ratio, kl = torch.empty((3, B), dtype=torch.float32, device=dev).unbind(0)
-        logp_old, advantage = logp_old.contiguous(), advantage.contiguous()
-        d_out = ctx.d_out = _gradient_buffer(ctx, call)
-        _lib.check(_lib.lib().ddmi_train_policy_loss(C.byref(call.struct()), B, transition.data_ptr(), logp_old.data_ptr(), advantage.data_ptr(),
-                                                     clip_range, kl_coef, ws.data_ptr(), ws.numel(), loss.data_ptr(), logp.data_ptr(), ratio.data_ptr(),
-                                                     kl.data_ptr(), _p(d_out), _lib.raw_stream(call.index)))
-        ctx.save_for_backward(ws, transition, *call.tensors)
-        call.tensors = None
-        ctx.call = call
-        ctx.logit_shape = tuple(mixing_logit.shape) if mixing_logit is not None else None
-        ctx.mark_non_differentiable(logp, ratio, kl)
-        return loss, logp, ratio, kl
+        logp, ratio, kl = torch.empty((3, call.B), dtype=torch.float32, device=dev).unbind(0)
+        d_out, d_logit = PolicyLossFn.buffers(call, grads, mixed)
+        _lib.check(_lib.lib().ddmi_train_policy_loss(C.byref(call.struct()), call.B, *map(_p, extra), *args, _p(g), ws.data_ptr(), ws.numel(),
+                                                     loss.data_ptr(), logp.data_ptr(), ratio.data_ptr(), kl.data_ptr(), _p(d_out), _p(d_logit),
+                                                     _lib.raw_stream(call.index)))
+        return (loss, logp, ratio, kl), (d_out, d_logit)
 
     @staticmethod
     def backward(ctx, g, *_stats):
-        ws, transition, call = ctx.saved_tensors[0], ctx.saved_tensors[1], ctx.call
-        call.tensors = ctx.saved_tensors[2:]
-        d_out, state = _take_buffer(ctx, call)
-        d_logit = torch.empty(ctx.logit_shape, dtype=torch.float32, device=ws.device) if ctx.logit_shape else None
-        g = g.contiguous()
-        with _lib.on_device(call.index):
-            _lib.check(_lib.lib().ddmi_train_policy_loss_bwd(C.byref(call.struct()), call.B, transition.data_ptr(), ws.data_ptr(), ws.numel(),
-                                                             g.data_ptr(), state, d_out.data_ptr(), _p(d_logit), _lib.raw_stream(call.index)))
-        call.tensors = None
-        return (d_out, d_logit) + (None,) * 11
+        return PolicyLossFn._backward(ctx, g) + (None,) * 11
 
 
 def preference_loss(model_out, ref_out, x_t, noise, sqrt_1mac, beta, mixing_logit=None, ref_mixing_logit=None, weight=None,
@@ -285,6 +284,6 @@ def transition_log_prob(model_out, x_t, x_prev, transition, sqrt_1mac, mixing_lo
         call = _Call(model_out, None, x_t, x_prev, sqrt_1mac, mixing_logit, None, weight)
         ws, transition = call.workspace(), transition.detach().contiguous()
         logp = torch.empty((call.B,), dtype=torch.float32, device=model_out.device)
-        _lib.check(_lib.lib().ddmi_train_policy_loss(C.byref(call.struct()), call.B, transition.data_ptr(), None, None, 0.0, 0.0, ws.data_ptr(), ws.numel(),
-                                                     None, logp.data_ptr(), None, None, None, _lib.raw_stream(call.index)))
+        _lib.check(_lib.lib().ddmi_train_policy_loss(C.byref(call.struct()), call.B, transition.data_ptr(), None, None, 0.0, 0.0, None, ws.data_ptr(),
+                                                     ws.numel(), None, logp.data_ptr(), None, None, None, None, _lib.raw_stream(call.index)))
         return logp

@@ -9,6 +9,7 @@ step gives the same bits on every run.
 """
 from __future__ import annotations
 
+import operator
 from typing import Dict, List, Optional, Sequence, Union
 
 import numpy as np
@@ -23,6 +24,7 @@ _ENTRY = np.dtype([("param", "u8"), ("grad", "u8"), ("exp_avg", "u8"), ("exp_avg
 
 
 _NUMEL, _CONTIGUOUS, _POINTER, _DEVICE = torch.Tensor.numel, torch.Tensor.is_contiguous, torch.Tensor.data_ptr, torch.Tensor.get_device
+_DTYPE, _SHAPE = operator.attrgetter("dtype"), operator.attrgetter("shape")
 
 
 def blocks_of(n: int) -> int:
@@ -55,7 +57,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
         raise ValueError(f"{who}: params, grads, exp_avgs and exp_avg_sqs have {[len(v) for v in lists]} tensors")
     if n == 0:
         return
-    kinds = {t.dtype for t in exp_avgs} | {t.dtype for t in exp_avg_sqs}
+    kinds = set(map(_DTYPE, exp_avgs)) | set(map(_DTYPE, exp_avg_sqs))
     if kinds == {torch.float32}:
         bits = 32
         if exp_avg_scales is not None or exp_avg_sq_scales is not None:
@@ -70,7 +72,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
         lists = lists + scales
     else:
         raise ValueError(f"{who}: moments are all fp32 or all float8_e4m3fn, got {sorted(map(str, kinds))}")
-    p_types, g_types = [t.dtype for t in params], [t.dtype for t in grads]
+    p_types, g_types = list(map(_DTYPE, params)), list(map(_DTYPE, grads))
     kinds = set(zip(p_types, g_types))
     bad = {k for kind in kinds for k in kind} - set(_TYPES)
     if bad:
@@ -80,13 +82,13 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     for name, ts in (("gradient", grads), ("exp_avg", exp_avgs), ("exp_avg_sq", exp_avg_sqs)):
         if list(map(_NUMEL, ts)) != sizes:
             raise ValueError(f"{who}: a tensor's {name} has another number of values than the parameter")
-    if [t.shape for t in grads] != [t.shape for t in params]:
+    if list(map(_SHAPE, grads)) != list(map(_SHAPE, params)):
         raise ValueError(f"{who}: a gradient has another shape than its parameter")
     e["numel"] = numel = np.array(sizes, dtype=np.int64)
     blocks = -(-numel // BLOCK)
     if bits == 8:
         for ts in scales:
-            if list(map(_NUMEL, ts)) != blocks.tolist() or {t.dtype for t in ts} != {torch.float32}:
+            if list(map(_NUMEL, ts)) != blocks.tolist() or set(map(_DTYPE, ts)) != {torch.float32}:
                 raise ValueError(f"{who}: scales are fp32, one for each {BLOCK} values of a tensor")
     for ts in lists:
         if not all(map(_CONTIGUOUS, ts)):
@@ -101,7 +103,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     if dev < 0 or not params[0].is_cuda or any(set(map(_DEVICE, ts)) != {dev} for ts in lists):
         raise ValueError(f"{who}: all tensors live on one GPU, got {sorted({str(t.device) for ts in lists for t in ts})}")
     for name, ts in zip(("param", "grad", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale"), lists):
-        e[name] = list(map(_POINTER, ts))
+        e[name] = np.fromiter(map(_POINTER, ts), np.uint64, n)
     p_bytes = numel * (4 if p_types.count(torch.float32) == n else np.array([t.itemsize for t in p_types], dtype=np.int64))
     state = [("exp_avg", 4 * numel if bits == 32 else numel), ("exp_avg_sq", 4 * numel if bits == 32 else numel)]
     state += [("exp_avg_scale", 4 * blocks), ("exp_avg_sq_scale", 4 * blocks)] if bits == 8 else []

@@ -503,8 +503,7 @@ int ddmi_train_ema(float* ema, const float* param, int64_t n, float decay, void*
 /* ---------------------------------------------------------------------------------------------------------
  * Fine-tuning: the losses that move a trained LDM towards preferences or rewards, and the optimizer step over separately allocated
  * tensors.  They stand beside ddmi_train_eps_loss / ddmi_train_adamw; no handle: every buffer is the caller's, the losses' workspace
- * included (ddmi_train_loss_workspace_bytes; 16-byte aligned, contents undefined before the forward call; the backward call of a loss
- * takes the workspace its forward call filled, any number of times).  All of them only enqueue work: capturable.
+ * included (ddmi_train_loss_workspace_bytes; 16-byte aligned, undefined contents).  All of them only enqueue work: capturable.
  *
  * Per value of sample b, channel ch:  m = sqrt_1mac[b] x_t, c = sigmoid(mixing_logit[ch]), eps = m + c (model_out - m) - the mixed
  * prediction of diffusion/ddpm.py:469-477; eps = model_out without logits.  Samples are [C, HW], contiguous.  Sums are held in fp64.
@@ -523,36 +522,27 @@ typedef struct {
   int64_t HW;
   int C, out_dtype;
 } ddmi_loss_in;
-/* A loss's forward call may be given the gradient's buffer: where the batch is large it then reads every input once and leaves d loss /
- * d model_out (for an upstream gradient of 1) there, unless it could not wait for a neighbour's sums; where it is small it leaves the buffer
- * alone.  The backward call, which completes it in any case, is told: */
-enum {
-  DDMI_GRAD_NONE = 0,     /* the forward call had no d_model_out */
-  DDMI_GRAD_OTHER = 1,    /* it had one, this is another buffer */
-  DDMI_GRAD_THIS = 2      /* it had this one, which nobody has written since */
-};
+/* A loss call gives the gradients along with the loss (d_model_out [B, C, HW] of out_dtype, d_logit [C]; both nullable, d_logit needs
+ * d_model_out), times *dloss, a device scalar (nullable = 1); a large batch's inputs are then read once. */
 int ddmi_train_loss_workspace_bytes(int B, int C, int64_t HW, int mixed, size_t* bytes);
 /* Preference loss over `pairs` pairs: samples [0, pairs) preferred, [pairs, 2 pairs) rejected (B = 2 pairs).  e = mean((eps - noise)^2),
  * margin = -beta / 2 ((e - e_ref) of the preferred - that of the rejected), loss = weighted mean of
  * -(1 - label_smoothing) log sigma(margin) - label_smoothing log sigma(-margin).  noise_rows: 2 pairs, or pairs when both samples of a
  * pair got the same noise.  margin [pairs], mse [2 pairs] = e; 0 for pairs left out. */
-int ddmi_train_pref_loss(const ddmi_loss_in* in, int pairs, int noise_rows, double beta, double label_smoothing, void* ws, size_t ws_bytes, float* loss,
-                         float* margin, float* mse, void* d_model_out /* nullable */, void* stream);
-/* d_model_out [B, C, HW] of out_dtype, d_logit [C] (nullable), both times *dloss (a device scalar, nullable = 1) */
-int ddmi_train_pref_loss_bwd(const ddmi_loss_in* in, int pairs, int noise_rows, double beta, double label_smoothing, void* ws, size_t ws_bytes,
-                             const float* dloss, int state, void* d_model_out, float* d_logit, void* stream);
+int ddmi_train_pref_loss(const ddmi_loss_in* in, int pairs, int noise_rows, double beta, double label_smoothing, const float* dloss, void* ws,
+                         size_t ws_bytes, float* loss, float* margin, float* mse, void* d_model_out, float* d_logit, void* stream);
 /* Clipped policy loss over B denoising transitions x_t -> second: mean mu = A x_t + E eps and deviation s with transition[b] = (A, E, s);
  * logp = mean over the values of log N(second; mu, s^2), ratio = exp(logp - logp_old), kl = mean((mu - mu_ref)^2) / (2 s^2), loss =
  * weighted mean of max(-advantage ratio, -advantage clip(ratio, 1 -+ clip_range)) + kl_coef kl.  A transition with s = 0 has no density
  * and is left out like one of weight 0.  logp_old = NULL: logp alone is computed (a rollout records it), the other outputs are not
  * touched.  logp, ratio, kl [B]; 0 for transitions left out. */
 int ddmi_train_policy_loss(const ddmi_loss_in* in, int B, const float* transition, const float* logp_old, const float* advantage, double clip_range,
-                           double kl_coef, void* ws, size_t ws_bytes, float* loss, float* logp, float* ratio, float* kl,
-                           void* d_model_out /* nullable */, void* stream);
-int ddmi_train_policy_loss_bwd(const ddmi_loss_in* in, int B, const float* transition, void* ws, size_t ws_bytes, const float* dloss, int state,
-                               void* d_model_out, float* d_logit, void* stream);
-/* how often a workgroup of a loss's one-pass form looks for its neighbours' sums before it leaves its part to the backward call (4096 by
- * default; 0: one look - the results are the same bits) */
+                           double kl_coef, const float* dloss, void* ws, size_t ws_bytes, float* loss, float* logp, float* ratio, float* kl,
+                           void* d_model_out, float* d_logit, void* stream);
+/* gradients of a loss call without dloss, times *dloss in place (n values of out_dtype, C logits; nothing is touched when it is 1) */
+int ddmi_train_loss_scale(const float* dloss, void* d_model_out, int out_dtype, int64_t n, float* d_logit, int C, void* stream);
+/* how often a workgroup of a loss's one-pass form looks for its neighbours' sums before it leaves its part to the kernel after it (4096
+ * by default; 0: one look - the results are the same bits) */
 int ddmi_debug_loss_polls(int n);
 /* One tensor of an AdamW step.  Moments in 32 bits: exp_avg, exp_avg_sq fp32 [numel].  In 8 bits: e4m3 codes [numel] of the first moment
  * and of the ROOT of the second, one fp32 power-of-two scale for each 256 values (exp_avg_scale, exp_avg_sq_scale [ceil(numel / 256)]). */

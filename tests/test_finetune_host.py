@@ -133,21 +133,27 @@ def test_c_entries_refuse():
         assert L.ddmi_train_loss_workspace_bytes(*args, C.byref(ws)) == 1
     assert L.ddmi_train_loss_workspace_bytes(4, 3, 5, 1, C.byref(ws)) == 0 and ws.value > 0
     s = _lib.LossIn(64, 64, 64, 64, 64, 64, 64, None, 5, 3, 0)
-    call = lambda st, pairs=2, rows=2, a=0.0, at=64, size=None: L.ddmi_train_pref_loss(      # noqa: E731
-        C.byref(st), pairs, rows, 1.0, a, C.c_void_p(at), ws.value if size is None else size, one, one, one, None, None)
-    assert call(s, size=ws.value - 1) == 1 and call(s, at=65) == 1 and call(s, rows=3) == 1 and call(s, a=2.0) == 1 and call(s, pairs=0) == 1
+
+    def pref(pairs=2, rows=2, a=0.0, at=64, size=None, d_out=one, d_logit=one):
+        return L.ddmi_train_pref_loss(C.byref(s), pairs, rows, 1.0, a, None, C.c_void_p(at), ws.value if size is None else size, one, one, one, d_out,
+                                      d_logit, None)
+
+    assert pref(size=ws.value - 1) == 1 and pref(at=65) == 1 and pref(rows=3) == 1 and pref(a=2.0) == 1 and pref(pairs=0) == 1 and pref(d_out=None) == 1
     s.out_dtype = 7
-    assert call(s) == 1
+    assert pref() == 1
     s.out_dtype, s.ref_mixing_logit = 0, None
-    assert call(s) == 1
+    assert pref() == 1
     s.ref_mixing_logit, s.ref_out = 64, None
-    assert call(s) == 1
-    assert L.ddmi_train_policy_loss(C.byref(s), 4, one, one, one, 0.1, 0.5, one, ws.value, one, one, one, one, None, None) == 1      # KL without a reference
-    assert L.ddmi_train_policy_loss(C.byref(s), 4, one, one, None, 0.1, 0.0, one, ws.value, one, one, one, one, None, None) == 1     # no advantages
-    assert L.ddmi_train_policy_loss(C.byref(s), 4, one, None, None, 0.1, 0.0, one, ws.value, None, one, None, None, one, None) == 1       # gradient of logp
-    s.ref_out = 64
-    back = lambda state, out=one: L.ddmi_train_pref_loss_bwd(C.byref(s), 2, 2, 1.0, 0.0, one, ws.value, None, state, out, None, None)      # noqa: E731
-    assert back(3) == 1 and back(-1) == 1 and back(0, None) == 1
+    assert pref() == 1
+
+    def policy(old=one, adv=one, kl=0.0, clip=0.1, loss=one, d_out=None, d_logit=None):
+        return L.ddmi_train_policy_loss(C.byref(s), 4, one, old, adv, clip, kl, None, one, ws.value, loss, one, one, one, d_out, d_logit, None)
+
+    assert policy(kl=0.5) == 1 and policy(adv=None) == 1 and policy(clip=-1.0) == 1 and policy(loss=None) == 1       # KL without a reference first
+    assert policy(old=None, adv=None, d_out=one) == 1 and policy(d_logit=one) == 1
+    s.mixing_logit = s.ref_mixing_logit = None
+    assert policy(d_out=one, d_logit=one) == 1
+    assert L.ddmi_train_loss_scale(None, one, 0, 4, None, 0, None) == 1 and L.ddmi_train_loss_scale(one, one, 0, 0, None, 0, None) == 1
     assert L.ddmi_debug_loss_polls(-1) == 1
     e = np.zeros(1, dtype=[("p", "u8", 6), ("n", "i8", 2), ("f", "f8", 2), ("i", "i8")])
     assert e.itemsize == 88
