@@ -132,7 +132,9 @@ def train_main(args, dc, rank, world, dev):
     """`data.mode: train` (image, occupancy and video domains): the LDM trainer's loop (tools/ldm/image.py:136-178, tools/ldm/occupancy.py:139-180, tools/ldm/video.py:125-167) on LATENTS - the VAE encoder that
     produces them from images is outside this path.  Latents come from `data.latents` (an .npy of [N,C,H,W] fp32, e.g.
     `vaemodel.encode(y).sample()` dumped by the reference) or, without one, are synthetic N(0,1).  One process per GPU; every
-    rank draws its own batches and the gradient slab is all-reduced over RCCL each optimizer step.  Writes `ldm-last.pt` in the
+    rank draws its own batches and the gradient slab is all-reduced over RCCL each optimizer step.  `lossconfig.objective: preference`
+    fine-tunes the loaded model on pairs of latents ([N,2,C,H,W]: preferred, rejected; `beta`, `label_smoothing`) against its own starting
+    weights; `lossconfig.optimizer_state_bits: 8` keeps AdamW's moments in 8 bits.  Writes `ldm-last.pt` in the
     layout LDMTrainer.save uses, so `mode: gen` picks it up."""
     import numpy as np
     import torch
@@ -147,10 +149,14 @@ def train_main(args, dc, rank, world, dev):
     lc = args.loss_config or {}
     B = int(dc.get("batch_size", dc.test_batch_size))
     steps = int(os.environ.get("DDMI_TRAIN_STEPS", dc.get("train_steps", 100)))
+    objective = str(lc.get("objective", "noise"))
+    if objective not in ("noise", "preference"):
+        raise SystemExit(f"lossconfig.objective is noise (p_losses) or preference, got {objective}")
     step = LDMTrainStep(args.unetconfig, dict(args.ddpmconfig, domain="video") if video else args.ddpmconfig, numerics=args.numerics,
                         lr=float(getattr(args, "lr", None) or 1e-4),
                         gradient_accumulate_every=int(lc.get("gradient_accumulate_every", 1)), ema_decay=float(lc.get("ema_decay", 0.9999)),
-                        ema_update_every=int(lc.get("ema_update_every", 10)), device=dev)
+                        ema_update_every=int(lc.get("ema_update_every", 10)), optimizer_state_bits=int(lc.get("optimizer_state_bits", 32)),
+                        device=dev)
     vae_state, mlp_state, ck = {}, {}, None
     path = CK.find_checkpoint(dc.save_pth, resume=bool(getattr(args, "resume", False)), pretrained=bool(args.pretrained))
     if path is not None:   # the reference's start modes: resume / pretrained continue an LDM, otherwise the stage-1 VAE + MLP
@@ -175,9 +181,13 @@ def train_main(args, dc, rank, world, dev):
         # EMA would restart from the online weights and AdamW's bias correction from step 0
         step.load_training_state(ck, resume=bool(getattr(args, "resume", False)))
         print(f"restored EMA (step {step.ema_step})" + (f", AdamW state, optimizer step {step.opt_step}" if getattr(args, "resume", False) else ""))
+    if objective == "preference":
+        step.set_reference()     # the weights that fine-tuning starts from
     lat = None
     if dc.get("latents") and os.path.exists(dc.latents):
         lat = torch.from_numpy(np.load(dc.latents).astype(np.float32))
+        if objective == "preference" and (lat.dim() != (4 if video else 5) or lat.shape[1] != 2):
+            raise SystemExit(f"lossconfig.objective preference takes latents [N, 2, C, ...] (preferred, rejected), got {tuple(lat.shape)}")
     g = torch.Generator(device=dev).manual_seed(args.seed * 1000 + rank)
     C_, S_ = int(args.ddpmconfig.get("channels", 64)), int(args.ddpmconfig.get("image_size", 64))
     for it in range(steps):
@@ -185,8 +195,12 @@ def train_main(args, dc, rank, world, dev):
             idx = torch.randint(0, lat.shape[0], (B,), generator=torch.Generator().manual_seed(args.seed * 7919 + it * world + rank))
             z = lat[idx].to(dev)
         else:
-            z = torch.randn((B, C_, step.model.seq_len) if video else (B, C_, S_, S_), device=dev, generator=g)
-        loss = step.train_step(z, world_size=world)
+            z = torch.randn((B,) + ((2,) if objective == "preference" else ()) + ((C_, step.model.seq_len) if video else (C_, S_, S_)), device=dev, generator=g)
+        if objective == "preference":      # latents [N, 2, C, ...]: preferred, rejected
+            loss = step.preference_step(z[:, 0], z[:, 1], beta=float(lc.get("beta", 2000.0)), label_smoothing=float(lc.get("label_smoothing", 0.0)),
+                                        world_size=world).loss
+        else:
+            loss = step.train_step(z, world_size=world)
         if rank == 0 and (it % 10 == 0 or it == steps - 1):
             print(f"iter {it}: Dae loss : {float(loss):.4f}", flush=True)
     if rank == 0:
