@@ -6,6 +6,7 @@ enum { FT_PREF = 0, FT_POLICY = 1 };
 #define FT_THREADS 256
 #define FT_VECS 16       // vectors of four residuals that a thread of the one-pass kernel keeps in registers
 #define FT_CACHE_BYTES 268435456.0   // the last-level cache: an optimizer step that touches more goes past it
+#define FT_MOST_GROUPS ((1ll << 24) - 1)   // workgroups of 256 threads in one launch: below 2^32 threads
 #define FT_ROWS 512      // most rows (sample, channel) of one workgroup: their mixing coefficients sit in LDS
 
 struct FtArgs {
@@ -34,8 +35,7 @@ struct FtArgs {
   int64_t T, seg;
   int wps, rows_per_wg, nseg, log_g, fused, polls;
   // workspace
-  unsigned* counter;
-  double* total;             // one pass: sum of the weights
+  double* total;             // sum of the weights
   int* done;                 // one pass: whether a span's gradient is written
   float2* coef;              // a sample: factors of the residual and of the step away from the reference
   double* term;

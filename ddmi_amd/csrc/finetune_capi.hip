@@ -44,7 +44,7 @@ int ddmi_train_loss_workspace_bytes(int B, int C, int64_t HW, int mixed, size_t*
 int ddmi_train_pref_loss(const ddmi_loss_in* in, int pairs, int noise_rows, double beta, double label_smoothing, const float* dloss, void* ws,
                          size_t ws_bytes, float* loss, float* margin, float* mse, void* d_model_out, float* d_logit, void* stream) {
   FtArgs a{};
-  DDMI_REQUIRE(in && in->ref_out && pairs > 0 && pairs <= (1 << 29), "pref_loss: null argument or no pairs");
+  DDMI_REQUIRE(in && in->ref_out && pairs > 0 && pairs <= (1 << 24), "pref_loss: null argument or no pairs");
   DDMI_REQUIRE(loss && margin && mse, "pref_loss: null output");
   DDMI_REQUIRE(noise_rows == pairs || noise_rows == 2 * pairs, "pref_loss: the noise has a row for each pair or for each sample");
   DDMI_REQUIRE(label_smoothing >= 0.0 && label_smoothing <= 1.0 && beta == beta, "pref_loss: label_smoothing in [0, 1], beta a number");

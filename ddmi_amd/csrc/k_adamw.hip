@@ -323,8 +323,8 @@ int launch_adamw_multi(const ddmi_adamw_tensor* t, int n, double beta1, double b
       const ddmi_adamw_tensor& d = t[i];
       const int64_t wgs = cdiv64(d.numel, AD_CHUNK);
       if (wgs == 0) { ++i; continue; }
-      if (wgs > (1ll << 30)) return ddmi_fail(DDMI_ERR_INVALID, "adamw_multi: a tensor of more than 2^42 values");
-      if ((int64_t)a.first[a.count] + wgs > (1ll << 30)) break;
+      if (wgs > FT_MOST_GROUPS) return ddmi_fail(DDMI_ERR_INVALID, "adamw_multi: a tensor of more than 2^36 values");
+      if ((int64_t)a.first[a.count] + wgs > FT_MOST_GROUPS) break;
       AdTensor& o = a.t[a.count];
       o.p = d.param; o.g = d.grad; o.m = d.exp_avg; o.v = d.exp_avg_sq; o.ms = d.exp_avg_scale; o.vs = d.exp_avg_sq_scale; o.n = d.numel;
       o.decay = (float)(1.0 - d.lr * d.weight_decay);

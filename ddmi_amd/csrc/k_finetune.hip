@@ -7,8 +7,8 @@
 //   policy:      z = (x_prev - A x_t) - E eps,     sums  z^2,  (eps - eps_ref)^2,  z (o - m),  (eps - eps_ref) (o - m)
 // One scalar (two with KL) a sample follows from the sums over ALL of its values, and only then is the gradient known:
 //   d loss / d o = c (k z' + q far).  So: sums_kernel (reads every input once), rows_kernel (a workgroup a pair / transition: the scalar
-//   work in 64 bits, the last one to finish adds up the loss), grad_kernel (reads again what the gradient needs, writes it).  A large
-//   batch is read once: fused_kernel below.
+//   work in 64 bits), grad_kernel (adds up loss and logits' gradients, reads again what the gradient needs and writes it).  A large batch is
+//   read once: fused_kernel below.
 // Factors are rounded in fp32, products and sums are held in fp64: a margin is the difference of two nearly equal errors times
 // beta ~ 10^3, and a logit's gradient a sum of either sign over the batch.  No float atomics: every sum has a fixed order.
 #include <algorithm>
@@ -111,12 +111,35 @@ __device__ __forceinline__ void add_up(float res, float far, float part, double&
   if (MIX) { S2 = fma(r, (double)part, S2); if (MODE == FT_POLICY && REF) S3 = fma(f, (double)part, S3); }
 }
 
+__device__ __forceinline__ double block_sum(double v, double* red) {
+  for (int st = 32; st > 0; st >>= 1) v += __shfl_xor(v, st);
+  __syncthreads();
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+  __syncthreads();
+  double t = 0.0;
+  for (int w = 0; w < FT_THREADS / 64; ++w) t += red[w];
+  return t;
+}
+// sum of the weights of the rows that take part, by one workgroup
+template <int MODE>
+__device__ __forceinline__ void total_weight(const FtArgs& a, double* red) {
+  const int rows = MODE == FT_PREF ? a.pairs : a.B;
+  double total = rows;
+  if (a.weight || MODE == FT_POLICY) {
+    total = 0.0;
+    for (int j = threadIdx.x; j < rows; j += FT_THREADS)
+      if (takes_part<MODE>(a, j)) total += a.weight ? (double)a.weight[j] : 1.0;
+    total = block_sum(total, red);
+  }
+  if (threadIdx.x == 0) *a.total = total;
+}
+
 template <int MODE, bool MIX, bool REF, typename T>
 __global__ void __launch_bounds__(FT_THREADS) sums_kernel(FtArgs a) {
   __shared__ float2 mix[FT_ROWS];
   __shared__ double red[2][FT_THREADS / 64];
   const int tid = threadIdx.x;
-  if (blockIdx.x == 0 && tid == 0) *a.counter = 0u;   // rows_kernel counts its workgroups; stream order makes this visible to it
+  if (blockIdx.x == 0) total_weight<MODE>(a, red[0]);
   const Span s = span_of<MODE>(a, blockIdx.x);
   const int G = 1 << a.log_g, lane = tid & (G - 1), group = tid >> a.log_g, ngroups = FT_THREADS >> a.log_g;
   const int wpg = G > 64 ? G / 64 : 1;                // waves that share a row
@@ -177,15 +200,6 @@ __global__ void __launch_bounds__(FT_THREADS) sums_kernel(FtArgs a) {
   }
 }
 
-__device__ __forceinline__ double block_sum(double v, double* red) {
-  for (int st = 32; st > 0; st >>= 1) v += __shfl_xor(v, st);
-  __syncthreads();
-  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
-  __syncthreads();
-  double t = 0.0;
-  for (int w = 0; w < FT_THREADS / 64; ++w) t += red[w];
-  return t;
-}
 // the scalar work of one pair / transition, from its sums
 struct RowOut {
   double term, stat[3];       // weighted loss; margin, mse, mse | logp, ratio, kl
@@ -222,13 +236,6 @@ __device__ __forceinline__ RowOut policy_row(const FtArgs& a, bool used, double 
   o.coef[0] = make_float2((float)((free ? open * w / (var * n) : (clipped ? 0.0 : open + bound)) * E), (float)(w * a.kl_coef * E * E / (var * n)));
   return o;
 }
-template <int MODE>
-__device__ __forceinline__ double total_weight(const FtArgs& a, int rows, double* red) {
-  double total = 0.0;
-  for (int j = threadIdx.x; j < rows; j += FT_THREADS)
-    if (takes_part<MODE>(a, j)) total += a.weight ? (double)a.weight[j] : 1.0;
-  return block_sum(total, red);
-}
 __device__ __forceinline__ double2 sample_sums(const FtArgs& a, int sample, double* red) {
   double u = 0.0, v = 0.0;
   for (int j = threadIdx.x; j < a.wps; j += FT_THREADS) {
@@ -239,13 +246,12 @@ __device__ __forceinline__ double2 sample_sums(const FtArgs& a, int sample, doub
   v = block_sum(v, red);
   return make_double2(u, v);
 }
-// one workgroup a pair / transition; the last one to finish adds up the loss over them, in their order
+// one workgroup a pair / transition
 template <int MODE>
 __global__ void __launch_bounds__(FT_THREADS) rows_kernel(FtArgs a) {
   __shared__ double red[FT_THREADS / 64];
-  __shared__ int last;
-  const int i = blockIdx.x, rows = gridDim.x, tid = threadIdx.x;
-  const double total = a.fused ? *a.total : total_weight<MODE>(a, rows, red);
+  const int i = blockIdx.x, tid = threadIdx.x;
+  const double total = *a.total;
   const bool used = takes_part<MODE>(a, i);
   const double w = used ? (a.weight ? (double)a.weight[i] : 1.0) / total : 0.0;
   RowOut o;
@@ -268,18 +274,18 @@ __global__ void __launch_bounds__(FT_THREADS) rows_kernel(FtArgs a) {
       a.coef[i] = o.coef[0];
     }
   }
-  if (!a.loss) return;
-  if (tid == 0) {
-    __hip_atomic_store(&a.term[i], o.term, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-    const unsigned done = __hip_atomic_fetch_add(a.counter, 1u, __ATOMIC_ACQ_REL, __HIP_MEMORY_SCOPE_AGENT);
-    last = done == (unsigned)rows - 1u;
-  }
-  __syncthreads();
-  if (!last) return;
+  if (a.loss && tid == 0) a.term[i] = o.term;
+}
+// the loss: the rows' terms, in their order
+__device__ __forceinline__ void sum_terms(const FtArgs& a, int rows, double* red) {
   double sum = 0.0;
-  for (int j = tid; j < rows; j += FT_THREADS) sum += __hip_atomic_load(&a.term[j], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  for (int j = threadIdx.x; j < rows; j += FT_THREADS) sum += a.term[j];
   sum = block_sum(sum, red);
-  if (tid == 0) *a.loss = (float)sum;
+  if (threadIdx.x == 0) *a.loss = (float)sum;
+}
+__global__ void __launch_bounds__(FT_THREADS) loss_kernel(FtArgs a, int rows) {
+  __shared__ double red[FT_THREADS / 64];
+  sum_terms(a, rows, red);
 }
 
 // ---- one pass: the residuals wait in registers for their sample's sums ----------------------------------------------------------
@@ -287,19 +293,16 @@ __global__ void __launch_bounds__(FT_THREADS) rows_kernel(FtArgs a) {
 // gradient from the residuals in its registers: every input is read once.  The sums' own bits are the signal - open_kernel fills their
 // places with a NaN that no sum is stored as - so publishing is two relaxed agent-scope stores, with no fence and no counter.  The wait is
 // bounded: a workgroup whose neighbours do not show up (other kernels hold the compute units) leaves its span undone, and grad_kernel,
-// which runs after it in any case (the logits' gradients need every sample's factors), computes what is not done.
+// which runs after it in any case (loss and logits' gradients need every sample), computes what is not done.
 constexpr unsigned long long FT_OPEN = 0xFFFFFFFFFFFFFFFFull;
 int g_polls = 1 << 12;                  // some milliseconds; the spans of a row start within microseconds of each other
 
 template <int MODE>
-__global__ void __launch_bounds__(FT_THREADS) open_kernel(FtArgs a, int64_t places, int rows) {
+__global__ void __launch_bounds__(FT_THREADS) open_kernel(FtArgs a, int64_t places) {
   __shared__ double red[FT_THREADS / 64];
   unsigned long long* p = reinterpret_cast<unsigned long long*>(a.part);
   for (int64_t i = (int64_t)blockIdx.x * FT_THREADS + threadIdx.x; i < places; i += (int64_t)gridDim.x * FT_THREADS) p[i] = FT_OPEN;
-  if (blockIdx.x == 0) {
-    const double total = total_weight<MODE>(a, rows, red);
-    if (threadIdx.x == 0) { *a.counter = 0u; *a.total = total; }
-  }
+  if (blockIdx.x == 0) total_weight<MODE>(a, red);
 }
 __device__ __forceinline__ void publish(double* place, double v) {
   const unsigned long long bits = v != v ? 0x7FF8000000000000ull : (unsigned long long)__double_as_longlong(v);
@@ -509,15 +512,21 @@ __device__ __forceinline__ void grad_span(const FtArgs& a, int blk, float up, fl
   }
 }
 
-// Workgroups [0, channels): one channel's logit each; the others take spans in turn, but for those that are in d_out already.
+// Workgroup 0: the loss; the next `channels`: one channel's logit each; the others take spans in turn, but for those that are in d_out
+// already.
 template <int MODE, bool MIX, bool REF, typename T>
 __global__ void __launch_bounds__(FT_THREADS) grad_kernel(FtArgs a, int spans, int channels) {
   __shared__ float2 mix[FT_ROWS];
   __shared__ double red[FT_THREADS / 64];
   const int tid = threadIdx.x;
   const float up = a.dloss ? *a.dloss : 1.f;
-  if ((int)blockIdx.x < channels) {
-    const int ch = (int)blockIdx.x, per = a.nseg * (a.log_g > 6 ? 1 << (a.log_g - 6) : 1);
+  const int wg = (int)blockIdx.x - 1 - channels, ch = (int)blockIdx.x - 1;
+  if (blockIdx.x == 0) {
+    sum_terms(a, MODE == FT_PREF ? a.pairs : a.B, red);
+    return;
+  }
+  if (ch < channels) {
+    const int per = a.nseg * (a.log_g > 6 ? 1 << (a.log_g - 6) : 1);
     double s = 0.0;
     for (int64_t j = tid; j < (int64_t)a.B * per; j += FT_THREADS) {
       const int b = (int)(j / per);
@@ -532,7 +541,7 @@ __global__ void __launch_bounds__(FT_THREADS) grad_kernel(FtArgs a, int spans, i
     }
     return;
   }
-  for (int blk = (int)blockIdx.x - channels; blk < spans; blk += (int)gridDim.x - channels) {
+  for (int blk = wg; blk < spans; blk += (int)gridDim.x - 1 - channels) {
     if (a.fused && a.done[blk]) continue;
     grad_span<MODE, MIX, REF, T>(a, blk, up, mix);
     __syncthreads();                                    // the next span's coefficients take this one's place
@@ -548,23 +557,23 @@ int launch_sums_t(const FtArgs& a, int dt, hipStream_t s) {
     const int64_t places = 2ll * a.B * a.wps;
     FtArgs f = a;
     f.polls = g_polls;
-    hipLaunchKernelGGL((open_kernel<MODE>), dim3((unsigned)std::min<int64_t>(cdiv64(places, FT_THREADS), 256)), dim3(FT_THREADS), 0, s, a, places, rows);
+    hipLaunchKernelGGL((open_kernel<MODE>), dim3((unsigned)std::min<int64_t>(cdiv64(places, FT_THREADS), 256)), dim3(FT_THREADS), 0, s, a, places);
     if (dt == DT_F32) hipLaunchKernelGGL((fused_kernel<MODE, MIX, REF, float, NV>), grid, dim3(FT_THREADS), 0, s, f);
     else hipLaunchKernelGGL((fused_kernel<MODE, MIX, REF, bf16_t, NV>), grid, dim3(FT_THREADS), 0, s, f);
-    hipLaunchKernelGGL((rows_kernel<MODE>), dim3((unsigned)rows), dim3(FT_THREADS), 0, s, a);
-    HIP_TRY(hipGetLastError());
-    return DDMI_OK;
+  } else if (dt == DT_F32) {
+    hipLaunchKernelGGL((sums_kernel<MODE, MIX, REF, float>), grid, dim3(FT_THREADS), 0, s, a);
+  } else {
+    hipLaunchKernelGGL((sums_kernel<MODE, MIX, REF, bf16_t>), grid, dim3(FT_THREADS), 0, s, a);
   }
-  if (dt == DT_F32) hipLaunchKernelGGL((sums_kernel<MODE, MIX, REF, float>), grid, dim3(FT_THREADS), 0, s, a);
-  else hipLaunchKernelGGL((sums_kernel<MODE, MIX, REF, bf16_t>), grid, dim3(FT_THREADS), 0, s, a);
   hipLaunchKernelGGL((rows_kernel<MODE>), dim3((unsigned)rows), dim3(FT_THREADS), 0, s, a);
+  if (a.loss && !a.d_out) hipLaunchKernelGGL(loss_kernel, dim3(1), dim3(FT_THREADS), 0, s, a, rows);   // else it is grad_kernel's
   HIP_TRY(hipGetLastError());
   return DDMI_OK;
 }
 template <int MODE, bool MIX, bool REF>
 int launch_grad_t(const FtArgs& a, int dt, hipStream_t s) {
   const int spans = a.B * a.wps, channels = MIX && a.d_logit ? a.C : 0;
-  const dim3 grid((unsigned)(channels + (a.fused ? std::min(spans, 1024) : spans)));   // 1 024 look through what is most often done
+  const dim3 grid((unsigned)(1 + channels + (a.fused ? std::min(spans, 1024) : spans)));   // 1 024 look through what is most often done
   if (dt == DT_F32) hipLaunchKernelGGL((grad_kernel<MODE, MIX, REF, float>), grid, dim3(FT_THREADS), 0, s, a, spans, channels);
   else hipLaunchKernelGGL((grad_kernel<MODE, MIX, REF, bf16_t>), grid, dim3(FT_THREADS), 0, s, a, spans, channels);
   HIP_TRY(hipGetLastError());
@@ -630,7 +639,7 @@ int ft_plan(FtArgs* a, int B, int C, int64_t HW, bool mixed, int rows_of, int ke
     ft_split(a, want);
   }
   const int64_t wps = cdiv64(a->C, a->rows_per_wg) * a->nseg;
-  if (wps * B > (1ll << 30) || (int64_t)B * a->C > (1ll << 40)) return ddmi_fail(DDMI_ERR_INVALID, "fine-tuning loss: too many values in one call");
+  if (wps * B + C > FT_MOST_GROUPS) return ddmi_fail(DDMI_ERR_INVALID, "fine-tuning loss: too many values in one call");
   a->wps = (int)wps;
   return DDMI_OK;
 }
@@ -643,8 +652,7 @@ size_t ft_workspace_bytes(const FtArgs& a) {
 }
 void ft_carve(FtArgs* a, void* ws) {
   unsigned char* p = (unsigned char*)ws;
-  a->counter = (unsigned*)p;
-  a->total = (double*)(p + 64); p += 256;
+  a->total = (double*)p; p += 256;
   a->coef = (float2*)p; p += up256((size_t)a->B * sizeof(float2));
   a->term = (double*)p; p += up256((size_t)a->B * sizeof(double));
   a->part = (double2*)p; p += up256((size_t)a->B * a->wps * sizeof(double2));

@@ -20,6 +20,7 @@ import functools
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 
@@ -175,6 +176,7 @@ class PreferenceLossFn(_LossFn):
         return (loss, margin, mse), (d_out, d_logit)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, g, _margin, _mse):
         return PreferenceLossFn._backward(ctx, g) + (None,) * 8
 
@@ -198,6 +200,7 @@ class PolicyLossFn(_LossFn):
         return (loss, logp, ratio, kl), (d_out, d_logit)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, g, *_stats):
         return PolicyLossFn._backward(ctx, g) + (None,) * 11
 

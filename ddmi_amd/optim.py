@@ -202,7 +202,7 @@ class AdamW:
         take = (lambda v: v) if len(at) == len(self.params) else (lambda v: [v[i] for i in at])
         steps = [s + 1 for s in take(self.steps)]
         with torch.no_grad():
-            adamw_step([p.detach() for p in take(self.params)], [self.params[i].grad for i in at], take(self.exp_avg), take(self.exp_avg_sq), steps,
+            adamw_step(take(self.params), [self.params[i].grad for i in at], take(self.exp_avg), take(self.exp_avg_sq), steps,
                        lr=take(self.lr), betas=self.betas, eps=self.eps, weight_decay=take(self.weight_decay), grad_scale=grad_scale,
                        exp_avg_scales=None if self.state_bits == 32 else take(self.exp_avg_scale),
                        exp_avg_sq_scales=None if self.state_bits == 32 else take(self.exp_avg_sq_scale), seed=self.seed)

@@ -170,6 +170,34 @@ def test_upstream_gradient_and_second_backward(op, B, C, T):
 
 
 @pytest.mark.parametrize("op", ["pref", "policy"])
+def test_second_order_gradients_are_refused(op):
+    d = R.make(op, 4, 3, 5, seed=4, device=DEV)
+    out = d["model_out"].clone().requires_grad_()
+    loss = (preference_loss if op == "pref" else policy_loss)(**dict(d, model_out=out)).loss
+    scale = torch.ones((), device=DEV, requires_grad=True)
+    g = torch.autograd.grad(loss * scale, out, create_graph=True)[0]
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()
+
+
+@pytest.mark.parametrize("op", ["pref", "policy"])
+def test_many_small_rows(op):
+    """More rows than one turn of any workgroup: 100 000 of three values each, weights among them."""
+    d = R.make(op, 100000, 3, 1, seed=12, device=DEV)
+    rows = 50000 if op == "pref" else 100000
+    d["weight"] = (torch.arange(rows, device=DEV) % 7).float()
+    if op == "policy":        # far from the clip's borders
+        d["clip_range"] = 1e-30
+    got = call(op, d)
+    assert torch.isfinite(got["loss"]) and torch.isfinite(got["d_model_out"]).all()
+    if op == "pref":
+        R.check(got, reference(op, d))
+    else:
+        want = R.policy(dict(d, clip_range=1e9))      # nothing clipped, for the statistics
+        R.check({k: got[k] for k in ("logp", "ratio", "kl")}, {k: want[k] for k in ("logp", "ratio", "kl")})
+
+
+@pytest.mark.parametrize("op", ["pref", "policy"])
 @pytest.mark.parametrize("B,C,T", [(8, 16, 1025), (80, 33, 2501)])
 def test_same_bits_on_every_run_and_stream(op, B, C, T):
     d = R.make(op, B, C, T, seed=6, device=DEV)
