@@ -134,6 +134,8 @@ __device__ __forceinline__ void total_weight(const FtArgs& a, double* red) {
   if (threadIdx.x == 0) *a.total = total;
 }
 
+// Two passes, the first: every input once.  Bound by memory where the batch fills the card (256 pairs of 64 x 64 x 64: 368 us, 5.1 TB/s),
+// by the latency of one round of loads where it does not (one pair of 64 x 64: 5 us).
 template <int MODE, bool MIX, bool REF, typename T>
 __global__ void __launch_bounds__(FT_THREADS) sums_kernel(FtArgs a) {
   __shared__ float2 mix[FT_ROWS];
@@ -331,18 +333,42 @@ __device__ __forceinline__ bool await_sums(const FtArgs& a, int64_t first, int l
   out = make_double2(u, v);
   return true;
 }
-template <typename T> __device__ __forceinline__ void load_some(const T* p, int left, float (&v)[4]) {
-  if (left == 4) { load4<true>(p, v); return; }
+// four values as they are stored, of which `left` exist: no conversion, so that the next load does not wait for this one
+template <typename T> struct Raw;
+template <> struct Raw<float> {
+  float v[4];
+  __device__ __forceinline__ void get(const float* p, int left) {
+    if (left == 4) { load4<true>(p, v); return; }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) v[i] = i < left ? to_f32(p[i]) : 0.f;
-}
+    for (int i = 0; i < 4; ++i) v[i] = i < left ? p[i] : 0.f;
+  }
+  __device__ __forceinline__ float at(int i) const { return v[i]; }
+};
+template <> struct Raw<bf16_t> {
+  unsigned v[2];
+  __device__ __forceinline__ void get(const bf16_t* q, int left) {
+    const unsigned short* p = reinterpret_cast<const unsigned short*>(q);
+    if (left == 4) {
+      typedef unsigned u32x2u __attribute__((ext_vector_type(2), aligned(2)));
+      const u32x2u t = __builtin_nontemporal_load(reinterpret_cast<const u32x2u*>(p));
+      v[0] = t.x; v[1] = t.y;
+      return;
+    }
+    v[0] = p[0] | (left > 1 ? (unsigned)p[1] << 16 : 0u);
+    v[1] = left > 2 ? p[2] : 0u;
+  }
+  __device__ __forceinline__ float at(int i) const { return __uint_as_float(i & 1 ? v[i >> 1] & 0xFFFF0000u : v[i >> 1] << 16); }
+};
 template <typename T> __device__ __forceinline__ void store_some(T* p, int left, const float (&v)[4]) {
   if (left == 4) { store4<true>(p, v); return; }
 #pragma unroll
   for (int i = 0; i < 4; ++i) if (i < left) p[i] = from_f32<T>(v[i]);
 }
 
-// NV vectors of four values a thread; a row's vectors lie on its G lanes in turn, `turns` to a lane
+// NV vectors of four values a thread; a row's vectors lie on its G lanes in turn, `turns` to a lane.  Sixteen vectors of residuals (two
+// times eight with KL) leave room for four workgroups a compute unit, so that three load while one waits.  256 pairs of 64 x 64 x 64: 453 us
+// for the 2.42 GB that any form has to move, 5.3 TB/s; 512 transitions with KL: 492 us, 5.5 TB/s.  What is left is the wait for the last of
+// a sample's spans; loading a vector ahead of its use costs more registers than it gains (2 % slower).
 template <int MODE, bool MIX, bool REF, typename T, int NV>
 __global__ void __launch_bounds__(FT_THREADS, 2) fused_kernel(FtArgs a) {
   constexpr bool TWO = MODE == FT_POLICY && REF;
@@ -383,18 +409,19 @@ __global__ void __launch_bounds__(FT_THREADS, 2) fused_kernel(FtArgs a) {
     if (rt < row_turns) {
       const int r = rt * ngroups + group, t = 4 * (turn * G + lane);
       const int left = r < s.rows ? min(4, len - t) : 0;
-      float o[4] = {0.f, 0.f, 0.f, 0.f}, q[4] = {0.f, 0.f, 0.f, 0.f}, x[4] = {0.f, 0.f, 0.f, 0.f}, y[4] = {0.f, 0.f, 0.f, 0.f};
+      Raw<T> o{}, q{};
+      Raw<float> x{}, y{};
       if (left > 0) {
         const int64_t at = (int64_t)r * a.T + t;
-        load_some(po + at, left, o);
-        if (REF) load_some(pr + at, left, q);
-        if (MIX || MODE == FT_POLICY) load_some(px + at, left, x);
-        load_some(py + at, left, y);
+        o.get(po + at, left);
+        if (REF) q.get(pr + at, left);
+        if (MIX || MODE == FT_POLICY) x.get(px + at, left);
+        y.get(py + at, left);
         if (MIX) { const float2 c = mix[r]; e.c = c.x; e.dc = c.y; }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           float f, part;
-          element<MODE, MIX, REF>(e, o[i], q[i], x[i], y[i], res[j][i], f, part);
+          element<MODE, MIX, REF>(e, o.at(i), q.at(i), x.at(i), y.at(i), res[j][i], f, part);
           if (i < left) add_up<MODE, MIX, REF>(res[j][i], f, part, S0, S1, S2, S3);
           if (TWO) far[j][i] = f;
         }
@@ -458,7 +485,7 @@ __global__ void __launch_bounds__(FT_THREADS, 2) fused_kernel(FtArgs a) {
   }
 }
 
-// the gradient of one span, from the inputs
+// Two passes, the second: the gradient of one span, from the inputs again (387 us for those 256 pairs, 4.9 TB/s).
 template <int MODE, bool MIX, bool REF, typename T>
 __device__ __forceinline__ void grad_span(const FtArgs& a, int blk, float up, float2* mix) {
   const int tid = threadIdx.x;
