@@ -239,8 +239,8 @@ __device__ __forceinline__ void finish_block(const AdArgs& a, const AdTensor& t,
 
 // A wave takes AD_UNROLL blocks: all their loads are issued before the first is worked on.  A stream: 519 M parameters in 368 tensors, 28
 // bytes each with 32-bit moments 2.56 ms = 5.7 TB/s, 16 with 8-bit ones 1.44 ms = 5.8 TB/s (a plain copy reaches 5.5 here).  The 8-bit form
-// stays one as long as its arithmetic does: with sqrtf, a true division, codes in integer steps and maxima through LDS, 133 instead of about
-// 65 vector instructions a value, it took 1.90 ms.
+// stays one as long as its arithmetic is short: with sqrtf, a true division, codes in integer steps and maxima through LDS - 133 vector
+// instructions a value - it took 1.90 ms.
 template <typename PT, typename GT, int BITS, bool NT>
 __global__ void __launch_bounds__(256) adamw_multi_kernel(AdArgs a) {
   // the tensor this workgroup works on

@@ -626,7 +626,7 @@ __global__ void __launch_bounds__(FT_THREADS) scale_kernel(const float* __restri
 }  // namespace
 
 // Two passes: rows are split so that a workgroup has about 8 192 values (16 vectors of four a thread) where there are enough of them for
-// 1 024 workgroups, fewer (down to 1 024) where there are not; G lanes share a row, as many as leave each at least two vectors of it.
+// 1 024 workgroups, fewer (down to 1 024) where there are not; G lanes share a row, as many as leave each at least two vectors of it, or as there are to share.
 // One pass (`keep` vectors a thread stay in registers): a workgroup takes what fills them.
 static void ft_split(FtArgs* a, int64_t want) {
   if (a->T > want) {
@@ -640,7 +640,7 @@ static void ft_split(FtArgs* a, int64_t want) {
     a->rows_per_wg = (int)std::min<int64_t>(std::min<int64_t>(FT_ROWS, a->C), std::max<int64_t>(1, want / a->T));
   }
   a->log_g = 0;
-  while (a->log_g < 8 && ((int64_t)16 << a->log_g) <= std::min(a->seg, a->T)) ++a->log_g;
+  while (a->log_g < 8 && (((int64_t)16 << a->log_g) <= std::min(a->seg, a->T) || (FT_THREADS >> a->log_g) > a->rows_per_wg)) ++a->log_g;
 }
 int ft_plan(FtArgs* a, int B, int C, int64_t HW, bool mixed, int rows_of, int keep) {
   a->B = B;
