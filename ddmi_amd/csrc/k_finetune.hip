@@ -130,6 +130,7 @@ __device__ __forceinline__ void total_weight(const FtArgs& a, double* red) {
     for (int j = threadIdx.x; j < rows; j += FT_THREADS)
       if (takes_part<MODE>(a, j)) total += a.weight ? (double)a.weight[j] : 1.0;
     total = block_sum(total, red);
+    __syncthreads();                  // `red` is the caller's again
   }
   if (threadIdx.x == 0) *a.total = total;
 }
@@ -238,7 +239,38 @@ __device__ __forceinline__ RowOut policy_row(const FtArgs& a, bool used, double 
   o.coef[0] = make_float2((float)((free ? open * w / (var * n) : (clipped ? 0.0 : open + bound)) * E), (float)(w * a.kl_coef * E * E / (var * n)));
   return o;
 }
+constexpr unsigned long long FT_OPEN = 0xFFFFFFFFFFFFFFFFull;   // a sum that is not there yet (one pass, below); no sum is stored as this NaN
+// the sums of one sample, by one wave: lane i adds those of spans i, i + 64 ...; false when one did not show up within `polls` looks
+__device__ __forceinline__ bool wave_sums(const FtArgs& a, int64_t first, int& polls, double2& out) {
+  unsigned long long* p = reinterpret_cast<unsigned long long*>(a.part + first);
+  double u = 0.0, v = 0.0;
+  for (int j0 = 0; j0 < a.wps; j0 += 64) {
+    const int j = j0 + (threadIdx.x & 63);
+    unsigned long long x = 0, y = 0;
+    for (;;) {
+      if (j < a.wps) {
+        x = __hip_atomic_load(p + 2 * j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        y = __hip_atomic_load(p + 2 * j + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+      }
+      if (__all(x != FT_OPEN && y != FT_OPEN)) break;
+      if (--polls < 0) return false;
+      __builtin_amdgcn_s_sleep(8);
+    }
+    u += __longlong_as_double((long long)x);
+    v += __longlong_as_double((long long)y);
+  }
+  for (int st = 32; st > 0; st >>= 1) { u += __shfl_xor(u, st); v += __shfl_xor(v, st); }
+  out = make_double2(u, v);
+  return true;
+}
 __device__ __forceinline__ double2 sample_sums(const FtArgs& a, int sample, double* red) {
+  if (a.fused) {                      // all are there; in the order of the workgroups that waited for them: the same factors to the last bit
+    double2 out;
+    int polls = 0;
+    wave_sums(a, (int64_t)sample * a.wps, polls, out);
+    return out;
+  }
+
   double u = 0.0, v = 0.0;
   for (int j = threadIdx.x; j < a.wps; j += FT_THREADS) {
     const double2 p = a.part[(int64_t)sample * a.wps + j];
@@ -296,7 +328,6 @@ __global__ void __launch_bounds__(FT_THREADS) loss_kernel(FtArgs a, int rows) {
 // places with a NaN that no sum is stored as - so publishing is two relaxed agent-scope stores, with no fence and no counter.  The wait is
 // bounded: a workgroup whose neighbours do not show up (other kernels hold the compute units) leaves its span undone, and grad_kernel,
 // which runs after it in any case (loss and logits' gradients need every sample), computes what is not done.
-constexpr unsigned long long FT_OPEN = 0xFFFFFFFFFFFFFFFFull;
 int g_polls = 1 << 12;                  // some milliseconds; the spans of a row start within microseconds of each other
 
 template <int MODE>
@@ -309,29 +340,6 @@ __global__ void __launch_bounds__(FT_THREADS) open_kernel(FtArgs a, int64_t plac
 __device__ __forceinline__ void publish(double* place, double v) {
   const unsigned long long bits = v != v ? 0x7FF8000000000000ull : (unsigned long long)__double_as_longlong(v);
   __hip_atomic_store(reinterpret_cast<unsigned long long*>(place), bits, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-// the sums of one sample, by one wave: lane i adds those of spans i, i + 64 ...; false when one did not show up
-__device__ __forceinline__ bool await_sums(const FtArgs& a, int64_t first, int lane, int& polls, double2& out) {
-  unsigned long long* p = reinterpret_cast<unsigned long long*>(a.part + first);
-  double u = 0.0, v = 0.0;
-  for (int j0 = 0; j0 < a.wps; j0 += 64) {
-    const int j = j0 + lane;
-    unsigned long long x = 0, y = 0;
-    for (;;) {
-      if (j < a.wps) {
-        x = __hip_atomic_load(p + 2 * j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-        y = __hip_atomic_load(p + 2 * j + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-      }
-      if (__all(x != FT_OPEN && y != FT_OPEN)) break;
-      if (--polls < 0) return false;
-      __builtin_amdgcn_s_sleep(8);
-    }
-    u += __longlong_as_double((long long)x);
-    v += __longlong_as_double((long long)y);
-  }
-  for (int st = 32; st > 0; st >>= 1) { u += __shfl_xor(u, st); v += __shfl_xor(v, st); }
-  out = make_double2(u, v);
-  return true;
 }
 // four values as they are stored, of which `left` exist: no conversion, so that the next load does not wait for this one
 template <typename T> struct Raw;
@@ -453,8 +461,8 @@ __global__ void __launch_bounds__(FT_THREADS, 2) fused_kernel(FtArgs a) {
     int polls = a.polls;
     double2 s0 = make_double2(0.0, 0.0), s1 = make_double2(0.0, 0.0);
     const int64_t first = (int64_t)(MODE == FT_PREF ? 2 * row : row) * a.wps;
-    bool ok = await_sums(a, first, tid, polls, s0);
-    if (MODE == FT_PREF && ok) ok = await_sums(a, first + a.wps, tid, polls, s1);
+    bool ok = wave_sums(a, first, polls, s0);
+    if (MODE == FT_PREF && ok) ok = wave_sums(a, first + a.wps, polls, s1);
     const RowOut o = MODE == FT_PREF ? pref_row(a, true, w, s0, s1) : policy_row(a, true, w, row, s0);
     if (tid == 0) {
       const float up = a.dloss ? *a.dloss : 1.f;

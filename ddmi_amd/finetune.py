@@ -124,17 +124,27 @@ class _Call:
 
 class _LossFn(torch.autograd.Function):
     """What the two losses share: `launch` computes loss, statistics and, along with them, the gradients for an upstream gradient of 1.  The
-    first backward hands those out - multiplied in place when the upstream gradient, which only the device knows, is another - and a later
-    one (retain_graph) computes them again from the saved inputs."""
+    first backward hands those out - multiplied in place when the upstream gradient, which only the device knows, is another (a bf16 gradient
+    is then rounded a second time) - and a later one (retain_graph) computes them again from the saved inputs."""
+
+    @classmethod
+    def run(cls, model_out, mixing_logit, *args):
+        """apply(), or without a graph to build, the loss alone."""
+        if torch.is_grad_enabled() and (model_out.requires_grad or (mixing_logit is not None and mixing_logit.requires_grad)):
+            return cls.apply(model_out, mixing_logit, *args)
+        call, extra, args = cls.arguments(model_out, mixing_logit, *args)
+        return cls.launch(call, extra, args, None, False, False)[0]
+
+    @classmethod
+    def _start(cls, ctx, *inputs):
+        return cls._forward(ctx, *cls.arguments(*inputs))
 
     @classmethod
     def _forward(cls, ctx, call, extra, args):
         ctx.mixed = call.tensors[5] is not None and ctx.needs_input_grad[1]
-        grads = ctx.needs_input_grad[0] or ctx.needs_input_grad[1]
-        outs, ctx.grads = cls.launch(call, extra, args, None, grads, ctx.mixed)
-        if grads:
-            ctx.save_for_backward(*call.tensors, *extra)
-            ctx.args, ctx.index = args, call.index
+        outs, ctx.grads = cls.launch(call, extra, args, None, True, ctx.mixed)
+        ctx.save_for_backward(*call.tensors, *extra)
+        ctx.args, ctx.index = args, call.index
         ctx.mark_non_differentiable(*outs[1:])
         return outs
 
@@ -160,9 +170,12 @@ class _LossFn(torch.autograd.Function):
 
 class PreferenceLossFn(_LossFn):
     @staticmethod
-    def forward(ctx, model_out, mixing_logit, ref_out, x_t, noise, sqrt_1mac, ref_logit, weight, beta, label_smoothing):
-        call = _Call(model_out, ref_out, x_t, noise, sqrt_1mac, mixing_logit, ref_logit, weight)
-        return PreferenceLossFn._forward(ctx, call, (), (beta, label_smoothing))
+    def arguments(model_out, mixing_logit, ref_out, x_t, noise, sqrt_1mac, ref_logit, weight, beta, label_smoothing):
+        return _Call(model_out, ref_out, x_t, noise, sqrt_1mac, mixing_logit, ref_logit, weight), (), (beta, label_smoothing)
+
+    @staticmethod
+    def forward(ctx, *inputs):
+        return PreferenceLossFn._start(ctx, *inputs)
 
     @staticmethod
     def launch(call, extra, args, g, grads, mixed):
@@ -183,10 +196,13 @@ class PreferenceLossFn(_LossFn):
 
 class PolicyLossFn(_LossFn):
     @staticmethod
-    def forward(ctx, model_out, mixing_logit, ref_out, x_t, x_prev, sqrt_1mac, ref_logit, weight, transition, logp_old, advantage, clip_range,
-                kl_coef):
-        call = _Call(model_out, ref_out, x_t, x_prev, sqrt_1mac, mixing_logit, ref_logit, weight)
-        return PolicyLossFn._forward(ctx, call, (transition.contiguous(), logp_old.contiguous(), advantage.contiguous()), (clip_range, kl_coef))
+    def arguments(model_out, mixing_logit, ref_out, x_t, x_prev, sqrt_1mac, ref_logit, weight, transition, logp_old, advantage, clip_range, kl_coef):
+        return (_Call(model_out, ref_out, x_t, x_prev, sqrt_1mac, mixing_logit, ref_logit, weight),
+                (transition.contiguous(), logp_old.contiguous(), advantage.contiguous()), (clip_range, kl_coef))
+
+    @staticmethod
+    def forward(ctx, *inputs):
+        return PolicyLossFn._start(ctx, *inputs)
 
     @staticmethod
     def launch(call, extra, args, g, grads, mixed):
@@ -235,7 +251,7 @@ def preference_loss(model_out, ref_out, x_t, noise, sqrt_1mac, beta, mixing_logi
     dev = _check_device(who, model_out, ref_out, x_t, noise, sqrt_1mac, mixing_logit, ref_mixing_logit, weight)
     with _lib.on_device(dev):
         _lib.init_device(dev)
-        return PreferenceLoss(*PreferenceLossFn.apply(model_out, mixing_logit, ref_out, x_t, noise, sqrt_1mac, ref_mixing_logit, weight, beta,
+        return PreferenceLoss(*PreferenceLossFn.run(model_out, mixing_logit, ref_out, x_t, noise, sqrt_1mac, ref_mixing_logit, weight, beta,
                                                       label_smoothing))
 
 
@@ -272,7 +288,7 @@ def policy_loss(model_out, x_t, x_prev, transition, sqrt_1mac, logp_old, advanta
     dev = _check_device(who, model_out, ref_out, x_t, x_prev, transition, sqrt_1mac, logp_old, advantage, mixing_logit, ref_mixing_logit, weight)
     with _lib.on_device(dev):
         _lib.init_device(dev)
-        return PolicyLoss(*PolicyLossFn.apply(model_out, mixing_logit, ref_out, x_t, x_prev, sqrt_1mac, ref_mixing_logit, weight, transition, logp_old,
+        return PolicyLoss(*PolicyLossFn.run(model_out, mixing_logit, ref_out, x_t, x_prev, sqrt_1mac, ref_mixing_logit, weight, transition, logp_old,
                                               advantage, clip_range, kl_coef))
 
 

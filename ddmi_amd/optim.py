@@ -32,10 +32,14 @@ def blocks_of(n: int) -> int:
     return -(-n // BLOCK)
 
 
-def _overlap(ptrs, nbytes) -> bool:
+def _overlap(ptrs, nbytes, written) -> bool:
+    """Whether a range that is written meets any other."""
     at = np.argsort(ptrs, kind="stable")
-    p, n = ptrs[at].astype(np.int64), nbytes[at]
-    return bool(np.any(p[:-1] + n[:-1] > p[1:]))
+    start, w = ptrs[at].astype(np.int64), written[at]
+    end = start + nbytes[at]
+    before = np.maximum.accumulate(end)[:-1]                                     # where the ranges so far end
+    before_written = np.maximum.accumulate(np.where(w, end, 0))[:-1]
+    return bool(np.any(before_written > start[1:]) or np.any(w[1:] & (before > start[1:])))
 
 
 def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], exp_avgs: Sequence[torch.Tensor], exp_avg_sqs: Sequence[torch.Tensor],
@@ -108,8 +112,11 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     state = [("exp_avg", 4 * numel if bits == 32 else numel), ("exp_avg_sq", 4 * numel if bits == 32 else numel)]
     state += [("exp_avg_scale", 4 * blocks), ("exp_avg_sq_scale", 4 * blocks)] if bits == 8 else []
     used = numel > 0
-    if _overlap(np.concatenate([e[k][used] for k in ("param", *(k for k, _ in state))]), np.concatenate([p_bytes[used], *(v[used] for _, v in state)])):
-        raise ValueError(f"{who}: two of the tensors that are written share memory (the same one twice?)")
+    g_bytes = numel * (4 if g_types.count(torch.float32) == n else np.array([t.itemsize for t in g_types], dtype=np.int64))
+    ranges = [("grad", g_bytes), ("param", p_bytes)] + state
+    ptrs, size = np.concatenate([e[k][used] for k, _ in ranges]), np.concatenate([v[used] for _, v in ranges])
+    if _overlap(ptrs, size, np.arange(len(ptrs)) >= int(used.sum())):
+        raise ValueError(f"{who}: a tensor that is written shares memory with another (the same one twice?)")
     with _lib.on_device(dev):
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError(f"{who}: not inside a graph capture: the step number is an argument and would be frozen")

@@ -1302,7 +1302,13 @@ class LDMTrainStep:
             ema["ema_model." + k] = v.clone()
         group = {"lr": self.lr, "betas": tuple(self.betas), "eps": self.eps, "weight_decay": self.wd, "amsgrad": False, "maximize": False,
                  "foreach": None, "capturable": False, "differentiable": False, "fused": None, "params": list(range(len(named)))}
-        return {"args": dict(args) if args else {"ddpmconfig": dict(self._ddpmconfig)}, "step": int(self.epoch),
+        extra = {}
+        if self.reference is not None:      # a fine-tuning that resumes goes on against the same reference network
+            off, extra["reference"] = 0, {}
+            for k, p in named:
+                extra["reference"][k] = self.reference[off:off + p.numel()].view(p.shape).clone()
+                off += p.numel()
+        return {**extra, "args": dict(args) if args else {"ddpmconfig": dict(self._ddpmconfig)}, "step": int(self.epoch),
                 "current_iters": int(self.current_iters), "vaemodel": vaemodel_state or {}, "mlp": mlp_state or {},
                 "diffusion": sd, "ema": ema, "dae_opt": {"state": opt_state if self.opt_step > 0 else {}, "param_groups": [group]},
                 "scaler": None}
@@ -1332,6 +1338,11 @@ class LDMTrainStep:
                 self.ema_step = int(ema["step"]) if "step" in ema else 0
             if not resume:
                 return self
+            if ck.get("reference"):
+                self.reference, off = torch.empty_like(self.flat.data), 0
+                for k, p in named:
+                    self.reference[off:off + p.numel()].copy_(torch.as_tensor(ck["reference"][k]).to(self.device, torch.float32).reshape(-1))
+                    off += p.numel()
             opt = ck.get("dae_opt") or {}
             if "state" in opt:
                 steps = []

@@ -181,8 +181,8 @@ def train_main(args, dc, rank, world, dev):
         # EMA would restart from the online weights and AdamW's bias correction from step 0
         step.load_training_state(ck, resume=bool(getattr(args, "resume", False)))
         print(f"restored EMA (step {step.ema_step})" + (f", AdamW state, optimizer step {step.opt_step}" if getattr(args, "resume", False) else ""))
-    if objective == "preference":
-        step.set_reference()     # the weights that fine-tuning starts from
+    if objective == "preference" and step.reference is None:     # a resumed fine-tuning has its reference from the checkpoint
+        step.set_reference()                                          # the weights that fine-tuning starts from
     lat = None
     if dc.get("latents") and os.path.exists(dc.latents):
         lat = torch.from_numpy(np.load(dc.latents).astype(np.float32))

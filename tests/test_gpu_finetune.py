@@ -363,11 +363,15 @@ def test_adamw_writes_nothing_behind_a_tensor():
 def test_adamw_refuses_shared_memory_and_captures():
     p = [torch.zeros(8, device=DEV)]
     s = lambda: [torch.zeros(8, device=DEV), torch.zeros(8, device=DEV)]      # noqa: E731
-    with pytest.raises(ValueError, match="share memory"):
+    with pytest.raises(ValueError, match="shares memory"):
         adamw_step(p * 2, s(), s(), s(), 1, lr=0.1)
     big = torch.zeros(12, device=DEV)
-    with pytest.raises(ValueError, match="share memory"):
+    with pytest.raises(ValueError, match="shares memory"):
         adamw_step([big[:8], big[4:]], s(), s(), s(), 1, lr=0.1)
+    with pytest.raises(ValueError, match="shares memory"):
+        adamw_step(p, [big[:8]], [big[4:]], s()[:1], 1, lr=0.1)
+    same = torch.ones(8, device=DEV)                      # one gradient for two parameters is only read
+    adamw_step(s(), [same, same], s(), s(), 1, lr=0.1)
     g, a, b = s()[:1], s()[:1], s()[:1]
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):

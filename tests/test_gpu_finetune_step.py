@@ -171,5 +171,12 @@ def test_main_fine_tunes_from_preferences(golden, tmp_path):
 
     log = run("a.yaml")
     assert "iter 0: Dae loss : 0.6931" in log and "after 2 optimizer steps" in log
+    import shutil
+    shutil.copy(os.path.join(save, "ldm-last.pt"), os.path.join(save, "first.pt"))
     log = run("b.yaml", resume=True)
     assert "AdamW state, optimizer step 2" in log and "after 4 optimizer steps" in log
+    first, second = (torch.load(p, map_location="cpu", weights_only=True) for p in (os.path.join(save, "first.pt"), os.path.join(save, "ldm-last.pt")))
+    assert second["reference"].keys() == first["reference"].keys()
+    for k, v in first["reference"].items():           # resumed against the network that the first run started from
+        assert torch.equal(v, second["reference"][k]), k
+    assert any(not torch.equal(v, first["diffusion"][k]) for k, v in first["reference"].items())
