@@ -199,7 +199,7 @@ def check(got, want, what=""):
         if v is None:
             assert got[name] is None, name
             continue
-        g, (w, bound) = got[name].double().cpu(), (t.cpu() for t in v)
+        g, (w, bound) = got[name].detach().double().cpu(), (t.cpu() for t in v)
         g = g.reshape(w.shape)
         assert torch.isfinite(g).all(), (what, name)
         over = (g - w).abs() - bound
@@ -221,11 +221,11 @@ def mix32(x):
     return x ^ (x >> 16)
 
 
-def random_bits(n, seed, step, index):
-    """32 bits for each value of tensor `index` of the list."""
+def random_bits(n, seed, step, index, first=0):
+    """32 bits for each of n values of tensor `index` of the list, from value `first` on."""
     key = mix32((mix32(mix32(seed & MASK) + step * 0x9E3779B9 & MASK) + (index + 1) * 0x85EBCA77) & MASK)
-    i = torch.arange(n, dtype=torch.int64)
-    return mix32((mix32((key + (i // 256) * 0x9E3779B9) & MASK) + (i % 256) * 0x9E3779B9) & MASK)
+    i = torch.arange(first, first + n, dtype=torch.int64)
+    return mix32((mix32((key + ((i // 256) & MASK) * 0x9E3779B9) & MASK) + (i % 256) * 0x9E3779B9) & MASK)
 
 
 GRID = torch.arange(127, dtype=torch.uint8).view(torch.float8_e4m3fn).double()      # the code's values that are not negative

@@ -212,6 +212,22 @@ def test_same_bits_on_every_run_and_stream(op, B, C, T):
         assert torch.equal(a[k], b[k]) and torch.equal(a[k], c[k]), k
 
 
+def test_two_streams_at_once():
+    """Large calls of both losses on two streams, each waiting for its own workgroups: the results are those of either alone."""
+    sets = [(op, R.make(op, B, C, T, seed=B, device=DEV)) for op, (B, C, T) in (("pref", LARGE[0]), ("policy", LARGE[1]), ("policy", LARGE[4]), ("pref", LARGE[1]))]
+    want = [call(op, d) for op, d in sets]
+    torch.cuda.synchronize()
+    streams, got = [torch.cuda.Stream(), torch.cuda.Stream()], []
+    for rep in range(4):
+        for i, (op, d) in enumerate(sets):
+            with torch.cuda.stream(streams[(i + rep) % 2]):
+                got.append((i, call(op, d)))
+    torch.cuda.synchronize()
+    for i, g in got:
+        for k in g:
+            assert torch.equal(g[k], want[i][k]), (i, k)
+
+
 @pytest.mark.parametrize("op", ["pref", "policy"])
 @pytest.mark.parametrize("B,C,T", [(6, 7, 131), (80, 33, 2501)])
 def test_captured_and_replayed(op, B, C, T):
@@ -464,3 +480,71 @@ def test_adamw_class_steps_groups_and_checkpoints(bits):
     before = [p.detach().clone() for p in ps]
     a.step()
     assert all(torch.equal(x, p) for x, p in zip(before, ps)) and a.steps == [4, 3, 4]
+
+
+def test_adamw_of_a_tensor_of_more_than_2_to_32_values():
+    """Offsets that pass 32 bits: places around 2^32 and the end, against the formula with their own random bits."""
+    n = 2 ** 32 + 777
+    g = torch.Generator().manual_seed(5)
+    base = [torch.randn(1 << 20, generator=g).to(DEV, torch.bfloat16) for _ in range(2)]
+    tile = lambda b: b.repeat(-(-n // b.numel()))[:n]      # noqa: E731
+    p, grad = tile(base[0]), tile(base[1])
+    m, v = (torch.zeros(n, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn) for _ in range(2))
+    scales = [torch.ones(blocks_of(n), device=DEV) for _ in range(2)]
+    hyper = dict(lr=2e-3, betas=(0.9, 0.99), eps=1e-7, weight_decay=0.1)
+    adamw_step([p], [grad], [m], [v], 1, seed=3, exp_avg_scales=[scales[0]], exp_avg_sq_scales=[scales[1]], **hyper)
+    for first, count in ((0, 1024), (2 ** 31 - 512, 1024), (2 ** 32 - 512, 1024), (2 ** 32 + 512, 265)):
+        here = slice(first, first + count)
+        old = [tile_of.repeat(2)[first % (1 << 20):][:count].cpu().double() for tile_of in base]
+        want = R.adamw(old[0], old[1], torch.zeros(count, dtype=torch.float64), torch.zeros(count, dtype=torch.float64), 1, **hyper)
+        rnd = R.random_bits(count, 3, 1, 0, first)
+        p1, e_p = want["p"]
+        unit = torch.exp2(torch.frexp(p1)[1].double() - 8)
+        cut = (R.mix32(rnd ^ 0x68E31DA4) & 0xFFFF).double() * 2.0 ** -16
+        lo, hi = (((p1.abs() + s * e_p) / unit + cut).floor() * unit for s in (-1, 1))
+        got = p[here].cpu().double()
+        assert ((got.abs() >= lo - e_p) & (got.abs() <= hi + e_p)).all(), first
+        blk = slice(first // 256, -(-(first + count) // 256))
+        for k, t, scale, r, root in (("m", m, scales[0], ((rnd & 0xFFF) << 8) | 0x80, False), ("root", v, scales[1], rnd >> 12, True)):
+            w, e = want[k]
+            s = scale[blk].cpu().double()
+            assert ((s >= R.block_scales((w.abs() - e).clamp_min(0))) & (s <= R.block_scales(w.abs() + e))).all(), (first, k)
+            lo, hi = R.codes_allowed(w, e, s, r, root)
+            code = t[here].cpu().float().double()
+            assert ((code.abs() >= lo) & (code.abs() <= hi)).all(), (first, k)
+
+
+@pytest.mark.parametrize("op", ["pref", "policy"])
+def test_losses_of_more_than_2_to_31_values(op):
+    """The last pair / transition of a batch whose offsets pass 2^31, against the same one alone (the mean over n rows divides by n)."""
+    C, T, B = 64, 65536, 514
+    rows = B // 2 if op == "pref" else B
+    small = R.make(op, 2 if op == "pref" else 1, C, T, torch.bfloat16, seed=3, device=DEV)
+    d = {}
+    for k, t in small.items():
+        if not isinstance(t, torch.Tensor) or "logit" in k:
+            d[k] = t
+        elif op == "pref":        # preferred rows, then rejected ones
+            d[k] = torch.cat([h.expand((rows,) + h.shape[1:]) for h in t.split(1)]).contiguous()
+        else:
+            d[k] = t.expand((B,) + t.shape[1:]).contiguous()
+    alone, got = call(op, small), call(op, d)
+    for k in ("margin",) if op == "pref" else ("logp", "ratio", "kl"):
+        assert torch.allclose(got[k].double(), alone[k].double().expand(rows), rtol=4 * R.U, atol=1e-9), k
+    # The gradient times n is that of the row alone, and within the same bound of the formula: every rounding is relative to what it rounds (a
+    # bare multiple of bf16's half step is not enough where the residual's and the KL term's parts of a gradient cancel: they are rounded
+    # before they are added), but for the least numbers, which grow with n.
+    w, bound = reference(op, small)["d_model_out"]
+    for i in ([0, rows - 1, rows, B - 1] if op == "pref" else [0, 256, B - 1]):
+        j = i // rows if op == "pref" else 0
+        assert ((got["d_model_out"][i].double() * rows - w[j].to(DEV)).abs() <= bound[j].to(DEV) + rows * 2.0 ** -133).all(), i
+    assert torch.allclose(got["d_logit"], alone["d_logit"], rtol=1e-4, atol=1e-4 * float(alone["d_logit"].abs().max()))
+
+
+def test_adamw_skips_empty_tensors_and_steps_nothing_else():
+    z = lambda *s: torch.zeros(s, device=DEV)      # noqa: E731
+    a = AdamW([z(0), torch.ones(3, device=DEV), z(4, 0)], lr=0.1, state_bits=8)
+    for p in a.params:
+        p.grad = torch.ones_like(p)
+    a.step()
+    assert a.steps == [1, 1, 1] and (a.params[1] < 1).all()

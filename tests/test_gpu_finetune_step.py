@@ -51,6 +51,7 @@ def test_preference_step_gradients():
     h = -2.5 * ((e - e_ref)[:3] - (e - e_ref)[3:])
     loss = -(0.9 * torch.nn.functional.logsigmoid(h) + 0.1 * torch.nn.functional.logsigmoid(-h)).mean()
     loss.backward()
+    loss = loss.detach()
     assert abs(float(out.loss) - float(loss)) < TOL_FP32 * float(loss)
     assert rel_err(out.margin.cpu(), h.detach().cpu()) < TOL_FP32 and rel_err(out.mse.cpu(), e.detach().cpu()) < TOL_FP32
     floor = 1e-6 * float(b.flat.grad.abs().max())
@@ -78,6 +79,24 @@ def test_preference_steps_leave_the_reference_alone(numerics, bits):
     assert not torch.equal(tr.flat.data, before)
     tr.train_step(zw, t, noise)                       # ordinary training goes on with the same optimizer
     assert tr.opt_step == 5
+
+
+def test_8_bit_moments_with_a_captured_micro_step():
+    """use_graph: the captured micro-step fills the slab, the optimizer runs behind it; the same states as without a graph."""
+    runs = []
+    for graph in (False, True):
+        tr = trainer(optimizer_state_bits=8, use_graph=graph)
+        for k in range(4):
+            zw, _, noise, t = (v.to(DEV) for v in pairs(seed=k))
+            tr.train_step(zw, t, noise)
+        runs.append(tr)
+    assert torch.equal(runs[0].flat.data, runs[1].flat.data)
+    tr = runs[1].set_reference()
+    zw, zl, noise, t = (v.to(DEV) for v in pairs(seed=9))
+    tr.preference_step(zw, zl, beta=10.0, t=t, noise=noise)        # twice the batch: the arena may move, graphs are made again
+    tr.train_step(zw, t, noise)
+    tr.train_step(zw, t, noise)
+    assert torch.isfinite(tr.flat.data).all() and tr.opt_step == 7
 
 
 def test_first_step_of_8_bit_moments_is_that_of_32():
