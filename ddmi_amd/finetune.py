@@ -104,121 +104,66 @@ def _flat(t):
     return None if t is None else (t.detach() if t.requires_grad else t).contiguous()
 
 
-class _Call:
-    """The arguments of a loss's C entry points: contiguous tensors, kept alive, and the struct that points at them."""
-    __slots__ = ("tensors", "B", "C", "HW", "out_dtype", "index")
+def _launch(entry, tensors, extra, args, stats, g, grads, mixed):
+    """One call of a loss's C entry point: ((loss, *statistics), (d_model_out, d_logit)).  tensors: model_out, ref_out, x_t, noise / x_prev,
+    sqrt_1mac, mixing_logit, ref_mixing_logit, weight - contiguous; extra: the tensors, args: the numbers behind them; stats: rows of each
+    statistic; g: the upstream gradient (None: 1); grads, mixed: whether the output's / the logit's gradient is wanted."""
+    out, logit = tensors[0], tensors[5]
+    B, Cc, dev = out.shape[0], out.shape[1], out.device
+    HW = out.numel() // (B * Cc)
+    d_out = torch.empty_like(out) if grads else None
+    d_logit = torch.empty_like(logit) if mixed else None
+    results = [torch.empty((), dtype=torch.float32, device=dev)] + [torch.empty((n,), dtype=torch.float32, device=dev) for n in stats]
+    ws = torch.empty(_workspace_bytes(B, Cc, HW, logit is not None), dtype=torch.uint8, device=dev)
+    given = _lib.LossIn(*map(_p, tensors), HW, Cc, _OUT_TYPES[out.dtype])
+    _lib.check(entry(C.byref(given), *args[0], *map(_p, extra), *args[1], _p(g), ws.data_ptr(), ws.numel(), *map(_p, results), _p(d_out), _p(d_logit),
+                     _lib.raw_stream(out.get_device())))
+    return results, (d_out, d_logit)
 
-    def __init__(self, *tensors):      # model_out, ref_out, x_t, noise / x_prev, sqrt_1mac, mixing_logit, ref_mixing_logit, weight
-        self.tensors = tuple(map(_flat, tensors))
-        out = tensors[0]
-        self.B, self.C = out.shape[0], out.shape[1]
-        self.HW = out.numel() // (self.B * self.C)
-        self.out_dtype, self.index = _OUT_TYPES[out.dtype], out.get_device()
 
-    def struct(self):
-        return _lib.LossIn(*map(_p, self.tensors), self.HW, self.C, self.out_dtype)
+class LossFn(torch.autograd.Function):
+    """A loss that is computed already, its gradients for an upstream gradient of 1 along with it.  The first backward hands those out -
+    multiplied in place when the upstream gradient, which only the device knows, is another (a bf16 gradient is then rounded a second time) -
+    and a later one (retain_graph) computes them again from the saved inputs."""
 
-    def workspace(self):
-        return torch.empty(_workspace_bytes(self.B, self.C, self.HW, self.tensors[5] is not None), dtype=torch.uint8, device=self.tensors[0].device)
+    @staticmethod
+    def forward(ctx, model_out, mixing_logit, loss, grads, again):      # loss, grads in lists: they are no inputs
+        entry, tensors, extra, *rest = again
+        ctx.save_for_backward(*tensors, *extra)
+        ctx.grads, ctx.again, ctx.index = grads, (entry, rest), model_out.get_device()
+        return loss[0]
 
+    @staticmethod
+    def backward(ctx, g):
+        return LossFn._with_graph(ctx, g) if torch.is_grad_enabled() else LossFn._gradients(ctx, g)
 
-class _LossFn(torch.autograd.Function):
-    """What the two losses share: `launch` computes loss, statistics and, along with them, the gradients for an upstream gradient of 1.  The
-    first backward hands those out - multiplied in place when the upstream gradient, which only the device knows, is another (a bf16 gradient
-    is then rounded a second time) - and a later one (retain_graph) computes them again from the saved inputs."""
-
-    @classmethod
-    def run(cls, model_out, mixing_logit, *args):
-        """apply(), or without a graph to build, the loss alone."""
-        if torch.is_grad_enabled() and (model_out.requires_grad or (mixing_logit is not None and mixing_logit.requires_grad)):
-            return cls.apply(model_out, mixing_logit, *args)
-        call, extra, args = cls.arguments(model_out, mixing_logit, *args)
-        return cls.launch(call, extra, args, None, False, False)[0]
-
-    @classmethod
-    def _start(cls, ctx, *inputs):
-        return cls._forward(ctx, *cls.arguments(*inputs))
-
-    @classmethod
-    def _forward(cls, ctx, call, extra, args):
-        ctx.mixed = call.tensors[5] is not None and ctx.needs_input_grad[1]
-        outs, ctx.grads = cls.launch(call, extra, args, None, True, ctx.mixed)
-        ctx.save_for_backward(*call.tensors, *extra)
-        ctx.args, ctx.index = args, call.index
-        ctx.mark_non_differentiable(*outs[1:])
-        return outs
-
-    @classmethod
-    def _backward(cls, ctx, g):
-        if g.dtype != torch.float32 or not g.is_contiguous():
-            g = g.float().contiguous()
+    @staticmethod
+    def _gradients(ctx, g):
+        if not g.is_contiguous():
+            g = g.contiguous()
         with _lib.on_device(ctx.index):
             if ctx.grads is not None:
                 (d_out, d_logit), ctx.grads = ctx.grads, None
                 _lib.check(_lib.lib().ddmi_train_loss_scale(g.data_ptr(), d_out.data_ptr(), _OUT_TYPES[d_out.dtype], d_out.numel(), _p(d_logit),
                                                             0 if d_logit is None else d_logit.numel(), _lib.raw_stream(ctx.index)))
             else:
-                saved = ctx.saved_tensors
-                d_out, d_logit = cls.launch(_Call(*saved[:8]), saved[8:], ctx.args, g, True, ctx.mixed)[1]
-        return d_out, d_logit
+                saved, (entry, (args, stats, mixed)) = ctx.saved_tensors, ctx.again
+                d_out, d_logit = _launch(entry, saved[:8], saved[8:], args, stats, g, True, mixed)[1]
+        return d_out, d_logit, None, None, None
 
-    @staticmethod
-    def buffers(call, grads, mixed):
-        d_out = torch.empty_like(call.tensors[0]) if grads else None
-        return d_out, torch.empty_like(call.tensors[5]) if mixed else None
+    _with_graph = staticmethod(once_differentiable(_gradients.__func__))      # create_graph: a second derivative through here raises
 
 
-class PreferenceLossFn(_LossFn):
-    @staticmethod
-    def arguments(model_out, mixing_logit, ref_out, x_t, noise, sqrt_1mac, ref_logit, weight, beta, label_smoothing):
-        return _Call(model_out, ref_out, x_t, noise, sqrt_1mac, mixing_logit, ref_logit, weight), (), (beta, label_smoothing)
-
-    @staticmethod
-    def forward(ctx, *inputs):
-        return PreferenceLossFn._start(ctx, *inputs)
-
-    @staticmethod
-    def launch(call, extra, args, g, grads, mixed):
-        dev, pairs, ws = call.tensors[0].device, call.B // 2, call.workspace()
-        loss = torch.empty((), dtype=torch.float32, device=dev)
-        margin = torch.empty((pairs,), dtype=torch.float32, device=dev)
-        mse = torch.empty((2 * pairs,), dtype=torch.float32, device=dev)
-        d_out, d_logit = PreferenceLossFn.buffers(call, grads, mixed)
-        _lib.check(_lib.lib().ddmi_train_pref_loss(C.byref(call.struct()), pairs, call.tensors[3].shape[0], *args, _p(g), ws.data_ptr(), ws.numel(),
-                                                   loss.data_ptr(), margin.data_ptr(), mse.data_ptr(), _p(d_out), _p(d_logit), _lib.raw_stream(call.index)))
-        return (loss, margin, mse), (d_out, d_logit)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g, _margin, _mse):
-        return PreferenceLossFn._backward(ctx, g) + (None,) * 8
-
-
-class PolicyLossFn(_LossFn):
-    @staticmethod
-    def arguments(model_out, mixing_logit, ref_out, x_t, x_prev, sqrt_1mac, ref_logit, weight, transition, logp_old, advantage, clip_range, kl_coef):
-        return (_Call(model_out, ref_out, x_t, x_prev, sqrt_1mac, mixing_logit, ref_logit, weight),
-                (transition.contiguous(), logp_old.contiguous(), advantage.contiguous()), (clip_range, kl_coef))
-
-    @staticmethod
-    def forward(ctx, *inputs):
-        return PolicyLossFn._start(ctx, *inputs)
-
-    @staticmethod
-    def launch(call, extra, args, g, grads, mixed):
-        dev, ws = call.tensors[0].device, call.workspace()
-        loss = torch.empty((), dtype=torch.float32, device=dev)
-        logp, ratio, kl = torch.empty((3, call.B), dtype=torch.float32, device=dev).unbind(0)
-        d_out, d_logit = PolicyLossFn.buffers(call, grads, mixed)
-        _lib.check(_lib.lib().ddmi_train_policy_loss(C.byref(call.struct()), call.B, *map(_p, extra), *args, _p(g), ws.data_ptr(), ws.numel(),
-                                                     loss.data_ptr(), logp.data_ptr(), ratio.data_ptr(), kl.data_ptr(), _p(d_out), _p(d_logit),
-                                                     _lib.raw_stream(call.index)))
-        return (loss, logp, ratio, kl), (d_out, d_logit)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, g, *_stats):
-        return PolicyLossFn._backward(ctx, g) + (None,) * 11
+def _loss(entry, model_out, mixing_logit, others, extra, args, stats):
+    """(loss, *statistics), the loss differentiable in model_out and mixing_logit where they ask for it."""
+    ref_out, x_t, second, sqrt_1mac, ref_mixing_logit, weight = others
+    tensors = tuple(map(_flat, (model_out, ref_out, x_t, second, sqrt_1mac, mixing_logit, ref_mixing_logit, weight)))
+    extra = tuple(map(_flat, extra))
+    mixed = mixing_logit is not None and mixing_logit.requires_grad
+    if not (torch.is_grad_enabled() and (model_out.requires_grad or mixed)):
+        return _launch(entry, tensors, extra, args, stats, None, False, False)[0]
+    results, grads = _launch(entry, tensors, extra, args, stats, None, True, mixed)
+    return [LossFn.apply(model_out, mixing_logit, results[:1], grads, (entry, tensors, extra, args, stats, mixed))] + results[1:]
 
 
 def preference_loss(model_out, ref_out, x_t, noise, sqrt_1mac, beta, mixing_logit=None, ref_mixing_logit=None, weight=None,
@@ -241,7 +186,7 @@ def preference_loss(model_out, ref_out, x_t, noise, sqrt_1mac, beta, mixing_logi
     pairs = model_out.shape[0] // 2
     if not isinstance(noise, torch.Tensor) or noise.dim() < 1 or noise.shape[0] not in (pairs, 2 * pairs):
         raise ValueError(f"{who}: noise has {pairs} (shared by a pair) or {2 * pairs} rows")
-    _expect(who, "noise", noise, (noise.shape[0],) + tuple(model_out.shape[1:]))
+    _expect(who, "noise", noise, (noise.shape[0],) + model_out.shape[1:])
     if weight is not None:
         _expect(who, "weight", weight, (pairs,))
     beta, label_smoothing = float(beta), float(label_smoothing)
@@ -251,13 +196,13 @@ def preference_loss(model_out, ref_out, x_t, noise, sqrt_1mac, beta, mixing_logi
     dev = _check_device(who, model_out, ref_out, x_t, noise, sqrt_1mac, mixing_logit, ref_mixing_logit, weight)
     with _lib.on_device(dev):
         _lib.init_device(dev)
-        return PreferenceLoss(*PreferenceLossFn.run(model_out, mixing_logit, ref_out, x_t, noise, sqrt_1mac, ref_mixing_logit, weight, beta,
-                                                      label_smoothing))
+        return PreferenceLoss(*_loss(_lib.lib().ddmi_train_pref_loss, model_out, mixing_logit, (ref_out, x_t, noise, sqrt_1mac, ref_mixing_logit, weight),
+                                     (), ((pairs, noise.shape[0]), (beta, label_smoothing)), (pairs, 2 * pairs)))
 
 
 def _check_transition(who, model_out, x_prev, transition, weight, **rows):
     B = model_out.shape[0]
-    _expect(who, "x_prev", x_prev, tuple(model_out.shape))
+    _expect(who, "x_prev", x_prev, model_out.shape)
     _expect(who, "transition", transition, (B, 3))
     for name, t in dict(rows, weight=weight).items():
         if t is not None or name != "weight":
@@ -288,8 +233,10 @@ def policy_loss(model_out, x_t, x_prev, transition, sqrt_1mac, logp_old, advanta
     dev = _check_device(who, model_out, ref_out, x_t, x_prev, transition, sqrt_1mac, logp_old, advantage, mixing_logit, ref_mixing_logit, weight)
     with _lib.on_device(dev):
         _lib.init_device(dev)
-        return PolicyLoss(*PolicyLossFn.run(model_out, mixing_logit, ref_out, x_t, x_prev, sqrt_1mac, ref_mixing_logit, weight, transition, logp_old,
-                                              advantage, clip_range, kl_coef))
+        B = model_out.shape[0]
+        return PolicyLoss(*_loss(_lib.lib().ddmi_train_policy_loss, model_out, mixing_logit,
+                                 (ref_out, x_t, x_prev, sqrt_1mac, ref_mixing_logit, weight), (transition, logp_old, advantage),
+                                 ((B,), (clip_range, kl_coef)), (B, B, B)))
 
 
 def transition_log_prob(model_out, x_t, x_prev, transition, sqrt_1mac, mixing_logit=None, weight=None) -> torch.Tensor:
@@ -300,9 +247,13 @@ def transition_log_prob(model_out, x_t, x_prev, transition, sqrt_1mac, mixing_lo
     dev = _check_device(who, model_out, x_t, x_prev, transition, sqrt_1mac, mixing_logit, weight)
     with _lib.on_device(dev):
         _lib.init_device(dev)
-        call = _Call(model_out, None, x_t, x_prev, sqrt_1mac, mixing_logit, None, weight)
-        ws, transition = call.workspace(), transition.detach().contiguous()
-        logp = torch.empty((call.B,), dtype=torch.float32, device=model_out.device)
-        _lib.check(_lib.lib().ddmi_train_policy_loss(C.byref(call.struct()), call.B, transition.data_ptr(), None, None, 0.0, 0.0, None, ws.data_ptr(),
-                                                     ws.numel(), None, logp.data_ptr(), None, None, None, None, _lib.raw_stream(call.index)))
+        B, Cc = model_out.shape[:2]
+        HW = model_out.numel() // (B * Cc)
+        tensors = tuple(map(_flat, (model_out, None, x_t, x_prev, sqrt_1mac, mixing_logit, None, weight)))
+        transition = _flat(transition)
+        logp = torch.empty((B,), dtype=torch.float32, device=model_out.device)
+        ws = torch.empty(_workspace_bytes(B, Cc, HW, mixing_logit is not None), dtype=torch.uint8, device=model_out.device)
+        given = _lib.LossIn(*map(_p, tensors), HW, Cc, _OUT_TYPES[model_out.dtype])
+        _lib.check(_lib.lib().ddmi_train_policy_loss(C.byref(given), B, transition.data_ptr(), None, None, 0.0, 0.0, None, ws.data_ptr(), ws.numel(), None,
+                                                     logp.data_ptr(), None, None, None, None, _lib.raw_stream(dev)))
         return logp
