@@ -7,15 +7,14 @@ namespace {
 bool dtype_ok(int dt) { return dt == DDMI_DTYPE_F32 || dt == DDMI_DTYPE_BF16; }
 int internal_dt(int dt) { return dt == DDMI_DTYPE_F32 ? DT_F32 : DT_BF16; }
 
-int common_args(FtArgs* a, const ddmi_loss_in* in, int B, int rows_of, int keep, void* ws, size_t ws_bytes, const char* who) {
-  const std::string w(who);
-  DDMI_REQUIRE(in->model_out && in->second && B > 0 && in->C > 0 && in->HW > 0, w + ": null argument or empty batch");
-  DDMI_REQUIRE(dtype_ok(in->out_dtype), w + ": model_out / ref_out are fp32 or bf16");
-  DDMI_REQUIRE((in->mixing_logit == nullptr) == (in->ref_mixing_logit == nullptr) || (in->mixing_logit && !in->ref_out), w + ": both mixing logits or none");
-  DDMI_REQUIRE(!in->mixing_logit || (in->x_t && in->sqrt_1mac), w + ": mixing needs x_t and sqrt_1mac");
-  DDMI_REQUIRE((double)in->C * (double)in->HW < 1.1e12, w + ": sample too large");
+int common_args(FtArgs* a, const ddmi_loss_in* in, int B, int rows_of, int keep, void* ws, size_t ws_bytes) {
+  DDMI_REQUIRE(in->model_out && in->second && B > 0 && in->C > 0 && in->HW > 0, "fine-tuning loss: null argument or empty batch");
+  DDMI_REQUIRE(dtype_ok(in->out_dtype), "fine-tuning loss: model_out / ref_out are fp32 or bf16");
+  DDMI_REQUIRE((in->mixing_logit == nullptr) == (in->ref_mixing_logit == nullptr) || (in->mixing_logit && !in->ref_out), "fine-tuning loss: both mixing logits or none");
+  DDMI_REQUIRE(!in->mixing_logit || (in->x_t && in->sqrt_1mac), "fine-tuning loss: mixing needs x_t and sqrt_1mac");
+  DDMI_REQUIRE((double)in->C * (double)in->HW < 1.1e12, "fine-tuning loss: sample too large");
   DDMI_TRY(ft_plan(a, B, in->C, in->HW, in->mixing_logit != nullptr, rows_of, keep));
-  DDMI_REQUIRE(ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= ft_workspace_bytes(*a), w + ": workspace too small or not 16-byte aligned");
+  DDMI_REQUIRE(ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= ft_workspace_bytes(*a), "fine-tuning loss: workspace too small or not 16-byte aligned");
   ft_carve(a, ws);
   a->out = in->model_out; a->ref = in->ref_out; a->x = in->x_t; a->second = in->second; a->s1 = in->mixing_logit ? in->sqrt_1mac : nullptr;
   a->logit = in->mixing_logit; a->ref_logit = in->ref_mixing_logit; a->weight = in->weight;
@@ -49,7 +48,7 @@ int ddmi_train_pref_loss(const ddmi_loss_in* in, int pairs, int noise_rows, doub
   DDMI_REQUIRE(noise_rows == pairs || noise_rows == 2 * pairs, "pref_loss: the noise has a row for each pair or for each sample");
   DDMI_REQUIRE(label_smoothing >= 0.0 && label_smoothing <= 1.0 && beta == beta, "pref_loss: label_smoothing in [0, 1], beta a number");
   DDMI_REQUIRE(!d_logit || (in->mixing_logit && d_model_out), "pref_loss: d_logit goes with mixing_logit and d_model_out");
-  DDMI_TRY(common_args(&a, in, 2 * pairs, 2, d_model_out ? FT_VECS : 0, ws, ws_bytes, "pref_loss"));
+  DDMI_TRY(common_args(&a, in, 2 * pairs, 2, d_model_out ? FT_VECS : 0, ws, ws_bytes));
   if (!in->mixing_logit) a.x = nullptr;      // not read
   a.pairs = pairs; a.second_rows = noise_rows; a.beta = beta; a.smoothing = label_smoothing;
   a.loss = loss; a.row_out[0] = margin; a.row_out[1] = mse; a.dloss = dloss; a.d_out = d_model_out; a.d_logit = d_logit;
@@ -65,7 +64,7 @@ int ddmi_train_policy_loss(const ddmi_loss_in* in, int B, const float* transitio
   DDMI_REQUIRE(kl_coef == 0.0 || in->ref_out, "policy_loss: a KL term needs the reference's output");
   DDMI_REQUIRE(logp_old || !d_model_out, "policy_loss: a gradient of the log-density alone is not offered");
   DDMI_REQUIRE(!d_logit || (in->mixing_logit && d_model_out), "policy_loss: d_logit goes with mixing_logit and d_model_out");
-  DDMI_TRY(common_args(&a, in, B, 1, d_model_out ? (in->ref_out ? FT_VECS / 2 : FT_VECS) : 0, ws, ws_bytes, "policy_loss"));
+  DDMI_TRY(common_args(&a, in, B, 1, d_model_out ? (in->ref_out ? FT_VECS / 2 : FT_VECS) : 0, ws, ws_bytes));
   a.pairs = B; a.second_rows = B; a.transition = transition;
   a.logp_old = logp_old; a.advantage = advantage; a.clip = clip_range; a.kl_coef = kl_coef;
   a.loss = logp_old ? loss : nullptr; a.row_out[0] = logp; a.row_out[1] = ratio; a.row_out[2] = kl;

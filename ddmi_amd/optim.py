@@ -9,6 +9,7 @@ step gives the same bits on every run.
 """
 from __future__ import annotations
 
+import itertools
 import operator
 from typing import Dict, List, Optional, Sequence, Union
 
@@ -77,53 +78,53 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     else:
         raise ValueError(f"{who}: moments are all fp32 or all float8_e4m3fn, got {sorted(map(str, kinds))}")
     p_types, g_types = list(map(_DTYPE, params)), list(map(_DTYPE, grads))
-    kinds = set(zip(p_types, g_types))
-    bad = {k for kind in kinds for k in kind} - set(_TYPES)
-    if bad:
-        raise ValueError(f"{who}: parameters and gradients are fp32 or bf16, got {sorted(map(str, bad))}")
-    e = np.zeros(n, dtype=_ENTRY)
-    sizes = list(map(_NUMEL, params))
-    for name, ts in (("gradient", grads), ("exp_avg", exp_avgs), ("exp_avg_sq", exp_avg_sqs)):
-        if list(map(_NUMEL, ts)) != sizes:
+    p_kinds, g_kinds = set(p_types), set(g_types)
+    if not p_kinds | g_kinds <= set(_TYPES):
+        raise ValueError(f"{who}: parameters and gradients are fp32 or bf16, got {sorted(map(str, p_kinds | g_kinds))}")
+    flat = list(itertools.chain.from_iterable(lists))
+    numels = np.fromiter(map(_NUMEL, flat), np.int64, len(flat)).reshape(-1, n)      # a row for each list
+    numel = numels[0]
+    for name, row in zip(("gradient", "exp_avg", "exp_avg_sq"), numels[1:4]):
+        if not np.array_equal(row, numel):
             raise ValueError(f"{who}: a tensor's {name} has another number of values than the parameter")
     if list(map(_SHAPE, grads)) != list(map(_SHAPE, params)):
         raise ValueError(f"{who}: a gradient has another shape than its parameter")
-    e["numel"] = numel = np.array(sizes, dtype=np.int64)
     blocks = -(-numel // BLOCK)
-    if bits == 8:
-        for ts in scales:
-            if list(map(_NUMEL, ts)) != blocks.tolist() or set(map(_DTYPE, ts)) != {torch.float32}:
-                raise ValueError(f"{who}: scales are fp32, one for each {BLOCK} values of a tensor")
-    for ts in lists:
-        if not all(map(_CONTIGUOUS, ts)):
-            raise ValueError(f"{who}: tensors are contiguous")
-    e["step"], e["lr"], e["weight_decay"], e["index"] = step, lr, weight_decay, np.arange(n)
+    if bits == 8 and (np.any(numels[4:] != blocks) or any(set(map(_DTYPE, ts)) != {torch.float32} for ts in scales)):
+        raise ValueError(f"{who}: scales are fp32, one for each {BLOCK} values of a tensor")
+    if not all(map(_CONTIGUOUS, flat)):
+        raise ValueError(f"{who}: tensors are contiguous")
+    e = np.zeros(n, dtype=_ENTRY)
+    e["numel"], e["step"], e["lr"], e["weight_decay"], e["index"] = numel, step, lr, weight_decay, np.arange(n)
     if e["step"].min() < 1:
         raise ValueError(f"{who}: step counts from 1")
     b1, b2 = float(betas[0]), float(betas[1])
     if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and eps >= 0.0):
         raise ValueError(f"{who}: betas in [0, 1) and eps >= 0, got {betas}, {eps}")
     dev = params[0].get_device()
-    if dev < 0 or not params[0].is_cuda or any(set(map(_DEVICE, ts)) != {dev} for ts in lists):
-        raise ValueError(f"{who}: all tensors live on one GPU, got {sorted({str(t.device) for ts in lists for t in ts})}")
-    for name, ts in zip(("param", "grad", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale"), lists):
-        e[name] = np.fromiter(map(_POINTER, ts), np.uint64, n)
-    p_bytes = numel * (4 if p_types.count(torch.float32) == n else np.array([t.itemsize for t in p_types], dtype=np.int64))
-    state = [("exp_avg", 4 * numel if bits == 32 else numel), ("exp_avg_sq", 4 * numel if bits == 32 else numel)]
-    state += [("exp_avg_scale", 4 * blocks), ("exp_avg_sq_scale", 4 * blocks)] if bits == 8 else []
-    used = numel > 0
-    g_bytes = numel * (4 if g_types.count(torch.float32) == n else np.array([t.itemsize for t in g_types], dtype=np.int64))
-    ranges = [("grad", g_bytes), ("param", p_bytes)] + state
-    ptrs, size = np.concatenate([e[k][used] for k, _ in ranges]), np.concatenate([v[used] for _, v in ranges])
-    if _overlap(ptrs, size, np.arange(len(ptrs)) >= int(used.sum())):
+    if dev < 0 or not params[0].is_cuda or set(map(_DEVICE, flat)) != {dev}:
+        raise ValueError(f"{who}: all tensors live on one GPU, got {sorted({str(t.device) for t in flat})}")
+    ptrs = np.fromiter(map(_POINTER, flat), np.uint64, len(flat)).reshape(-1, n)
+    for name, row in zip(("param", "grad", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale"), ptrs):
+        e[name] = row
+    sizes = numels.copy()                                                                # bytes
+    sizes[0] *= 4 if p_kinds == {torch.float32} else np.array([t.itemsize for t in p_types])
+    sizes[1] *= 4 if g_kinds == {torch.float32} else np.array([t.itemsize for t in g_types])
+    sizes[2:] *= 4
+    if bits == 8:
+        sizes[2:4] = numel
+    written = np.ones(ptrs.shape, dtype=bool)
+    written[1] = False
+    some = (numels > 0).ravel()
+    if _overlap(ptrs.ravel()[some], sizes.ravel()[some], written.ravel()[some]):
         raise ValueError(f"{who}: a tensor that is written shares memory with another (the same one twice?)")
     with _lib.on_device(dev):
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError(f"{who}: not inside a graph capture: the step number is an argument and would be frozen")
         _lib.init_device(dev)
-        of = list(zip(p_types, g_types)) if len(kinds) > 1 else None
-        for kind in kinds if of is None else dict.fromkeys(of):
-            part = e if of is None else np.ascontiguousarray(e[[k == kind for k in of]])
+        of = list(zip(p_types, g_types)) if len(p_kinds) + len(g_kinds) > 2 else None
+        for kind in dict.fromkeys(of) if of else [(p_types[0], g_types[0])]:
+            part = np.ascontiguousarray(e[[k == kind for k in of]]) if of else e
             _lib.check(_lib.lib().ddmi_train_adamw_multi(part.ctypes.data, len(part), b1, b2, float(eps), float(grad_scale), int(seed) & 0xFFFFFFFF,
                                                          _TYPES[kind[0]], _TYPES[kind[1]], bits, _lib.raw_stream(dev)))
 

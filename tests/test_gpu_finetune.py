@@ -541,6 +541,21 @@ def test_losses_of_more_than_2_to_31_values(op):
     assert torch.allclose(got["d_logit"], alone["d_logit"], rtol=1e-4, atol=1e-4 * float(alone["d_logit"].abs().max()))
 
 
+def test_adamw_of_mixed_types_in_one_list():
+    """fp32 and bf16 parameters and gradients side by side: each is what it is in a list of its own kind at the same place."""
+    kinds = [(torch.float32, torch.float32), (torch.bfloat16, torch.float32), (torch.float32, torch.bfloat16), (torch.bfloat16, torch.bfloat16)]
+    shapes = [(300,), (1000,), (77,), (513,)]
+    for bits in (32, 8):
+        made = [lists(shapes, p, g, bits, 5) for p, g in kinds]
+        pick = [[made[i][j][i] for i in range(4)] for j in range(4)]
+        scales = {k: [made[i][4][k][i].clone() for i in range(4)] for k in made[0][4]}
+        p, g, m, v = [[t.clone() for t in ts] for ts in pick]
+        adamw_step(p, g, m, v, 2, lr=1e-3, seed=7, **scales)
+        for i, (a, b, c, d, sc) in enumerate(made):
+            adamw_step(a, b, c, d, 2, lr=1e-3, seed=7, **sc)
+            assert torch.equal(a[i], p[i]) and torch.equal(bits_of(c[i]), bits_of(m[i])) and torch.equal(bits_of(d[i]), bits_of(v[i])), (bits, i)
+
+
 def test_adamw_skips_empty_tensors_and_steps_nothing_else():
     z = lambda *s: torch.zeros(s, device=DEV)      # noqa: E731
     a = AdamW([z(0), torch.ones(3, device=DEV), z(4, 0)], lr=0.1, state_bits=8)
