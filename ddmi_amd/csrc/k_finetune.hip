@@ -374,7 +374,8 @@ template <typename T> __device__ __forceinline__ void store_some(T* p, int left,
 }
 
 // NV vectors of four values a thread; a row's vectors lie on its G lanes in turn, `turns` to a lane.  Sixteen vectors of residuals (two
-// times eight with KL) leave room for four workgroups a compute unit, so that three load while one waits.  256 pairs of 64 x 64 x 64: 453 us
+// times eight with KL) leave room for four workgroups a compute unit, so that three load while one waits (256 pairs as a graph, 8 | 12 | 16 |
+// 20 | 24 vectors: 488 | 506 | 470 | 501 | 509 us; 512 transitions: 605 | 633 | 519 | 520 | 529).  256 pairs of 64 x 64 x 64: 453 us
 // for the 2.42 GB that any form has to move, 5.3 TB/s; 512 transitions with KL: 492 us, 5.5 TB/s.  What is left is the wait for the last of
 // a sample's spans; loading a vector ahead of its use costs more registers than it gains (2 % slower).
 template <int MODE, bool MIX, bool REF, typename T, int NV>

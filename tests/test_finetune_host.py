@@ -168,6 +168,26 @@ def test_c_entries_refuse():
     assert adam() == 1
 
 
+def test_struct_layouts_match_the_header(tmp_path):
+    import os
+    import shutil
+    import subprocess
+    from ddmi_amd import optim
+    fields = lambda name, names: "".join(f'_Static_assert(offsetof({name}, {f}) == {o}, "{f}");\n' for f, o in names)      # noqa: E731
+    text = '#include "ddmi_hip.h"\n' + f"_Static_assert(sizeof(ddmi_loss_in) == {C.sizeof(_lib.LossIn)}, \"\");\n" + \
+        f"_Static_assert(sizeof(ddmi_adamw_tensor) == {optim._ENTRY.itemsize}, \"\");\n" + \
+        fields("ddmi_loss_in", [(n, getattr(_lib.LossIn, n).offset) for n, _ in _lib.LossIn._fields_]) + \
+        fields("ddmi_adamw_tensor", [(n, optim._ENTRY.fields[n][1]) for n in optim._ENTRY.names])
+    gcc = shutil.which("gcc")
+    if gcc is None:
+        pytest.skip("no gcc")
+    src = tmp_path / "h.c"
+    src.write_text(text)
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([gcc, "-std=c11", "-fsyntax-only", "-I", os.path.join(root, "include"), str(src)], capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
+
+
 @pytest.mark.parametrize("n", [1, 255, 256, 257, 1000])
 @pytest.mark.parametrize("root", [False, True])
 def test_moments_round_trip(n, root):

@@ -165,6 +165,25 @@ def test_rollout_and_policy_step(numerics, steps):
     assert torch.isfinite(out.loss) and out.kl[1:].all() and torch.isfinite(tr.flat.data).all() and tr.opt_step == 3
 
 
+def test_video_latents_fine_tune_too():
+    """The tri-plane network on [B, C, L] latents with a mixing logit [1, C, 1]: preference step, rollout, policy step."""
+    unet = dict(size1=8, size2=8, size3=4, in_channels=64, model_channels=32, out_channels=64, attention_resolutions=[2], num_res_blocks=1,
+                channel_mult=[1, 2], num_head_channels=32)
+    tr = LDMTrainStep(unet, dict(timesteps=10, channels=64, domain="video"), numerics="fp32", lr=1e-4, device=DEV)
+    st = {"model." + k: v for k, v in named_state("ft.unet3", [(k, tuple(p.shape)) for k, p in tr.model.state_dict().items()]).items()}
+    tr.load_state_dict(st, strict=False).finalize().set_reference()
+    L = 8 * 8 + 2 * 8 * 4
+    g = torch.Generator(DEV).manual_seed(1)
+    zw, zl = (torch.randn((2, 64, L), device=DEV, generator=g) for _ in range(2))
+    out = tr.preference_step(zw, zl, beta=100.0, t=torch.tensor([3, 7]))
+    assert float(out.loss) == pytest.approx(math.log(2.0), rel=2 * R.U) and tr.opt_step == 1
+    r = tr.rollout(2, generator=g)
+    assert r.x_0.shape == (2, 64, L) and r.logp.shape == (10, 2) and r.logp[:-1].all()
+    k, b = torch.tensor([2, 5], device=DEV), torch.arange(2, device=DEV)
+    out = tr.policy_step(r.x_t[k, b], r.x_prev[k, b], r.t[k], r.transition[k], r.logp[k, b], torch.tensor([1.0, -1.0]), clip_range=0.1, kl_coef=0.1)
+    assert ((out.ratio - 1).abs() <= 4 * R.U * (1 + r.logp[k, b].abs())).all() and out.kl.all() and torch.isfinite(tr.flat.data).all()
+
+
 def test_main_fine_tunes_from_preferences(golden, tmp_path):
     """`main.py` with lossconfig.objective preference: pairs of latents from a file, 8-bit moments, a checkpoint that resumes."""
     import yaml
