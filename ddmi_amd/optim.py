@@ -158,7 +158,8 @@ def decode_moment(codes: torch.Tensor, scales: torch.Tensor, root: bool) -> torc
 
 class AdamW:
     """The optimizer over parameters or parameter groups ({"params": [...], "lr": ..., "weight_decay": ...}), as torch.optim.AdamW is made;
-    a parameter whose `.grad` is None sits the step out, its step count too.  state_bits: 32 or 8.  The moments of all parameters lie in one
+    a parameter whose `.grad` is None sits the step out, its step count too.  `param_groups[i]["lr"]` and `["weight_decay"]` are read at every
+    step.  state_bits: 32 or 8.  The moments of all parameters lie in one
     slab each, a parameter's from a multiple of 256 values on."""
 
     def __init__(self, params, lr: float = 1e-4, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.0, state_bits: int = 32, seed: int = 0):
@@ -167,8 +168,6 @@ class AdamW:
         params = list(params)
         groups = params if params and isinstance(params[0], dict) else [{"params": params}]
         self.params: List[torch.Tensor] = []
-        self.lr: List[float] = []
-        self.weight_decay: List[float] = []
         self.param_groups: List[Dict] = []
         for g in groups:
             ps = list(g["params"])
@@ -177,8 +176,6 @@ class AdamW:
                 raise ValueError(f"AdamW: a parameter group sets lr and weight_decay, got {sorted(unknown)}")
             first = len(self.params)
             self.params += ps
-            self.lr += [float(g.get("lr", lr))] * len(ps)
-            self.weight_decay += [float(g.get("weight_decay", weight_decay))] * len(ps)
             self.param_groups.append({"lr": float(g.get("lr", lr)), "weight_decay": float(g.get("weight_decay", weight_decay)),
                                       "params": list(range(first, len(self.params)))})
         if not self.params:
@@ -209,9 +206,10 @@ class AdamW:
         at = [i for i, p in enumerate(self.params) if p.grad is not None]
         take = (lambda v: v) if len(at) == len(self.params) else (lambda v: [v[i] for i in at])
         steps = [s + 1 for s in take(self.steps)]
+        lr, weight_decay = (take([float(g[k]) for g in self.param_groups for _ in g["params"]]) for k in ("lr", "weight_decay"))
         with torch.no_grad():
             adamw_step(take(self.params), [self.params[i].grad for i in at], take(self.exp_avg), take(self.exp_avg_sq), steps,
-                       lr=take(self.lr), betas=self.betas, eps=self.eps, weight_decay=take(self.weight_decay), grad_scale=grad_scale,
+                       lr=lr, betas=self.betas, eps=self.eps, weight_decay=weight_decay, grad_scale=grad_scale,
                        exp_avg_scales=None if self.state_bits == 32 else take(self.exp_avg_scale),
                        exp_avg_sq_scales=None if self.state_bits == 32 else take(self.exp_avg_sq_scale), seed=self.seed)
         for i, s in zip(at, steps):      # only a step that was taken counts
@@ -265,8 +263,6 @@ class AdamW:
             raise ValueError("AdamW: the state dict has other parameter groups")
         for g, mine in zip(groups, self.param_groups):
             mine["lr"], mine["weight_decay"] = float(g["lr"]), float(g["weight_decay"])
-            for i in mine["params"]:
-                self.lr[i], self.weight_decay[i] = mine["lr"], mine["weight_decay"]
         self.betas, self.eps = tuple(float(b) for b in groups[0]["betas"]), float(groups[0]["eps"])
         extra = [i for i in sd["state"] if not (isinstance(i, int) and 0 <= i < len(self.params))]
         if extra:

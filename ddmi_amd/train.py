@@ -1228,7 +1228,7 @@ class LDMTrainStep:
         f = self.flat
         if self.opt8 is not None:
             o = self.opt8
-            o.lr, o.weight_decay = [self.lr] * len(o.params), [self.wd] * len(o.params)
+            o.param_groups[0].update(lr=self.lr, weight_decay=self.wd)
             o.betas, o.eps, o.steps = tuple(self.betas), self.eps, [self.opt_step - 1] * len(o.params)
             o.step(grad_scale)
             return

@@ -446,6 +446,9 @@ def test_adamw_class_steps_groups_and_checkpoints(bits):
                            for v in groups(ps)], lr=1e-3, weight_decay=0.0)
     tp = [p for gr in t.param_groups for p in gr["params"]]
     for k in range(4):
+        if k == 3:                                # a schedule
+            for opt in (a, b, t):
+                opt.param_groups[0]["lr"] = 5e-4
         for p, q in zip(ps, tp):
             grad = torch.randn(p.shape, generator=g).to(DEV)
             p.grad, q.grad = grad, grad.clone()
