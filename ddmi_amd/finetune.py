@@ -11,7 +11,8 @@ forward and backward.  `train.LDMTrainStep.preference_step` / `.policy_step` are
 Tensors live on one GPU, samples along the first axis, channels along the second, anything behind them ([B, C, H, W] latents, [B, C, L]
 clips).  model_out and ref_out are both fp32 or both bf16, everything else is fp32; strides are free (a strided tensor is copied).  The
 calls enqueue work on the tensors' device's current stream and nothing else: no synchronisation, and a forward + backward can be captured
-in a hipGraph (the workspace is a torch tensor of the call, so graphs share none).
+in a hipGraph (the workspace is a torch tensor of the call, so graphs share none) - while no eager loss of the same leaves that was built on
+the default stream lives: that one is refused.
 """
 from __future__ import annotations
 
@@ -154,6 +155,25 @@ class LossFn(torch.autograd.Function):
     _with_graph = staticmethod(once_differentiable(_gradients.__func__))      # create_graph: a second derivative through here raises
 
 
+# A leaf's gradient is added on the stream that was current when the first graph on that leaf was built, as long as such a graph lives.  If that
+# is the default stream, a captured backward of the leaf would draw it into the capture, which ends the process: the leaf's node is marked,
+# and a capture that finds the mark is refused before anything is recorded.  The mark goes when the graph does.
+_ON_DEFAULT_STREAM = "ddmi: built on the default stream"
+
+
+def _mark_leaves(loss, *inputs):
+    for t, (node, _) in zip(inputs, loss.grad_fn.next_functions):
+        if node is not None and t.is_leaf:
+            node.metadata[_ON_DEFAULT_STREAM] = True
+
+
+def _check_leaves(*inputs):
+    if any(_ON_DEFAULT_STREAM in torch.autograd.graph.get_gradient_edge(t).node.metadata
+           for t in inputs if t is not None and t.requires_grad and t.is_leaf):
+        raise RuntimeError("fine-tuning loss: captured while the graph of an eager loss of the same tensors, built on the default stream, lives: drop "
+                           "that loss first, or run it on a side stream")
+
+
 def _loss(entry, model_out, mixing_logit, others, extra, args, stats):
     """(loss, *statistics), the loss differentiable in model_out and mixing_logit where they ask for it."""
     ref_out, x_t, second, sqrt_1mac, ref_mixing_logit, weight = others
@@ -162,8 +182,14 @@ def _loss(entry, model_out, mixing_logit, others, extra, args, stats):
     mixed = mixing_logit is not None and mixing_logit.requires_grad
     if not (torch.is_grad_enabled() and (model_out.requires_grad or mixed)):
         return _launch(entry, tensors, extra, args, stats, None, False, False)[0]
+    stream = _lib.raw_stream(model_out.get_device())
+    if stream and torch.cuda.is_current_stream_capturing():
+        _check_leaves(model_out, mixing_logit)
     results, grads = _launch(entry, tensors, extra, args, stats, None, True, mixed)
-    return [LossFn.apply(model_out, mixing_logit, results[:1], grads, (entry, tensors, extra, args, stats, mixed))] + results[1:]
+    loss = LossFn.apply(model_out, mixing_logit, results[:1], grads, (entry, tensors, extra, args, stats, mixed))
+    if not stream:
+        _mark_leaves(loss, model_out, mixing_logit)
+    return [loss] + results[1:]
 
 
 def preference_loss(model_out, ref_out, x_t, noise, sqrt_1mac, beta, mixing_logit=None, ref_mixing_logit=None, weight=None,

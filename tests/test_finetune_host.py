@@ -1,5 +1,6 @@
 """The fine-tuning operators without a GPU: what they refuse, the 8-bit moments' format, transition coefficients."""
 import ctypes as C
+import gc
 import math
 
 import numpy as np
@@ -7,7 +8,7 @@ import pytest
 import torch
 
 import finetune_ref as R
-from ddmi_amd import _lib
+from ddmi_amd import _lib, finetune
 from ddmi_amd.ddpm import DDPM, ddim_time_pairs
 from ddmi_amd.finetune import policy_loss, preference_loss, transition_log_prob
 from ddmi_amd.optim import AdamW, adamw_step, blocks_of, decode_moment, encode_moment
@@ -227,3 +228,18 @@ def test_transition_coefs_give_the_samplers_mean():
         assert abs(A * x + E * eps - mean) <= 1e-6 * (abs(x0) + abs(x)) and math.isclose(s, 0.0 if t_next < 0 else k.sigma)
     with pytest.raises(ValueError, match="clip"):
         DDPM(model=None, timesteps=40, sampling_timesteps=40, clip_denoised=True, channels=2).transition_coefs(3)
+
+
+def test_leaves_are_marked_as_long_as_their_graph_lives():
+    a, b = torch.zeros(3, requires_grad=True), torch.zeros(3, requires_grad=True)
+    inner = a * 2
+    loss = torch.mul(inner, b)                       # a graph node with an inner and a leaf input, as a loss has them
+    finetune._check_leaves(a, b)
+    finetune._mark_leaves(loss, inner, b)
+    finetune._check_leaves(a, None)
+    finetune._check_leaves(inner, None)
+    with pytest.raises(RuntimeError, match="captured while"):
+        finetune._check_leaves(inner, b)
+    del loss
+    gc.collect()
+    finetune._check_leaves(inner, b)

@@ -1,4 +1,5 @@
 """The fine-tuning losses and AdamW over many tensors on the GPU, against 64-bit formulas with derived bounds (finetune_ref)."""
+import gc
 import math
 
 import pytest
@@ -260,6 +261,31 @@ def test_captured_and_replayed(op, B, C, T):
         for j in (0, 1):
             for k in want[0]:
                 assert torch.equal(graphs[j][1][k], want[(i + j) % 4][k]), (i, j, k)
+
+
+def test_capture_refused_while_an_eager_loss_of_the_leaves_lives():
+    """An eager loss that was built on the default stream ties its leaves' gradients to that stream; gone, the capture runs."""
+    d = R.make("pref", 6, 7, 131, device=DEV)
+    d["model_out"].requires_grad_()
+    d["mixing_logit"].requires_grad_()
+    leaves = [d["model_out"], d["mixing_logit"]]
+    eager = preference_loss(**d)
+    want = torch.autograd.grad(eager.loss, leaves)
+    refused, graph = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    other = torch.zeros(1, device=DEV)
+    with torch.cuda.graph(refused):
+        with pytest.raises(RuntimeError, match="captured while the graph of an eager loss"):
+            preference_loss(**d)
+        other.add_(1)
+    del eager
+    gc.collect()
+    assert not any(torch.autograd.graph.get_gradient_edge(t).node.metadata for t in leaves)
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(preference_loss(**d).loss, leaves)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(map(torch.equal, got, want))
 
 
 # ---------------------------------------------------------------------------------------------------------------------
