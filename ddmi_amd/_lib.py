@@ -196,6 +196,7 @@ SYMBOLS = {
     "ddmi_train_pref_loss": (_I, [C.POINTER(LossIn), _I, _I, C.c_double, C.c_double, _VP, _VP, C.c_size_t] + [_VP] * 6),
     "ddmi_train_policy_loss": (_I, [C.POINTER(LossIn), _I, _VP, _VP, _VP, C.c_double, C.c_double, _VP, _VP, C.c_size_t] + [_VP] * 7),
     "ddmi_train_loss_scale": (_I, [_VP, _VP, _I, C.c_int64, _VP, _I, _VP]),
+    "ddmi_stream_capture_id": (_I, [_VP, C.POINTER(C.c_uint64)]),
     "ddmi_debug_loss_polls": (_I, [_I]),
     "ddmi_train_adamw_multi": (_I, [_VP, _I, C.c_double, C.c_double, C.c_double, C.c_double, C.c_uint32, _I, _I, _I, _VP]),
 }
@@ -271,6 +272,15 @@ def raw_stream(device_index: int) -> int:
     """The handle of a device's current stream, without making a torch.cuda.Stream of it."""
     import torch
     return torch._C._cuda_getCurrentRawStream(device_index)
+
+
+def capture_id(stream: int) -> int:
+    """Which capture the stream is recorded into; 0: none."""
+    if not stream:      # the default stream is never captured
+        return 0
+    n = C.c_uint64(0)
+    check(lib().ddmi_stream_capture_id(stream, C.byref(n)))
+    return n.value
 
 
 class on_device:

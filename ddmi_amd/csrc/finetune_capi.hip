@@ -75,6 +75,16 @@ int ddmi_train_loss_scale(const float* dloss, void* d_model_out, int out_dtype, 
   DDMI_REQUIRE(dloss && d_model_out && n > 0 && dtype_ok(out_dtype) && (!d_logit || C > 0), "loss_scale: bad arguments");
   return launch_ft_scale(dloss, d_model_out, internal_dt(out_dtype), n, d_logit, C, (hipStream_t)stream);
 }
+int ddmi_stream_capture_id(void* stream, uint64_t* id) {
+  DDMI_REQUIRE(id, "stream_capture_id: null argument");
+  *id = 0;
+  if (!stream) return DDMI_OK;      // the default stream is never captured
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  unsigned long long n = 0;
+  HIP_TRY(hipStreamGetCaptureInfo((hipStream_t)stream, &status, &n));
+  if (status == hipStreamCaptureStatusActive) *id = n;
+  return DDMI_OK;
+}
 int ddmi_debug_loss_polls(int n) {
   DDMI_REQUIRE(n >= 0, "debug_loss_polls: not negative");
   ft_set_polls(n);

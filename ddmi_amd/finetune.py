@@ -125,13 +125,14 @@ def _launch(entry, tensors, extra, args, stats, g, grads, mixed):
 class LossFn(torch.autograd.Function):
     """A loss that is computed already, its gradients for an upstream gradient of 1 along with it.  The first backward hands those out -
     multiplied in place when the upstream gradient, which only the device knows, is another (a bf16 gradient is then rounded a second time) -
-    and a later one (retain_graph) computes them again from the saved inputs."""
+    and a later one (retain_graph) computes them again from the saved inputs, as does one that is captured apart from its forward: each replay
+    of it would multiply once more."""
 
     @staticmethod
-    def forward(ctx, model_out, mixing_logit, loss, grads, again):      # loss, grads in lists: they are no inputs
+    def forward(ctx, model_out, mixing_logit, loss, grads, again, capture):      # loss, grads in lists: they are no inputs
         entry, tensors, extra, *rest = again
         ctx.save_for_backward(*tensors, *extra)
-        ctx.grads, ctx.again, ctx.index = grads, (entry, rest), model_out.get_device()
+        ctx.grads, ctx.again, ctx.index, ctx.capture = grads, (entry, rest), model_out.get_device(), capture
         return loss[0]
 
     @staticmethod
@@ -143,14 +144,14 @@ class LossFn(torch.autograd.Function):
         if not g.is_contiguous():
             g = g.contiguous()
         with _lib.on_device(ctx.index):
-            if ctx.grads is not None:
+            if ctx.grads is not None and _lib.capture_id(_lib.raw_stream(ctx.index)) == ctx.capture:
                 (d_out, d_logit), ctx.grads = ctx.grads, None
                 _lib.check(_lib.lib().ddmi_train_loss_scale(g.data_ptr(), d_out.data_ptr(), _OUT_TYPES[d_out.dtype], d_out.numel(), _p(d_logit),
                                                             0 if d_logit is None else d_logit.numel(), _lib.raw_stream(ctx.index)))
             else:
                 saved, (entry, (args, stats, mixed)) = ctx.saved_tensors, ctx.again
                 d_out, d_logit = _launch(entry, saved[:8], saved[8:], args, stats, g, True, mixed)[1]
-        return d_out, d_logit, None, None, None
+        return d_out, d_logit, None, None, None, None
 
     _with_graph = staticmethod(once_differentiable(_gradients.__func__))      # create_graph: a second derivative through here raises
 
@@ -183,10 +184,11 @@ def _loss(entry, model_out, mixing_logit, others, extra, args, stats):
     if not (torch.is_grad_enabled() and (model_out.requires_grad or mixed)):
         return _launch(entry, tensors, extra, args, stats, None, False, False)[0]
     stream = _lib.raw_stream(model_out.get_device())
-    if stream and torch.cuda.is_current_stream_capturing():
+    capture = _lib.capture_id(stream)
+    if capture:
         _check_leaves(model_out, mixing_logit)
     results, grads = _launch(entry, tensors, extra, args, stats, None, True, mixed)
-    loss = LossFn.apply(model_out, mixing_logit, results[:1], grads, (entry, tensors, extra, args, stats, mixed))
+    loss = LossFn.apply(model_out, mixing_logit, results[:1], grads, (entry, tensors, extra, args, stats, mixed), capture)
     if not stream:
         _mark_leaves(loss, model_out, mixing_logit)
     return [loss] + results[1:]

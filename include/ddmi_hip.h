@@ -541,6 +541,9 @@ int ddmi_train_policy_loss(const ddmi_loss_in* in, int B, const float* transitio
                            void* d_model_out, float* d_logit, void* stream);
 /* gradients of a loss call without dloss, times *dloss in place (n values of out_dtype, C logits; nothing is touched when it is 1) */
 int ddmi_train_loss_scale(const float* dloss, void* d_model_out, int out_dtype, int64_t n, float* d_logit, int C, void* stream);
+/* the capture that `stream` is recorded into, 0 outside of one: gradients of a loss call may be scaled in place only within the capture that
+ * computed them (a second replay would scale them again) */
+int ddmi_stream_capture_id(void* stream, uint64_t* id);
 /* how often a workgroup of a loss's one-pass form looks for its neighbours' sums before it leaves its part to the kernel after it (4096
  * by default; 0: one look - the results are the same bits) */
 int ddmi_debug_loss_polls(int n);

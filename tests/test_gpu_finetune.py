@@ -288,6 +288,52 @@ def test_capture_refused_while_an_eager_loss_of_the_leaves_lives():
         assert all(map(torch.equal, got, want))
 
 
+@pytest.mark.parametrize("op", ["pref", "policy"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_backward_captured_apart_from_its_forward(op, dtype):
+    """Replayed several times with an upstream gradient that is not 1: each replay is the eager backward, nothing is multiplied twice."""
+    d = R.make(op, 6, 7, 131, dtype, device=DEV)
+    leaves = [d["model_out"].requires_grad_(), d["mixing_logit"].requires_grad_()]
+    up = torch.tensor(3.0, device=DEV)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        loss = (preference_loss if op == "pref" else policy_loss)(**d).loss
+        torch.autograd.grad(loss, leaves, up, retain_graph=True)                # handed out; those after it are computed from the inputs
+        want = {v: torch.autograd.grad(loss, leaves, torch.tensor(v, device=DEV), retain_graph=True) for v in (3.0, -0.7)}
+        loss = (preference_loss if op == "pref" else policy_loss)(**d).loss
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        got = torch.autograd.grad(loss, leaves, up, retain_graph=True)
+    for v in (3.0, 3.0, -0.7, -0.7, 3.0):
+        up.fill_(v)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(map(torch.equal, got, want[v])), v
+
+
+def test_graphed_callable():
+    """Forward and backward in two graphs, the backward taken twice."""
+    d = R.make("pref", 6, 7, 131, device=DEV)
+    leaves = [d.pop("model_out").requires_grad_(), d.pop("mixing_logit").requires_grad_()]
+
+    def loss_of(model_out, mixing_logit):
+        return preference_loss(model_out=model_out, mixing_logit=mixing_logit, **d).loss
+
+    graphed = torch.cuda.make_graphed_callables(loss_of, tuple(t.detach().clone().requires_grad_() for t in leaves))
+    for _ in range(2):
+        first = loss_of(*leaves)
+        torch.autograd.grad(3.0 * first, leaves, retain_graph=True)
+        want = torch.autograd.grad(3.0 * first, leaves)
+        loss = 3.0 * graphed(*leaves)
+        assert torch.equal(loss, 3.0 * first)
+        for _ in range(3):
+            got = torch.autograd.grad(loss, leaves, retain_graph=True)
+            torch.cuda.synchronize()
+            assert all(map(torch.equal, got, want))
+        del first
+
+
 # ---------------------------------------------------------------------------------------------------------------------
 # AdamW
 # ---------------------------------------------------------------------------------------------------------------------
