@@ -127,6 +127,7 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
             part = np.ascontiguousarray(e[[k == kind for k in of]]) if of else e
             _lib.check(_lib.lib().ddmi_train_adamw_multi(part.ctypes.data, len(part), b1, b2, float(eps), float(grad_scale), int(seed) & 0xFFFFFFFF,
                                                          _TYPES[kind[0]], _TYPES[kind[1]], bits, _lib.raw_stream(dev)))
+    torch.autograd.graph.increment_version(params)      # a backward through a graph that saved the old values raises, as after torch's own step
 
 
 def encode_moment(x: torch.Tensor, root: bool):

@@ -638,3 +638,17 @@ def test_adamw_skips_empty_tensors_and_steps_nothing_else():
         p.grad = torch.ones_like(p)
     a.step()
     assert a.steps == [1, 1, 1] and (a.params[1] < 1).all()
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_adamw_step_counts_as_a_change_of_the_parameters(bits):
+    """A graph that saved the values before the step refuses its backward."""
+    p = torch.nn.Parameter(torch.ones(300, device=DEV))
+    opt = AdamW([p], lr=0.1, state_bits=bits)
+    loss, before = (p * p).sum(), p._version
+    p.grad = torch.ones_like(p)
+    opt.step()
+    assert p._version > before
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    (p * p).sum().backward()
