@@ -131,7 +131,9 @@ class LossFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, model_out, mixing_logit, loss, grads, again, capture):      # loss, grads in lists: they are no inputs
         entry, tensors, extra, *rest = again
-        ctx.save_for_backward(*tensors, *extra)
+        saved = tensors + extra
+        ctx.beside = {i: t for i, t in enumerate(saved) if t is not None and t.is_inference()}      # autograd does not save these itself
+        ctx.save_for_backward(*(saved if not ctx.beside else [None if i in ctx.beside else t for i, t in enumerate(saved)]))
         ctx.grads, ctx.again, ctx.index, ctx.capture = grads, (entry, rest), model_out.get_device(), capture
         return loss[0]
 
@@ -150,6 +152,7 @@ class LossFn(torch.autograd.Function):
                                                             0 if d_logit is None else d_logit.numel(), _lib.raw_stream(ctx.index)))
             else:
                 saved, (entry, (args, stats, mixed)) = ctx.saved_tensors, ctx.again
+                saved = [ctx.beside.get(i, t) for i, t in enumerate(saved)]
                 d_out, d_logit = _launch(entry, saved[:8], saved[8:], args, stats, g, True, mixed)[1]
         return d_out, d_logit, None, None, None, None
 

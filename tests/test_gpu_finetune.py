@@ -312,6 +312,20 @@ def test_backward_captured_apart_from_its_forward(op, dtype):
         assert all(map(torch.equal, got, want[v])), v
 
 
+@pytest.mark.parametrize("op", ["pref", "policy"])
+def test_reference_output_made_in_inference_mode(op):
+    d = R.make(op, 6, 7, 131, device=DEV)
+    leaves = [d["model_out"].requires_grad_(), d["mixing_logit"].requires_grad_()]
+    loss_of = preference_loss if op == "pref" else policy_loss
+    want = loss_of(**d).loss
+    with torch.inference_mode():
+        d = {k: t.clone() if k in ("ref_out", "x_t") else t for k, t in d.items()}
+    loss = loss_of(**d).loss
+    assert d["ref_out"].is_inference() and torch.equal(loss, want)
+    for _ in range(2):      # handed out, computed again
+        assert all(map(torch.equal, torch.autograd.grad(loss, leaves, retain_graph=True), torch.autograd.grad(want, leaves, retain_graph=True)))
+
+
 def test_graphed_callable():
     """Forward and backward in two graphs, the backward taken twice."""
     d = R.make("pref", 6, 7, 131, device=DEV)
