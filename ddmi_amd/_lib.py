@@ -283,6 +283,14 @@ def capture_id(stream: int) -> int:
     return n.value
 
 
+def refuse_tangents(who: str, *tensors) -> None:
+    """Raises where a tensor carries a forward-mode derivative: the kernels go by its pointer, which would drop the tangent in silence (a
+    dual tensor does not require a gradient)."""
+    from torch.autograd import forward_ad
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{who}: forward-mode derivatives are not offered")
+
+
 class on_device:
     """`with torch.cuda.device(index)`, entered only where it is not the current device already (the common case costs a comparison)."""
     __slots__ = ("guard",)

@@ -9,8 +9,10 @@ the output and to `mixing_logit`; every value is computed in libddmi_hip (includ
 forward and backward.  `train.LDMTrainStep.preference_step` / `.policy_step` are the training steps made of them.
 
 Tensors live on one GPU, samples along the first axis, channels along the second, anything behind them ([B, C, H, W] latents, [B, C, L]
-clips).  model_out and ref_out are both fp32 or both bf16, everything else is fp32; strides are free (a strided tensor is copied).  The
-calls enqueue work on the tensors' device's current stream and nothing else: no synchronisation, and a forward + backward can be captured
+clips).  model_out and ref_out are both fp32 or both bf16, everything else is fp32; strides are free (a strided tensor is copied).
+Gradients are those of first order in reverse mode: a second order, or a forward-mode tangent, raises.
+
+The calls enqueue work on the tensors' device's current stream and nothing else: no synchronisation, and a forward + backward can be captured
 in a hipGraph (the workspace is a torch tensor of the call, so graphs share none) - while no eager loss of the same leaves that was built on
 the default stream lives: that one is refused.
 """
@@ -224,6 +226,7 @@ def preference_loss(model_out, ref_out, x_t, noise, sqrt_1mac, beta, mixing_logi
     if beta != beta or not 0.0 <= label_smoothing <= 1.0:
         raise ValueError(f"{who}: beta is a number and label_smoothing in [0, 1], got {beta}, {label_smoothing}")
     _check_constants(who, ref_out=ref_out, x_t=x_t, noise=noise, sqrt_1mac=sqrt_1mac, ref_mixing_logit=ref_mixing_logit, weight=weight)
+    _lib.refuse_tangents(who, model_out, ref_out, x_t, noise, sqrt_1mac, mixing_logit, ref_mixing_logit, weight)
     dev = _check_device(who, model_out, ref_out, x_t, noise, sqrt_1mac, mixing_logit, ref_mixing_logit, weight)
     with _lib.on_device(dev):
         _lib.init_device(dev)
@@ -261,6 +264,7 @@ def policy_loss(model_out, x_t, x_prev, transition, sqrt_1mac, logp_old, advanta
         raise ValueError(f"{who}: kl_coef without ref_out, the reference network's output")
     _check_constants(who, ref_out=ref_out, x_t=x_t, x_prev=x_prev, transition=transition, sqrt_1mac=sqrt_1mac, logp_old=logp_old, advantage=advantage,
                      ref_mixing_logit=ref_mixing_logit, weight=weight)
+    _lib.refuse_tangents(who, model_out, ref_out, x_t, x_prev, transition, sqrt_1mac, logp_old, advantage, mixing_logit, ref_mixing_logit, weight)
     dev = _check_device(who, model_out, ref_out, x_t, x_prev, transition, sqrt_1mac, logp_old, advantage, mixing_logit, ref_mixing_logit, weight)
     with _lib.on_device(dev):
         _lib.init_device(dev)
@@ -275,6 +279,7 @@ def transition_log_prob(model_out, x_t, x_prev, transition, sqrt_1mac, mixing_lo
     who = "transition_log_prob"
     _check_outputs(who, model_out, None, x_t, sqrt_1mac, mixing_logit, None)
     _check_transition(who, model_out, x_prev, transition, weight)
+    _lib.refuse_tangents(who, model_out, x_t, x_prev, transition, sqrt_1mac, mixing_logit, weight)
     dev = _check_device(who, model_out, x_t, x_prev, transition, sqrt_1mac, mixing_logit, weight)
     with _lib.on_device(dev):
         _lib.init_device(dev)
