@@ -75,8 +75,8 @@ __device__ __forceinline__ Span span_of(const FtArgs& a, int blk) {
 template <int MODE>
 __device__ __forceinline__ bool takes_part(const FtArgs& a, int b) {
   if (a.weight && !(a.weight[MODE == FT_PREF ? b % a.pairs : b] > 0.f)) return false;
-  // a transition without noise has no density
-  if (MODE == FT_POLICY && !(a.transition[3 * (int64_t)b + 2] > 0.f)) return false;
+  // a transition without noise has no density; a deviation that is none (negative, NaN) takes part and shows as NaN: its logarithm is one
+  if (MODE == FT_POLICY && a.transition[3 * (int64_t)b + 2] == 0.f) return false;
   return true;
 }
 // c and c - c_ref of the span's rows; the difference is taken in fp64, it may be far below c

@@ -253,7 +253,7 @@ def policy_loss(model_out, x_t, x_prev, transition, sqrt_1mac, logp_old, advanta
         loss  = the weighted mean of max(-advantage ratio, -advantage clip(ratio, 1 - clip_range, 1 + clip_range)) + kl_coef kl
 
     logp_old [B] is what `transition_log_prob` gave when the transition was sampled.  A transition with s = 0 (a chain's last step) has no
-    density and is left out, as is one whose weight [B] is not > 0.  Differentiable in model_out and mixing_logit."""
+    density and is left out, as is one whose weight [B] is not > 0; a negative or NaN deviation shows as NaN.  Differentiable in model_out and mixing_logit."""
     who = "policy_loss"
     _check_outputs(who, model_out, ref_out, x_t, sqrt_1mac, mixing_logit, ref_mixing_logit)
     _check_transition(who, model_out, x_prev, transition, weight, logp_old=logp_old, advantage=advantage)

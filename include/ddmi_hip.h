@@ -534,7 +534,7 @@ int ddmi_train_pref_loss(const ddmi_loss_in* in, int pairs, int noise_rows, doub
 /* Clipped policy loss over B denoising transitions x_t -> second: mean mu = A x_t + E eps and deviation s with transition[b] = (A, E, s);
  * logp = mean over the values of log N(second; mu, s^2), ratio = exp(logp - logp_old), kl = mean((mu - mu_ref)^2) / (2 s^2), loss =
  * weighted mean of max(-advantage ratio, -advantage clip(ratio, 1 -+ clip_range)) + kl_coef kl.  A transition with s = 0 has no density
- * and is left out like one of weight 0.  logp_old = NULL: logp alone is computed (a rollout records it), the other outputs are not
+ * and is left out like one of weight 0; a negative or NaN deviation shows as NaN in logp and loss.  logp_old = NULL: logp alone is computed (a rollout records it), the other outputs are not
  * touched.  logp, ratio, kl [B]; 0 for transitions left out. */
 int ddmi_train_policy_loss(const ddmi_loss_in* in, int B, const float* transition, const float* logp_old, const float* advantage, double clip_range,
                            double kl_coef, const float* dloss, void* ws, size_t ws_bytes, float* loss, float* logp, float* ratio, float* kl,
