@@ -6,7 +6,7 @@ import torch
 
 import finetune_ref as R
 from ddmi_amd.finetune import transition_log_prob
-from test_gpu_finetune import DEV, call
+from test_gpu_finetune import DEV, SHAPES, call, reference
 
 pytestmark = pytest.mark.gpu
 # two passes; one pass
@@ -29,3 +29,51 @@ def test_a_deviation_that_is_none_shows(s, B, C, T):
     d["weight"] = other.float()                       # left out by its weight, it does not show
     got = call("policy", d)
     assert torch.isfinite(got["loss"]) and not got["d_model_out"][2].any() and float(got["logp"][2]) == 0.0
+
+
+# ---- sums in 64 bits: the bounds without what sums in 32 would add -------------------------------------------------------------------
+D = 2.0 ** -53
+
+
+def sum_64(t, e):
+    """A sum of n terms in 64 bits, in whatever order: n - 1 additions, each off by half a step of a partial sum (and the products' own)."""
+    return t.sum((1, 2)), (e + (t[0].numel() + 64) * D * t.abs()).sum((1, 2))
+
+
+def gradients_64(general):
+    """The logit's gradient as a 64-bit sum over batch and values of the terms' errors alone; the rest as it was."""
+    def gradients(out, d, row, c, part, e_part, res, e_res, k, e_k, far=None, e_far=None, q=None, e_q=None):
+        done = general(out, d, row, c, part, e_part, res, e_res, k, e_k, far, e_far, q, e_q)
+        if c is None:
+            return done
+        chan, bound = 0.0, 0.0
+        for f, e_f, r, e_r in ((k, e_k, res, e_res), (q, e_q, far, e_far)):
+            if f is None:
+                continue
+            s = r * part
+            chan = chan + (row(f) * s).sum((0, 2))
+            each = e_r * part.abs() + r.abs() * e_part + e_r * e_part + (len(s) * s.shape[2] + 64) * D * s.abs()
+            bound = bound + (row(e_f) * (s.abs() + each) + row(f.abs()) * each).sum((0, 2))
+        slope = (c * (1 - c)).reshape(-1)
+        want = chan * slope
+        done["d_logit"] = (want, bound * slope + 1.01 * R.U * (want.abs() + bound * slope) + 2.0 ** -149)
+        return done
+    return gradients
+
+
+@pytest.mark.parametrize("B,C,T", SHAPES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("op,kl", [("pref", True), ("policy", True), ("policy", False)])
+def test_sums_are_held_in_64_bits(op, kl, B, C, T, dtype, monkeypatch):
+    monkeypatch.setattr(R, "_gradients", gradients_64(R._gradients))
+    monkeypatch.setattr(R, "_sum", sum_64)
+    d = R.make(op, B, C, T, dtype, kl=kl, seed=B + C + T + 1, device=DEV)
+    R.check(call(op, d), reference(op, d), (B, C, T))
+
+
+def test_gradients_of_many_small_transitions():
+    """100 000 transitions of three values, weights among them, and a clip too wide to have a border nearby: every output."""
+    d = R.make("policy", 100000, 3, 1, seed=12, device=DEV)
+    d["weight"] = (torch.arange(100000, device=DEV) % 7).float()
+    d["clip_range"] = 1e9
+    R.check(call("policy", d), reference("policy", d))
