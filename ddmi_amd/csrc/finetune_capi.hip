@@ -1,6 +1,8 @@
 // C ABI of the fine-tuning operators (include/ddmi_hip.h, "Fine-tuning"): no handle, no state; the caller owns every buffer, the losses'
 // workspace among them (so two captured graphs, or two streams, that use workspaces of their own share nothing).
 #include <algorithm>
+#include <cmath>
+#include <initializer_list>
 #include "finetune.h"
 
 namespace {
@@ -46,7 +48,7 @@ int ddmi_train_pref_loss(const ddmi_loss_in* in, int pairs, int noise_rows, doub
   DDMI_REQUIRE(in && in->ref_out && pairs > 0 && pairs <= (1 << 24), "pref_loss: null argument or no pairs");
   DDMI_REQUIRE(loss && margin && mse, "pref_loss: null output");
   DDMI_REQUIRE(noise_rows == pairs || noise_rows == 2 * pairs, "pref_loss: the noise has a row for each pair or for each sample");
-  DDMI_REQUIRE(label_smoothing >= 0.0 && label_smoothing <= 1.0 && beta == beta, "pref_loss: label_smoothing in [0, 1], beta a number");
+  DDMI_REQUIRE(label_smoothing >= 0.0 && label_smoothing <= 1.0 && std::isfinite(beta), "pref_loss: label_smoothing in [0, 1], beta finite");
   DDMI_REQUIRE(!d_logit || (in->mixing_logit && d_model_out), "pref_loss: d_logit goes with mixing_logit and d_model_out");
   DDMI_TRY(common_args(&a, in, 2 * pairs, 2, d_model_out ? FT_VECS : 0, ws, ws_bytes));
   if (!in->mixing_logit) a.x = nullptr;      // not read
@@ -60,7 +62,7 @@ int ddmi_train_policy_loss(const ddmi_loss_in* in, int B, const float* transitio
   FtArgs a{};
   DDMI_REQUIRE(in && transition && in->x_t && logp, "policy_loss: null argument");
   DDMI_REQUIRE(!logp_old || (advantage && loss && ratio && kl), "policy_loss: null argument");
-  DDMI_REQUIRE(clip_range >= 0.0 && kl_coef == kl_coef, "policy_loss: clip_range >= 0, kl_coef a number");
+  DDMI_REQUIRE(clip_range >= 0.0 && std::isfinite(kl_coef), "policy_loss: clip_range >= 0, kl_coef finite");
   DDMI_REQUIRE(kl_coef == 0.0 || in->ref_out, "policy_loss: a KL term needs the reference's output");
   DDMI_REQUIRE(logp_old || !d_model_out, "policy_loss: a gradient of the log-density alone is not offered");
   DDMI_REQUIRE(!d_logit || (in->mixing_logit && d_model_out), "policy_loss: d_logit goes with mixing_logit and d_model_out");

@@ -20,6 +20,7 @@ from __future__ import annotations
 
 import ctypes as C
 import functools
+import math
 from typing import NamedTuple, Optional
 
 import torch
@@ -223,8 +224,8 @@ def preference_loss(model_out, ref_out, x_t, noise, sqrt_1mac, beta, mixing_logi
     if weight is not None:
         _expect(who, "weight", weight, (pairs,))
     beta, label_smoothing = float(beta), float(label_smoothing)
-    if beta != beta or not 0.0 <= label_smoothing <= 1.0:
-        raise ValueError(f"{who}: beta is a number and label_smoothing in [0, 1], got {beta}, {label_smoothing}")
+    if not math.isfinite(beta) or not 0.0 <= label_smoothing <= 1.0:
+        raise ValueError(f"{who}: beta is finite and label_smoothing in [0, 1], got {beta}, {label_smoothing}")
     _check_constants(who, ref_out=ref_out, x_t=x_t, noise=noise, sqrt_1mac=sqrt_1mac, ref_mixing_logit=ref_mixing_logit, weight=weight)
     _lib.refuse_tangents(who, model_out, ref_out, x_t, noise, sqrt_1mac, mixing_logit, ref_mixing_logit, weight)
     dev = _check_device(who, model_out, ref_out, x_t, noise, sqrt_1mac, mixing_logit, ref_mixing_logit, weight)
@@ -258,8 +259,8 @@ def policy_loss(model_out, x_t, x_prev, transition, sqrt_1mac, logp_old, advanta
     _check_outputs(who, model_out, ref_out, x_t, sqrt_1mac, mixing_logit, ref_mixing_logit)
     _check_transition(who, model_out, x_prev, transition, weight, logp_old=logp_old, advantage=advantage)
     clip_range, kl_coef = float(clip_range), float(kl_coef)
-    if not clip_range >= 0.0 or kl_coef != kl_coef:
-        raise ValueError(f"{who}: clip_range >= 0 and kl_coef a number, got {clip_range}, {kl_coef}")
+    if not clip_range >= 0.0 or not math.isfinite(kl_coef):
+        raise ValueError(f"{who}: clip_range >= 0 and kl_coef finite, got {clip_range}, {kl_coef}")
     if kl_coef != 0.0 and ref_out is None:
         raise ValueError(f"{who}: kl_coef without ref_out, the reference network's output")
     _check_constants(who, ref_out=ref_out, x_t=x_t, x_prev=x_prev, transition=transition, sqrt_1mac=sqrt_1mac, logp_old=logp_old, advantage=advantage,
