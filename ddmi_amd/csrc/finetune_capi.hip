@@ -9,11 +9,21 @@ namespace {
 bool dtype_ok(int dt) { return dt == DDMI_DTYPE_F32 || dt == DDMI_DTYPE_BF16; }
 int internal_dt(int dt) { return dt == DDMI_DTYPE_F32 ? DT_F32 : DT_BF16; }
 
+bool aligned(std::initializer_list<const void*> ps, int bytes) {      // null is
+  for (const void* p : ps)
+    if ((uintptr_t)p & (uintptr_t)(bytes - 1)) return false;
+  return true;
+}
+int size_of(int dt) { return dt == DDMI_DTYPE_F32 ? 4 : 2; }
+
 int common_args(FtArgs* a, const ddmi_loss_in* in, int B, int rows_of, int keep, void* ws, size_t ws_bytes) {
   DDMI_REQUIRE(in->model_out && in->second && B > 0 && in->C > 0 && in->HW > 0, "fine-tuning loss: null argument or empty batch");
   DDMI_REQUIRE(dtype_ok(in->out_dtype), "fine-tuning loss: model_out / ref_out are fp32 or bf16");
   DDMI_REQUIRE((in->mixing_logit == nullptr) == (in->ref_mixing_logit == nullptr) || (in->mixing_logit && !in->ref_out), "fine-tuning loss: both mixing logits or none");
   DDMI_REQUIRE(!in->mixing_logit || (in->x_t && in->sqrt_1mac), "fine-tuning loss: mixing needs x_t and sqrt_1mac");
+  DDMI_REQUIRE(aligned({in->model_out, in->ref_out}, size_of(in->out_dtype)) &&
+                   aligned({in->x_t, in->second, in->sqrt_1mac, in->mixing_logit, in->ref_mixing_logit, in->weight}, 4),
+               "fine-tuning loss: inputs aligned to their values");
   DDMI_REQUIRE((double)in->C * (double)in->HW < 1.1e12, "fine-tuning loss: sample too large");
   DDMI_TRY(ft_plan(a, B, in->C, in->HW, in->mixing_logit != nullptr, rows_of, keep));
   DDMI_REQUIRE(ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= ft_workspace_bytes(*a), "fine-tuning loss: workspace too small or not 16-byte aligned");
@@ -50,6 +60,7 @@ int ddmi_train_pref_loss(const ddmi_loss_in* in, int pairs, int noise_rows, doub
   DDMI_REQUIRE(noise_rows == pairs || noise_rows == 2 * pairs, "pref_loss: the noise has a row for each pair or for each sample");
   DDMI_REQUIRE(label_smoothing >= 0.0 && label_smoothing <= 1.0 && std::isfinite(beta), "pref_loss: label_smoothing in [0, 1], beta finite");
   DDMI_REQUIRE(!d_logit || (in->mixing_logit && d_model_out), "pref_loss: d_logit goes with mixing_logit and d_model_out");
+  DDMI_REQUIRE(aligned({loss, margin, mse, dloss, d_logit}, 4) && aligned({d_model_out}, size_of(in->out_dtype)), "pref_loss: outputs aligned to their values");
   DDMI_TRY(common_args(&a, in, 2 * pairs, 2, d_model_out ? FT_VECS : 0, ws, ws_bytes));
   if (!in->mixing_logit) a.x = nullptr;      // not read
   a.pairs = pairs; a.second_rows = noise_rows; a.beta = beta; a.smoothing = label_smoothing;
@@ -66,6 +77,8 @@ int ddmi_train_policy_loss(const ddmi_loss_in* in, int B, const float* transitio
   DDMI_REQUIRE(kl_coef == 0.0 || in->ref_out, "policy_loss: a KL term needs the reference's output");
   DDMI_REQUIRE(logp_old || !d_model_out, "policy_loss: a gradient of the log-density alone is not offered");
   DDMI_REQUIRE(!d_logit || (in->mixing_logit && d_model_out), "policy_loss: d_logit goes with mixing_logit and d_model_out");
+  DDMI_REQUIRE(aligned({transition, logp_old, advantage, loss, logp, ratio, kl, dloss, d_logit}, 4) && aligned({d_model_out}, size_of(in->out_dtype)),
+               "policy_loss: tensors aligned to their values");
   DDMI_TRY(common_args(&a, in, B, 1, d_model_out ? (in->ref_out ? FT_VECS / 2 : FT_VECS) : 0, ws, ws_bytes));
   a.pairs = B; a.second_rows = B; a.transition = transition;
   a.logp_old = logp_old; a.advantage = advantage; a.clip = clip_range; a.kl_coef = kl_coef;
@@ -75,6 +88,7 @@ int ddmi_train_policy_loss(const ddmi_loss_in* in, int B, const float* transitio
 }
 int ddmi_train_loss_scale(const float* dloss, void* d_model_out, int out_dtype, int64_t n, float* d_logit, int C, void* stream) {
   DDMI_REQUIRE(dloss && d_model_out && n > 0 && dtype_ok(out_dtype) && (!d_logit || C > 0), "loss_scale: bad arguments");
+  DDMI_REQUIRE(aligned({dloss, d_logit}, 4) && aligned({d_model_out}, size_of(out_dtype)), "loss_scale: tensors aligned to their values");
   return launch_ft_scale(dloss, d_model_out, internal_dt(out_dtype), n, d_logit, C, (hipStream_t)stream);
 }
 int ddmi_stream_capture_id(void* stream, uint64_t* id) {
@@ -105,7 +119,8 @@ int ddmi_train_adamw_multi(const ddmi_adamw_tensor* tensors, int n, double beta1
     if (t.numel == 0) continue;
     DDMI_REQUIRE(t.param && t.grad && t.exp_avg && t.exp_avg_sq, "adamw_multi: null tensor");
     DDMI_REQUIRE(state_bits == 32 || (t.exp_avg_scale && t.exp_avg_sq_scale), "adamw_multi: 8-bit moments need their scales");
-    DDMI_REQUIRE(((uintptr_t)t.param & (param_dtype == DDMI_DTYPE_F32 ? 3 : 1)) == 0 && ((uintptr_t)t.grad & (grad_dtype == DDMI_DTYPE_F32 ? 3 : 1)) == 0,
+    DDMI_REQUIRE(aligned({t.param}, size_of(param_dtype)) && aligned({t.grad}, size_of(grad_dtype)) &&
+                     (state_bits == 32 ? aligned({t.exp_avg, t.exp_avg_sq}, 4) : aligned({t.exp_avg_scale, t.exp_avg_sq_scale}, 4)),
                  "adamw_multi: tensors aligned to their values");
   }
   return launch_adamw_multi(tensors, n, beta1, beta2, eps, grad_scale, seed, internal_dt(param_dtype), internal_dt(grad_dtype), state_bits,

@@ -2,6 +2,7 @@
 import ctypes as C
 import math
 
+import numpy as np
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -9,7 +10,7 @@ from torch.autograd import forward_ad
 import finetune_ref as R
 from ddmi_amd import _lib, finetune
 from ddmi_amd.finetune import policy_loss, preference_loss, transition_log_prob
-from ddmi_amd.optim import adamw_step
+from ddmi_amd.optim import _ENTRY, adamw_step
 
 
 # ---- forward-mode derivatives -------------------------------------------------------------------------------------------------------
@@ -88,3 +89,46 @@ class CLoss:
         s = _lib.LossIn(**dict(self.fields, **fields))
         return self.lib.ddmi_train_policy_loss(C.byref(s), 4, transition, old, adv, 0.1, kl_coef, dloss, ws, size, loss, logp, ratio, kl, d_out, d_logit,
                                                None)
+
+
+@pytest.mark.parametrize("out_dtype", [0, 1])
+def test_c_losses_refuse_unaligned_pointers(out_dtype):
+    """A size of zero for the workspace ends a call that gets past the pointers, so that no kernel is launched on made-up ones."""
+    c = CLoss(out_dtype)
+    assert c.pref(size=0) == INVALID and b"workspace" in c.error()
+    assert c.policy(size=0) == INVALID and b"workspace" in c.error()
+    for call, outputs in ((c.pref, ("dloss", "loss", "margin", "mse", "d_logit")),
+                          (c.policy, ("transition", "old", "adv", "dloss", "loss", "logp", "ratio", "kl", "d_logit"))):
+        for name in c.names + outputs + ("d_out",):
+            of_output = name in ("model_out", "ref_out", "d_out")
+            for at in (65,) if of_output and out_dtype == 1 else (65, 66):
+                assert call(**{name: at, "size": 0}) == INVALID and b"aligned to their values" in c.error(), name
+            if of_output and out_dtype == 1:                     # two bytes a value
+                assert call(**{name: 66, "size": 0}) == INVALID and b"workspace" in c.error(), name
+
+
+def test_c_scale_refuses_unaligned_pointers():
+    scale = lambda up=64, out=64, dt=0, logit=64: _lib.lib().ddmi_train_loss_scale(up, out, dt, 4, logit, 3, None)      # noqa: E731
+    for kw in (dict(up=66), dict(out=66), dict(logit=65), dict(out=65, dt=1)):
+        assert scale(**kw) == INVALID and b"aligned" in _lib.lib().ddmi_last_error(), kw
+
+
+def entries(n):
+    e = np.zeros(n, dtype=_ENTRY)
+    for k in ("param", "grad", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale"):
+        e[k] = 64
+    e["numel"], e["step"], e["lr"] = 4, 1, 1e-3
+    return e
+
+
+def adamw_multi(e, bits=32):
+    return _lib.lib().ddmi_train_adamw_multi(e.ctypes.data, len(e), 0.9, 0.999, 1e-8, 1.0, 0, 0, 0, bits, None), _lib.lib().ddmi_last_error()
+
+
+@pytest.mark.parametrize("bits,names", [(32, ("param", "grad", "exp_avg", "exp_avg_sq")), (8, ("param", "grad", "exp_avg_scale", "exp_avg_sq_scale"))])
+def test_c_adamw_refuses_unaligned_pointers(bits, names):
+    for name in names:
+        e = entries(2)
+        e[name][1] = 66
+        rc, text = adamw_multi(e, bits)
+        assert rc == INVALID and b"aligned to their values" in text, name
