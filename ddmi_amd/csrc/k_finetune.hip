@@ -675,7 +675,7 @@ int ft_plan(FtArgs* a, int B, int C, int64_t HW, bool mixed, int rows_of, int ke
     ft_split(a, want);
   }
   const int64_t wps = cdiv64(a->C, a->rows_per_wg) * a->nseg;
-  if (wps * B + C > FT_MOST_GROUPS) return ddmi_fail(DDMI_ERR_INVALID, "fine-tuning loss: too many values in one call");
+  if (1 + C + wps * B > FT_MOST_GROUPS) return ddmi_fail(DDMI_ERR_INVALID, "fine-tuning loss: too many values in one call");
   a->wps = (int)wps;
   return DDMI_OK;
 }

@@ -132,3 +132,15 @@ def test_c_adamw_refuses_unaligned_pointers(bits, names):
         e[name][1] = 66
         rc, text = adamw_multi(e, bits)
         assert rc == INVALID and b"aligned to their values" in text, name
+
+
+# ---- grids -----------------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("mixed", [0, 1])
+def test_loss_grids_stay_below_2_to_32_threads(mixed):
+    """The gradient's launch has a workgroup of 256 threads for each span, one for each channel and one for the loss: at most 2^24 - 1."""
+    size = C.c_size_t(0)
+    ask = lambda B, channels: _lib.lib().ddmi_train_loss_workspace_bytes(B, channels, 1, mixed, C.byref(size))      # noqa: E731
+    most = 2 ** 24 - 1
+    for channels in (1, 3):
+        assert ask(most - 1 - channels, channels) == 0 and size.value > 0
+        assert ask(most - channels, channels) == INVALID and b"too many values" in _lib.lib().ddmi_last_error()
