@@ -312,7 +312,10 @@ int launch_bits(const AdArgs& a, unsigned grid, int pdt, int gdt, hipStream_t s)
 int launch_adamw_multi(const ddmi_adamw_tensor* t, int n, double beta1, double beta2, double eps, double grad_scale, unsigned seed, int pdt, int gdt,
                        int state_bits, hipStream_t s) {
   double values = 0.0;
-  for (int i = 0; i < n; ++i) values += (double)t[i].numel;
+  for (int i = 0; i < n; ++i) {                // before anything is launched: a call that is refused changes no tensor
+    if (cdiv64(t[i].numel, AD_CHUNK) > FT_MOST_GROUPS) return ddmi_fail(DDMI_ERR_INVALID, "adamw_multi: a tensor of more than 2^36 values");
+    values += (double)t[i].numel;
+  }
   PROF_SCOPE(state_bits == 8 ? "adamw8" : "adamw_multi", 0, values * (2.0 * dt_size(pdt) + dt_size(gdt) + (state_bits == 8 ? 4.0 : 16.0)), s);
   const bool nt = values * (dt_size(pdt) + dt_size(gdt) + (state_bits == 8 ? 2.0 : 8.0)) > FT_CACHE_BYTES;
   AdArgs a;
@@ -326,7 +329,6 @@ int launch_adamw_multi(const ddmi_adamw_tensor* t, int n, double beta1, double b
       const ddmi_adamw_tensor& d = t[i];
       const int64_t wgs = cdiv64(d.numel, AD_CHUNK);
       if (wgs == 0) { ++i; continue; }
-      if (wgs > FT_MOST_GROUPS) return ddmi_fail(DDMI_ERR_INVALID, "adamw_multi: a tensor of more than 2^36 values");
       if ((int64_t)a.first[a.count] + wgs > FT_MOST_GROUPS) break;
       AdTensor& o = a.t[a.count];
       o.p = d.param; o.g = d.grad; o.m = d.exp_avg; o.v = d.exp_avg_sq; o.ms = d.exp_avg_scale; o.vs = d.exp_avg_sq_scale; o.n = d.numel;

@@ -134,6 +134,14 @@ def test_c_adamw_refuses_unaligned_pointers(bits, names):
         assert rc == INVALID and b"aligned to their values" in text, name
 
 
+def test_c_adamw_refuses_a_tensor_too_large_before_it_launches():
+    """The 60th of a list whose first 48 would be a launch of their own (which no card here could run)."""
+    e = entries(60)
+    e["numel"][59] = 1 << 37
+    rc, text = adamw_multi(e)
+    assert rc == INVALID and b"more than 2^36" in text
+
+
 # ---- grids -----------------------------------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("mixed", [0, 1])
 def test_loss_grids_stay_below_2_to_32_threads(mixed):
