@@ -234,12 +234,18 @@ class AdamW:
         return (decode_moment(self.exp_avg[i], self.exp_avg_scale[i], False).view(shape),
                 decode_moment(self.exp_avg_sq[i], self.exp_avg_sq_scale[i], True).view(shape))
 
+    def _check_moments(self, i: int, exp_avg, exp_avg_sq, step: int) -> None:
+        for name, new in (("exp_avg", exp_avg), ("exp_avg_sq", exp_avg_sq)):
+            shape = tuple(torch.as_tensor(new).shape)
+            if shape != tuple(self.params[i].shape):
+                raise ValueError(f"AdamW: {name} of parameter {i} has shape {shape}, the parameter {tuple(self.params[i].shape)}")
+        if step < 0:
+            raise ValueError(f"AdamW: parameter {i} has taken {step} steps")
+
     def set_moments(self, i: int, exp_avg, exp_avg_sq, step: int) -> None:
+        self._check_moments(i, exp_avg, exp_avg_sq, step)
         for name, new, root in (("exp_avg", exp_avg, False), ("exp_avg_sq", exp_avg_sq, True)):
-            new = torch.as_tensor(new)
-            if tuple(new.shape) != tuple(self.params[i].shape):
-                raise ValueError(f"AdamW: {name} of parameter {i} has shape {tuple(new.shape)}, the parameter {tuple(self.params[i].shape)}")
-            new = new.to(self.params[i].device, torch.float32)
+            new = torch.as_tensor(new).to(self.params[i].device, torch.float32)
             if self.state_bits == 32:
                 getattr(self, name)[i].copy_(new.reshape(-1))
             else:
@@ -259,18 +265,36 @@ class AdamW:
         return {"state": state, "param_groups": [dict(g, **rest) for g in self.param_groups]}
 
     def load_state_dict(self, sd: Dict) -> None:
-        """torch.optim.AdamW's layout; 8-bit moments are rounded to the nearest code (exact for values that came out of an 8-bit state)."""
+        """torch.optim.AdamW's layout; 8-bit moments are rounded to the nearest code (exact for values that came out of an 8-bit state).  A
+        state of another optimizer - amsgrad, maximize, weight decay that is not decoupled, betas or eps of a group's own - is refused, and a
+        refused state changes nothing."""
         groups = sd["param_groups"]
         if [list(g["params"]) for g in groups] != [list(g["params"]) for g in self.param_groups]:
             raise ValueError("AdamW: the state dict has other parameter groups")
-        for g, mine in zip(groups, self.param_groups):
-            mine["lr"], mine["weight_decay"] = float(g["lr"]), float(g["weight_decay"])
-        self.betas, self.eps = tuple(float(b) for b in groups[0]["betas"]), float(groups[0]["eps"])
+        for k in ("amsgrad", "maximize"):
+            if any(g.get(k) for g in groups):
+                raise ValueError(f"AdamW: the state dict is that of an optimizer with {k}")
+        if any(float(g["weight_decay"]) != 0.0 and not g.get("decoupled_weight_decay", True) for g in groups):
+            raise ValueError("AdamW: the state dict is that of an optimizer whose weight decay is a part of the gradient")
+        rates = [(float(g["lr"]), float(g["weight_decay"])) for g in groups]
+        shared = {(tuple(float(b) for b in g["betas"]), float(g["eps"])) for g in groups}
+        if len(shared) > 1:
+            raise ValueError(f"AdamW: all groups have the same betas and eps, the state dict has {sorted(shared)}")
+        (betas, eps), = shared
+        if len(betas) != 2 or not (all(0.0 <= b < 1.0 for b in betas) and eps >= 0.0):
+            raise ValueError(f"AdamW: betas in [0, 1) and eps >= 0, the state dict has {betas}, {eps}")
         extra = [i for i in sd["state"] if not (isinstance(i, int) and 0 <= i < len(self.params))]
         if extra:
             raise ValueError(f"AdamW: state for parameters {extra[:5]}, of {len(self.params)}")
-        zero = [i for i in range(len(self.params)) if i not in sd["state"]]
+        state = {}
         for i, st in sd["state"].items():
-            self.set_moments(i, st["exp_avg"], st["exp_avg_sq"], int(float(st["step"])))
-        for i in zero:
-            self.set_moments(i, torch.zeros(self.params[i].shape), torch.zeros(self.params[i].shape), 0)
+            missing = {"step", "exp_avg", "exp_avg_sq"} - set(st)
+            if missing:
+                raise ValueError(f"AdamW: the state of parameter {i} has no {sorted(missing)}")
+            state[i] = (st["exp_avg"], st["exp_avg_sq"], int(float(st["step"])))
+            self._check_moments(i, *state[i])
+        for (lr, weight_decay), mine in zip(rates, self.param_groups):
+            mine["lr"], mine["weight_decay"] = lr, weight_decay
+        self.betas, self.eps = betas, eps
+        for i, p in enumerate(self.params):
+            self.set_moments(i, *(state[i] if i in state else (torch.zeros(p.shape), torch.zeros(p.shape), 0)))

@@ -10,7 +10,7 @@ from torch.autograd import forward_ad
 import finetune_ref as R
 from ddmi_amd import _lib, finetune
 from ddmi_amd.finetune import policy_loss, preference_loss, transition_log_prob
-from ddmi_amd.optim import _ENTRY, adamw_step
+from ddmi_amd.optim import _ENTRY, AdamW, adamw_step
 
 
 # ---- forward-mode derivatives -------------------------------------------------------------------------------------------------------
@@ -152,3 +152,74 @@ def test_loss_grids_stay_below_2_to_32_threads(mixed):
     for channels in (1, 3):
         assert ask(most - 1 - channels, channels) == 0 and size.value > 0
         assert ask(most - channels, channels) == INVALID and b"too many values" in _lib.lib().ddmi_last_error()
+
+
+# ---- optimizer states ------------------------------------------------------------------------------------------------------------------
+def stepped(cls=torch.optim.AdamW, **kw):
+    """Two groups of CPU parameters, and torch's state dict after a step over them."""
+    ps = [torch.nn.Parameter(torch.full((k + 2,), 1.0)) for k in range(3)]
+    opt = cls([{"params": ps[:2], "weight_decay": 0.1}, {"params": ps[2:]}], **dict(dict(lr=1e-3, betas=(0.8, 0.9), eps=1e-6), **kw))
+    for p in ps:
+        p.grad = torch.full_like(p, 0.5)
+    opt.step()
+    return ps, opt.state_dict()
+
+
+def snapshot(opt):
+    bits = lambda t: t.view(torch.uint8) if t.dtype == torch.float8_e4m3fn else t      # noqa: E731
+    slabs = [opt.exp_avg, opt.exp_avg_sq] + ([opt.exp_avg_scale, opt.exp_avg_sq_scale] if opt.state_bits == 8 else [])
+    return [bits(t).clone() for ts in slabs for t in ts], [dict(g) for g in opt.param_groups], opt.betas, opt.eps, list(opt.steps)
+
+
+def of_group(k, **kw):
+    return lambda sd: sd["param_groups"][k].update(kw)
+
+
+def of_state(i, **kw):
+    return lambda sd: sd["state"].__setitem__(i, {k: v for k, v in dict(sd["state"].get(i, {}), **kw).items() if v is not None})
+
+
+@pytest.mark.parametrize("change,message", [
+    (of_group(1, amsgrad=True), "amsgrad"),
+    (of_group(0, maximize=True), "maximize"),
+    (of_group(0, decoupled_weight_decay=False), "part of the gradient"),
+    (of_group(1, betas=(0.7, 0.9)), "same betas and eps"),
+    (of_group(1, eps=1e-3), "same betas and eps"),
+    (lambda sd: [g.update(betas=(1.0, 0.9)) for g in sd["param_groups"]], r"betas in \[0, 1\)"),
+    (of_group(0, params=[0]), "other parameter groups"),
+    (of_state(9, step=1.0, exp_avg=torch.zeros(2), exp_avg_sq=torch.zeros(2)), "state for parameters"),
+    (of_state(2, exp_avg=None), "has no"),
+    (of_state(1, exp_avg_sq=torch.zeros(9)), "exp_avg_sq of parameter 1 has shape"),
+    (of_state(0, step=-1.0), "steps"),
+])
+@pytest.mark.parametrize("bits", [32, 8])
+def test_state_dicts_of_other_optimizers_are_refused_and_change_nothing(change, message, bits):
+    ps, sd = stepped()
+    opt = AdamW([{"params": ps[:2], "weight_decay": 0.2}, {"params": ps[2:]}], lr=5e-4, state_bits=bits)
+    opt.set_moments(0, torch.ones(2), torch.ones(2), 3)
+    before = snapshot(opt)
+    sd["param_groups"][0]["lr"] = 9.0
+    change(sd)
+    with pytest.raises(ValueError, match=message):
+        opt.load_state_dict(sd)
+    after = snapshot(opt)
+    assert all(map(torch.equal, before[0], after[0])) and before[1:] == after[1:]
+
+
+def test_state_dict_of_torch_loads():
+    ps, sd = stepped()
+    opt = AdamW([{"params": ps[:2], "weight_decay": 0.2}, {"params": ps[2:]}], lr=5e-4)
+    opt.load_state_dict(sd)
+    assert [g["lr"] for g in opt.param_groups] == [1e-3] * 2 and [g["weight_decay"] for g in opt.param_groups] == [0.1, 0.01]
+    assert opt.betas == (0.8, 0.9) and opt.eps == 1e-6 and opt.steps == [1, 1, 1]
+    for i in range(3):
+        assert all(torch.equal(a, sd["state"][i][k]) for a, k in zip(opt.moments(i), ("exp_avg", "exp_avg_sq")))
+    with pytest.raises(ValueError, match="part of the gradient"):
+        opt.load_state_dict(stepped(torch.optim.Adam)[1])
+
+
+def test_set_moments_checks_both_before_either_is_set():
+    opt = AdamW([torch.zeros(4)])
+    with pytest.raises(ValueError, match="exp_avg_sq"):
+        opt.set_moments(0, torch.ones(4), torch.ones(5), 1)
+    assert not opt.exp_avg[0].any() and opt.steps == [0]
