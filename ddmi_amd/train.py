@@ -1190,10 +1190,13 @@ class LDMTrainStep:
     @torch.no_grad()
     def rollout(self, batch: int, sampling_timesteps: Optional[int] = None, eta: float = 1.0, x_T=None, generator=None) -> Rollout:
         """Chains of the trained network as `DDPM.sample` runs them (ancestral, or DDIM over `sampling_timesteps`), with every transition
-        and its log-density: what policy_step takes once the x_0 have been rewarded."""
+        and its log-density: what policy_step takes once the x_0 have been rewarded.  An ancestral chain with `clip_denoised` is refused: its
+        steps are not linear in the prediction (DDIM chains do not clip)."""
         from .ddpm import DDPM, ddim_time_pairs
         ddpm = DDPM(model=None, **dict(self._ddpmconfig, sampling_timesteps=sampling_timesteps or self.num_timesteps, ddim_sampling_eta=eta,
-                                       timesteps=self.num_timesteps, clip_denoised=False))
+                                       timesteps=self.num_timesteps))
+        if ddpm.is_ddim_sampling:
+            ddpm.clip_denoised = False
         ddpm.mixed_prediction = self.mixing_logit is not None
         logit = None if self.mixing_logit is None else self.mixing_logit.detach()
         ddpm._logit_dev = None if logit is None else logit.reshape(-1)

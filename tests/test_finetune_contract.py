@@ -1,6 +1,7 @@
 """Calls of the fine-tuning operators that are refused, and rules of their plans, without a GPU."""
 import ctypes as C
 import math
+import types
 
 import numpy as np
 import pytest
@@ -11,6 +12,7 @@ import finetune_ref as R
 from ddmi_amd import _lib, finetune
 from ddmi_amd.finetune import policy_loss, preference_loss, transition_log_prob
 from ddmi_amd.optim import _ENTRY, AdamW, adamw_step
+from ddmi_amd.train import LDMTrainStep
 
 
 # ---- forward-mode derivatives -------------------------------------------------------------------------------------------------------
@@ -223,3 +225,12 @@ def test_set_moments_checks_both_before_either_is_set():
     with pytest.raises(ValueError, match="exp_avg_sq"):
         opt.set_moments(0, torch.ones(4), torch.ones(5), 1)
     assert not opt.exp_avg[0].any() and opt.steps == [0]
+
+
+# ---- the training step -----------------------------------------------------------------------------------------------------------------
+def test_rollout_of_a_clipping_sampler_is_refused():
+    """The ancestral sampler clips x_0 where the configuration says so, and then its steps have no mean A x_t + E eps."""
+    host = types.SimpleNamespace(_ddpmconfig={"clip_denoised": True, "channels": 2}, num_timesteps=12, mixing_logit=None, video=False, channels=2, image_size=4,
+                                 device=torch.device("cpu"), model=lambda *a: pytest.fail("the chain was begun"))
+    with pytest.raises(ValueError, match="clip_denoised"):
+        LDMTrainStep.rollout(host, 2)
