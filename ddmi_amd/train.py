@@ -1342,10 +1342,15 @@ class LDMTrainStep:
             if not resume:
                 return self
             if ck.get("reference"):
-                self.reference, off = torch.empty_like(self.flat.data), 0
+                reference, off = torch.empty_like(self.flat.data), 0
                 for k, p in named:
-                    self.reference[off:off + p.numel()].copy_(torch.as_tensor(ck["reference"][k]).to(self.device, torch.float32).reshape(-1))
+                    v = ck["reference"].get(k)
+                    if v is None or tuple(torch.as_tensor(v).shape) != tuple(p.shape):
+                        raise ValueError(f"checkpoint reference: '{k}' {tuple(p.shape)} is " +
+                                         ("missing" if v is None else f"{tuple(torch.as_tensor(v).shape)} there") + ": the checkpoint is of another model")
+                    reference[off:off + p.numel()].copy_(torch.as_tensor(v).to(self.device, torch.float32).reshape(-1))
                     off += p.numel()
+                self.reference = reference                       # whole, or what it was
             opt = ck.get("dae_opt") or {}
             if "state" in opt:
                 steps = []

@@ -12,7 +12,7 @@ import finetune_ref as R
 from ddmi_amd import _lib, finetune
 from ddmi_amd.finetune import policy_loss, preference_loss, transition_log_prob
 from ddmi_amd.optim import _ENTRY, AdamW, adamw_step
-from ddmi_amd.train import LDMTrainStep
+from ddmi_amd.train import FlatParams, LDMTrainStep
 
 
 # ---- forward-mode derivatives -------------------------------------------------------------------------------------------------------
@@ -234,3 +234,16 @@ def test_rollout_of_a_clipping_sampler_is_refused():
                                  device=torch.device("cpu"), model=lambda *a: pytest.fail("the chain was begun"))
     with pytest.raises(ValueError, match="clip_denoised"):
         LDMTrainStep.rollout(host, 2)
+
+
+@pytest.mark.parametrize("change,message", [(lambda r: r.pop("b"), "'b' .* is missing"), (lambda r: r.update(b=torch.ones(1)), r"'b' \(3,\) is \(1,\) there")])
+def test_a_reference_of_another_model_is_refused(change, message):
+    """A missing parameter used to leave a reference half filled, one of a single value to be spread over the parameter."""
+    named = [("a", torch.nn.Parameter(torch.zeros(2))), ("b", torch.nn.Parameter(torch.zeros(3)))]
+    kept = torch.zeros(5)
+    host = types.SimpleNamespace(flat=FlatParams([p for _, p in named], "cpu"), named_parameters=lambda: named, device=torch.device("cpu"), reference=kept)
+    reference = {"a": torch.ones(2), "b": torch.ones(3)}
+    change(reference)
+    with pytest.raises(ValueError, match=message):
+        LDMTrainStep.load_training_state(host, {"reference": reference})
+    assert host.reference is kept and not kept.any()
