@@ -34,6 +34,7 @@ struct FtArgs {
   int B, C, pairs;
   int64_t T, seg;
   int wps, rows_per_wg, nseg, log_g, fused, polls;
+  int again;                 // gradients of a call that has run, from its workspace, unless the upstream gradient is 1
   // workspace
   double* total;             // sum of the weights
   int* done;                 // one pass: whether a span's gradient is written

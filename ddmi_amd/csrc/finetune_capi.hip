@@ -32,6 +32,8 @@ int common_args(FtArgs* a, const ddmi_loss_in* in, int B, int rows_of, int keep,
   a->logit = in->mixing_logit; a->ref_logit = in->ref_mixing_logit; a->weight = in->weight;
   return DDMI_OK;
 }
+// vectors a thread of the one-pass form keeps
+int kept(int mode, const ddmi_loss_in* in) { return mode == FT_POLICY && in->ref_out ? FT_VECS / 2 : FT_VECS; }
 int run(FtArgs* a, int mode, int out_dtype, hipStream_t s) {
   DDMI_TRY(launch_ft_sums(*a, mode, internal_dt(out_dtype), s));
   return a->d_out ? launch_ft_grad(*a, mode, internal_dt(out_dtype), s) : DDMI_OK;
@@ -61,7 +63,7 @@ int ddmi_train_pref_loss(const ddmi_loss_in* in, int pairs, int noise_rows, doub
   DDMI_REQUIRE(label_smoothing >= 0.0 && label_smoothing <= 1.0 && std::isfinite(beta), "pref_loss: label_smoothing in [0, 1], beta finite");
   DDMI_REQUIRE(!d_logit || (in->mixing_logit && d_model_out), "pref_loss: d_logit goes with mixing_logit and d_model_out");
   DDMI_REQUIRE(aligned({loss, margin, mse, dloss, d_logit}, 4) && aligned({d_model_out}, size_of(in->out_dtype)), "pref_loss: outputs aligned to their values");
-  DDMI_TRY(common_args(&a, in, 2 * pairs, 2, d_model_out ? FT_VECS : 0, ws, ws_bytes));
+  DDMI_TRY(common_args(&a, in, 2 * pairs, 2, d_model_out ? kept(FT_PREF, in) : 0, ws, ws_bytes));
   if (!in->mixing_logit) a.x = nullptr;      // not read
   a.pairs = pairs; a.second_rows = noise_rows; a.beta = beta; a.smoothing = label_smoothing;
   a.loss = loss; a.row_out[0] = margin; a.row_out[1] = mse; a.dloss = dloss; a.d_out = d_model_out; a.d_logit = d_logit;
@@ -79,7 +81,7 @@ int ddmi_train_policy_loss(const ddmi_loss_in* in, int B, const float* transitio
   DDMI_REQUIRE(!d_logit || (in->mixing_logit && d_model_out), "policy_loss: d_logit goes with mixing_logit and d_model_out");
   DDMI_REQUIRE(aligned({transition, logp_old, advantage, loss, logp, ratio, kl, dloss, d_logit}, 4) && aligned({d_model_out}, size_of(in->out_dtype)),
                "policy_loss: tensors aligned to their values");
-  DDMI_TRY(common_args(&a, in, B, 1, d_model_out ? (in->ref_out ? FT_VECS / 2 : FT_VECS) : 0, ws, ws_bytes));
+  DDMI_TRY(common_args(&a, in, B, 1, d_model_out ? kept(FT_POLICY, in) : 0, ws, ws_bytes));
   a.pairs = B; a.second_rows = B; a.transition = transition;
   a.logp_old = logp_old; a.advantage = advantage; a.clip = clip_range; a.kl_coef = kl_coef;
   a.loss = logp_old ? loss : nullptr; a.row_out[0] = logp; a.row_out[1] = ratio; a.row_out[2] = kl;
@@ -90,6 +92,21 @@ int ddmi_train_loss_scale(const float* dloss, void* d_model_out, int out_dtype, 
   DDMI_REQUIRE(dloss && d_model_out && n > 0 && dtype_ok(out_dtype) && (!d_logit || C > 0), "loss_scale: bad arguments");
   DDMI_REQUIRE(aligned({dloss, d_logit}, 4) && aligned({d_model_out}, size_of(out_dtype)), "loss_scale: tensors aligned to their values");
   return launch_ft_scale(dloss, d_model_out, internal_dt(out_dtype), n, d_logit, C, (hipStream_t)stream);
+}
+int ddmi_train_loss_again(const ddmi_loss_in* in, int B, int noise_rows, const float* transition, const float* dloss, void* ws, size_t ws_bytes,
+                          void* d_model_out, float* d_logit, void* stream) {
+  const int mode = transition ? FT_POLICY : FT_PREF;
+  FtArgs a{};
+  DDMI_REQUIRE(in && dloss && d_model_out, "loss_again: null argument");
+  DDMI_REQUIRE(transition ? in->x_t != nullptr : in->ref_out && B % 2 == 0 && (noise_rows == B / 2 || noise_rows == B), "loss_again: arguments of neither loss");
+  DDMI_REQUIRE(!d_logit || in->mixing_logit, "loss_again: d_logit goes with mixing_logit");
+  DDMI_REQUIRE(aligned({transition, dloss, d_logit}, 4) && aligned({d_model_out}, size_of(in->out_dtype)), "loss_again: tensors aligned to their values");
+  DDMI_TRY(common_args(&a, in, B, transition ? 1 : 2, kept(mode, in), ws, ws_bytes));
+  if (!transition && !in->mixing_logit) a.x = nullptr;      // not read
+  a.pairs = transition ? B : B / 2; a.second_rows = transition ? B : noise_rows; a.transition = transition;
+  a.dloss = dloss; a.d_out = d_model_out; a.d_logit = d_logit;
+  a.fused = 0; a.again = 1;
+  return launch_ft_grad(a, mode, internal_dt(in->out_dtype), (hipStream_t)stream);
 }
 int ddmi_stream_capture_id(void* stream, uint64_t* id) {
   DDMI_REQUIRE(id, "stream_capture_id: null argument");

@@ -549,7 +549,7 @@ __device__ __forceinline__ void grad_span(const FtArgs& a, int blk, float up, fl
 }
 
 // Workgroup 0: the loss; the next `channels`: one channel's logit each; the others take spans in turn, but for those that are in d_out
-// already.
+// already.  `again`: the loss stays, and so does everything where the gradients are those for an upstream gradient of 1 already.
 template <int MODE, bool MIX, bool REF, typename T>
 __global__ void __launch_bounds__(FT_THREADS) grad_kernel(FtArgs a, int spans, int channels) {
   __shared__ float2 mix[FT_ROWS];
@@ -557,8 +557,9 @@ __global__ void __launch_bounds__(FT_THREADS) grad_kernel(FtArgs a, int spans, i
   const int tid = threadIdx.x;
   const float up = a.dloss ? *a.dloss : 1.f;
   const int wg = (int)blockIdx.x - 1 - channels, ch = (int)blockIdx.x - 1;
+  if (a.again && up == 1.f) return;
   if (blockIdx.x == 0) {
-    sum_terms(a, MODE == FT_PREF ? a.pairs : a.B, red);
+    if (!a.again) sum_terms(a, MODE == FT_PREF ? a.pairs : a.B, red);
     return;
   }
   if (ch < channels) {
@@ -609,7 +610,8 @@ int launch_sums_t(const FtArgs& a, int dt, hipStream_t s) {
 template <int MODE, bool MIX, bool REF>
 int launch_grad_t(const FtArgs& a, int dt, hipStream_t s) {
   const int spans = a.B * a.wps, channels = MIX && a.d_logit ? a.C : 0;
-  const dim3 grid((unsigned)(1 + channels + (a.fused ? std::min(spans, 1024) : spans)));   // 1 024 look through what is most often done
+  // 1 024 look through what is most often done, 2 048 (eight a compute unit) take what may not have to be done at all
+  const dim3 grid((unsigned)(1 + channels + (a.fused ? std::min(spans, 1024) : a.again ? std::min(spans, 2048) : spans)));
   if (dt == DT_F32) hipLaunchKernelGGL((grad_kernel<MODE, MIX, REF, float>), grid, dim3(FT_THREADS), 0, s, a, spans, channels);
   else hipLaunchKernelGGL((grad_kernel<MODE, MIX, REF, bf16_t>), grid, dim3(FT_THREADS), 0, s, a, spans, channels);
   HIP_TRY(hipGetLastError());

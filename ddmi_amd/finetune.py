@@ -109,7 +109,8 @@ def _flat(t):
 
 
 def _launch(entry, tensors, extra, args, stats, g, grads, mixed):
-    """One call of a loss's C entry point: ((loss, *statistics), (d_model_out, d_logit)).  tensors: model_out, ref_out, x_t, noise / x_prev,
+    """One call of a loss's C entry point: ((loss, *statistics), (d_model_out, d_logit, its workspace if
+    gradients may be asked of it again)).  tensors: model_out, ref_out, x_t, noise / x_prev,
     sqrt_1mac, mixing_logit, ref_mixing_logit, weight - contiguous; extra: the tensors, args: the numbers behind them; stats: rows of each
     statistic; g: the upstream gradient (None: 1); grads, mixed: whether the output's / the logit's gradient is wanted."""
     out, logit = tensors[0], tensors[5]
@@ -119,17 +120,21 @@ def _launch(entry, tensors, extra, args, stats, g, grads, mixed):
     d_logit = torch.empty_like(logit) if mixed else None
     results = [torch.empty((), dtype=torch.float32, device=dev)] + [torch.empty((n,), dtype=torch.float32, device=dev) for n in stats]
     ws = torch.empty(_workspace_bytes(B, Cc, HW, logit is not None), dtype=torch.uint8, device=dev)
-    given = _lib.LossIn(*map(_p, tensors), HW, Cc, _OUT_TYPES[out.dtype])
-    _lib.check(entry(C.byref(given), *args[0], *map(_p, extra), *args[1], _p(g), ws.data_ptr(), ws.numel(), *map(_p, results), _p(d_out), _p(d_logit),
-                     _lib.raw_stream(out.get_device())))
-    return results, (d_out, d_logit)
+    _lib.check(entry(C.byref(_given(tensors)), *args[0], *map(_p, extra), *args[1], _p(g), ws.data_ptr(), ws.numel(), *map(_p, results), _p(d_out),
+                     _p(d_logit), _lib.raw_stream(out.get_device())))
+    return results, (d_out, d_logit, None if out.dtype == torch.float32 else ws)
+
+
+def _given(tensors):
+    out = tensors[0]
+    return _lib.LossIn(*map(_p, tensors), out.numel() // (out.shape[0] * out.shape[1]), out.shape[1], _OUT_TYPES[out.dtype])
 
 
 class LossFn(torch.autograd.Function):
-    """A loss that is computed already, its gradients for an upstream gradient of 1 along with it.  The first backward hands those out -
-    multiplied in place when the upstream gradient, which only the device knows, is another (a bf16 gradient is then rounded a second time) -
-    and a later one (retain_graph) computes them again from the saved inputs, as does one that is captured apart from its forward: each replay
-    of it would multiply once more."""
+    """A loss that is computed already, its gradients for an upstream gradient of 1 along with it.  The first backward hands those out.  Where
+    the upstream gradient, which only the device knows, is another, fp32 gradients are multiplied in place, and bf16 ones are computed again from
+    the inputs and the sums in the forward's workspace: multiplied, they would be rounded to bf16 twice.  A later backward (retain_graph) is a
+    call of its own from the saved inputs, as is one that is captured apart from its forward: each replay of it would multiply once more."""
 
     @staticmethod
     def forward(ctx, model_out, mixing_logit, loss, grads, again, capture):      # loss, grads in lists: they are no inputs
@@ -150,14 +155,24 @@ class LossFn(torch.autograd.Function):
             g = g.contiguous()
         with _lib.on_device(ctx.index):
             if ctx.grads is not None and _lib.capture_id(_lib.raw_stream(ctx.index)) == ctx.capture:
-                (d_out, d_logit), ctx.grads = ctx.grads, None
-                _lib.check(_lib.lib().ddmi_train_loss_scale(g.data_ptr(), d_out.data_ptr(), _OUT_TYPES[d_out.dtype], d_out.numel(), _p(d_logit),
-                                                            0 if d_logit is None else d_logit.numel(), _lib.raw_stream(ctx.index)))
+                (d_out, d_logit, ws), ctx.grads = ctx.grads, None
+                if d_out.dtype == torch.float32:
+                    _lib.check(_lib.lib().ddmi_train_loss_scale(g.data_ptr(), d_out.data_ptr(), _lib.DTYPE_F32, d_out.numel(), _p(d_logit),
+                                                                0 if d_logit is None else d_logit.numel(), _lib.raw_stream(ctx.index)))
+                else:
+                    saved = LossFn._saved(ctx)
+                    noise_rows = saved[3].shape[0]      # not read of the policy loss, which has a transition
+                    _lib.check(_lib.lib().ddmi_train_loss_again(C.byref(_given(saved[:8])), d_out.shape[0], noise_rows, _p(saved[8]) if saved[8:] else None,
+                                                                g.data_ptr(), ws.data_ptr(), ws.numel(), d_out.data_ptr(), _p(d_logit),
+                                                                _lib.raw_stream(ctx.index)))
             else:
-                saved, (entry, (args, stats, mixed)) = ctx.saved_tensors, ctx.again
-                saved = [ctx.beside.get(i, t) for i, t in enumerate(saved)]
-                d_out, d_logit = _launch(entry, saved[:8], saved[8:], args, stats, g, True, mixed)[1]
+                saved, (entry, (args, stats, mixed)) = LossFn._saved(ctx), ctx.again
+                d_out, d_logit, _ = _launch(entry, saved[:8], saved[8:], args, stats, g, True, mixed)[1]
         return d_out, d_logit, None, None, None, None
+
+    @staticmethod
+    def _saved(ctx):
+        return [ctx.beside.get(i, t) for i, t in enumerate(ctx.saved_tensors)]
 
     _with_graph = staticmethod(once_differentiable(_gradients.__func__))      # create_graph: a second derivative through here raises
 
@@ -290,7 +305,6 @@ def transition_log_prob(model_out, x_t, x_prev, transition, sqrt_1mac, mixing_lo
         transition = _flat(transition)
         logp = torch.empty((B,), dtype=torch.float32, device=model_out.device)
         ws = torch.empty(_workspace_bytes(B, Cc, HW, mixing_logit is not None), dtype=torch.uint8, device=model_out.device)
-        given = _lib.LossIn(*map(_p, tensors), HW, Cc, _OUT_TYPES[model_out.dtype])
-        _lib.check(_lib.lib().ddmi_train_policy_loss(C.byref(given), B, transition.data_ptr(), None, None, 0.0, 0.0, None, ws.data_ptr(), ws.numel(), None,
+        _lib.check(_lib.lib().ddmi_train_policy_loss(C.byref(_given(tensors)), B, transition.data_ptr(), None, None, 0.0, 0.0, None, ws.data_ptr(), ws.numel(), None,
                                                      logp.data_ptr(), None, None, None, None, _lib.raw_stream(dev)))
         return logp

@@ -541,6 +541,11 @@ int ddmi_train_policy_loss(const ddmi_loss_in* in, int B, const float* transitio
                            void* d_model_out, float* d_logit, void* stream);
 /* gradients of a loss call without dloss, times *dloss in place (n values of out_dtype, C logits; nothing is touched when it is 1) */
 int ddmi_train_loss_scale(const float* dloss, void* d_model_out, int out_dtype, int64_t n, float* d_logit, int C, void* stream);
+/* The same from the inputs, for types that a second rounding costs something: the arguments and the workspace of a loss call without dloss,
+ * neither changed since (B = 2 pairs and transition = NULL: the preference loss; noise_rows is its own, the policy loss has none).  Each value
+ * is rounded once, as by a loss call with dloss; nothing is touched when *dloss is 1. */
+int ddmi_train_loss_again(const ddmi_loss_in* in, int B, int noise_rows, const float* transition, const float* dloss, void* ws, size_t ws_bytes,
+                          void* d_model_out, float* d_logit, void* stream);
 /* the capture that `stream` is recorded into, 0 outside of one: gradients of a loss call may be scaled in place only within the capture that
  * computed them (a second replay would scale them again) */
 int ddmi_stream_capture_id(void* stream, uint64_t* id);

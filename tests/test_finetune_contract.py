@@ -247,3 +247,21 @@ def test_a_reference_of_another_model_is_refused(change, message):
     with pytest.raises(ValueError, match=message):
         LDMTrainStep.load_training_state(host, {"reference": reference})
     assert host.reference is kept and not kept.any()
+
+
+# ---- gradients asked again -------------------------------------------------------------------------------------------------------------
+def test_c_loss_again_refuses():
+    """A workspace of no bytes ends a call that gets past its arguments."""
+    c = CLoss(1)
+
+    def again(B=4, noise_rows=2, transition=None, dloss=64, size=0, d_out=64, d_logit=64, **fields):
+        s = _lib.LossIn(**dict(c.fields, **fields))
+        return c.lib.ddmi_train_loss_again(C.byref(s), B, noise_rows, transition, dloss, 64, size, d_out, d_logit, None)
+
+    for kw in (dict(), dict(noise_rows=4), dict(transition=64, noise_rows=0), dict(transition=64, ref_out=None, ref_mixing_logit=None)):
+        assert again(**kw) == INVALID and b"workspace" in c.error(), kw
+    for kw, text in ((dict(dloss=None), b"null"), (dict(d_out=None), b"null"), (dict(B=3), b"neither"), (dict(noise_rows=3), b"neither"),
+                     (dict(ref_out=None), b"neither"), (dict(transition=64, x_t=None), b"neither"),
+                     (dict(mixing_logit=None, ref_mixing_logit=None), b"d_logit goes"), (dict(dloss=66), b"aligned"), (dict(d_logit=66), b"aligned"),
+                     (dict(d_out=65), b"aligned"), (dict(transition=65), b"aligned"), (dict(x_t=66), b"aligned"), (dict(B=0, noise_rows=0), b"empty batch")):
+        assert again(**kw) == INVALID and text in c.error(), (kw, c.error())

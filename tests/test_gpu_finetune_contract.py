@@ -5,7 +5,7 @@ import pytest
 import torch
 
 import finetune_ref as R
-from ddmi_amd.finetune import transition_log_prob
+from ddmi_amd.finetune import policy_loss, preference_loss, transition_log_prob
 from test_gpu_finetune import DEV, SHAPES, call, reference
 
 pytestmark = pytest.mark.gpu
@@ -77,3 +77,70 @@ def test_gradients_of_many_small_transitions():
     d["weight"] = (torch.arange(100000, device=DEV) % 7).float()
     d["clip_range"] = 1e9
     R.check(call("policy", d), reference("policy", d))
+
+
+# ---- upstream gradients ----------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("op,kl", [("pref", True), ("policy", True), ("policy", False)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("B,C,T", BOTH)
+@pytest.mark.parametrize("mixed,weight", [(True, None), (False, "some")])
+@pytest.mark.parametrize("up", [3.0, -1.0 / 3.0])
+def test_an_upstream_gradient_costs_no_second_rounding_to_bf16(op, kl, dtype, B, C, T, mixed, weight, up):
+    """The first backward's gradients are `up` times the formula's within the formula's own bound: one rounding to the output's type, and the
+    fp32 factor's and product's own.  A second backward gives the same (in bf16 the same bits)."""
+    d = R.make(op, B, C, T, dtype, mixed, kl=kl, weight=weight, seed=31, device=DEV)
+    want = reference(op, d)
+    leaves = [d["model_out"].requires_grad_()] + ([d["mixing_logit"].requires_grad_()] if mixed else [])
+    loss = (preference_loss if op == "pref" else policy_loss)(**d).loss
+    up = torch.tensor(up, device=DEV)
+    first, second = (torch.autograd.grad(loss, leaves, up, retain_graph=True) for _ in range(2))
+    for grads in (first, second):
+        for g, name in zip(grads, ("d_model_out", "d_logit")):
+            w, bound = (t.to(DEV) for t in want[name])
+            w, scale = w * up.double(), float(up.double().abs())
+            # the bound holds what is rounded last relative to the value: it scales with it; two more roundings in fp32; the least numbers
+            over = (g.double().reshape(w.shape) - w).abs() - (bound * scale + 2.02 * R.U * (w.abs() + bound * scale) + 2.0 ** -133)
+            assert float(over.max()) <= 0, (name, float(over.max()))
+    if dtype == torch.bfloat16:
+        assert all(map(torch.equal, first, second))
+
+
+@pytest.mark.parametrize("op", ["pref", "policy"])
+@pytest.mark.parametrize("B,C,T", BOTH)
+def test_upstream_gradients_of_bf16_in_a_graph(op, B, C, T):
+    """Forward and backward captured together, replayed with upstream gradients that are 1 and are not, and with other inputs."""
+    sets = [R.make(op, B, C, T, torch.bfloat16, seed=s, device=DEV) for s in (1, 2)]
+    loss_of = preference_loss if op == "pref" else policy_loss
+
+    def grads(d, up):
+        d = dict(d, model_out=d["model_out"].detach().requires_grad_(), mixing_logit=d["mixing_logit"].detach().requires_grad_())
+        return torch.autograd.grad(loss_of(**d).loss, [d["model_out"], d["mixing_logit"]], up)
+
+    values = (1.0, 3.0, -0.7)
+    want = {(i, v): grads(d, torch.tensor(v, device=DEV)) for i, d in enumerate(sets) for v in values}
+    static = {k: t.clone() if isinstance(t, torch.Tensor) else t for k, t in sets[0].items()}
+    up, graph, side = torch.ones((), device=DEV), torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        grads(static, up)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        got = grads(static, up)
+    for i, v in ((0, 1.0), (0, 3.0), (1, 3.0), (1, 3.0), (0, -0.7), (1, 1.0), (1, -0.7)):
+        for k, t in static.items():
+            if isinstance(t, torch.Tensor):
+                t.copy_(sets[i][k])
+        up.fill_(v)
+        graph.replay()
+        grads(sets[1 - i], up)                        # eager work between the replays
+        torch.cuda.synchronize()
+        assert all(map(torch.equal, got, want[i, v])), (i, v)
+
+
+def test_inputs_changed_before_a_backward_that_reads_them():
+    """bf16 gradients are computed again from the inputs where the upstream gradient is not 1: changed in place, they are refused."""
+    d = R.make("pref", 6, 4, 9, torch.bfloat16, seed=5, device=DEV)
+    loss = preference_loss(**dict(d, model_out=d["model_out"].requires_grad_())).loss
+    d["x_t"].add_(1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
