@@ -13,14 +13,16 @@ clips).  model_out and ref_out are both fp32 or both bf16, everything else is fp
 Gradients are those of first order in reverse mode: a second order, or a forward-mode tangent, raises.
 
 The calls enqueue work on the tensors' device's current stream and nothing else: no synchronisation, and a forward + backward can be captured
-in a hipGraph (the workspace is a torch tensor of the call, so graphs share none) - while no eager loss of the same leaves that was built on
-the default stream lives: that one is refused.
+in a hipGraph (the workspace is a torch tensor of the call, so graphs share none).  A capture is refused while an eager loss lives that was built
+on the default stream over leaves that the captured one differentiates too (a network's parameters among them); other graphs on such leaves
+are the caller's to drop.  A backward that is captured apart from its forward needs the forward on a side stream.
 """
 from __future__ import annotations
 
 import ctypes as C
 import functools
 import math
+import weakref
 from typing import NamedTuple, Optional
 
 import torch
@@ -154,7 +156,10 @@ class LossFn(torch.autograd.Function):
         if not g.is_contiguous():
             g = g.contiguous()
         with _lib.on_device(ctx.index):
-            if ctx.grads is not None and _lib.capture_id(_lib.raw_stream(ctx.index)) == ctx.capture:
+            capture = _lib.capture_id(_lib.raw_stream(ctx.index))
+            if capture not in (0, ctx.capture):      # a backward alone is captured: of a graph that was not looked at when it was built
+                _check_graphs([n for n, _ in ctx.next_functions])
+            if ctx.grads is not None and capture == ctx.capture:
                 (d_out, d_logit, ws), ctx.grads = ctx.grads, None
                 if d_out.dtype == torch.float32:
                     _lib.check(_lib.lib().ddmi_train_loss_scale(g.data_ptr(), d_out.data_ptr(), _lib.DTYPE_F32, d_out.numel(), _p(d_logit),
@@ -178,22 +183,50 @@ class LossFn(torch.autograd.Function):
 
 
 # A leaf's gradient is added on the stream that was current when the first graph on that leaf was built, as long as such a graph lives.  If that
-# is the default stream, a captured backward of the leaf would draw it into the capture, which ends the process: the leaf's node is marked,
-# and a capture that finds the mark is refused before anything is recorded.  The mark goes when the graph does.
-_ON_DEFAULT_STREAM = "ddmi: built on the default stream"
+# is the default stream, a captured backward of the leaf would draw it into the capture, which ends the process.  Python cannot ask a node for
+# its stream, so what these losses see is kept: a leaf that is given to a loss has the first loss's stream noted on its node (gone with the
+# node), and the losses built on the default stream are kept in a weak set, whose graphs a capture walks for the leaves behind a network.  A
+# capture that finds one of its own leaves there is refused before anything is recorded.  Graphs that no loss of this module ends are not seen.
+_FIRST_STREAM = "ddmi: stream of the first loss"
+_DEFAULT = 0
+_on_default_stream = weakref.WeakSet()
+_REFUSED = ("fine-tuning loss: captured while the graph of an eager loss of the same tensors, built on the default stream, lives (or another graph "
+            "that keeps their accumulation nodes since): drop it first, or build it on a side stream")
 
 
-def _mark_leaves(loss, *inputs):
+def _mark_leaves(loss, *inputs, stream=_DEFAULT):
     for t, (node, _) in zip(inputs, loss.grad_fn.next_functions):
         if node is not None and t.is_leaf:
-            node.metadata[_ON_DEFAULT_STREAM] = True
+            node.metadata.setdefault(_FIRST_STREAM, stream)
 
 
 def _check_leaves(*inputs):
-    if any(_ON_DEFAULT_STREAM in torch.autograd.graph.get_gradient_edge(t).node.metadata
+    if any(torch.autograd.graph.get_gradient_edge(t).node.metadata.get(_FIRST_STREAM) == _DEFAULT
            for t in inputs if t is not None and t.requires_grad and t.is_leaf):
-        raise RuntimeError("fine-tuning loss: captured while the graph of an eager loss of the same tensors, built on the default stream, lives: drop "
-                           "that loss first, or run it on a side stream")
+        raise RuntimeError(_REFUSED)
+
+
+def _accumulation_nodes(starts):
+    """The accumulation nodes behind some nodes of a graph, by identity (a node's Python object is one as long as it is held)."""
+    seen, found, todo = {}, {}, [n for n in starts if n is not None]
+    while todo:
+        node = todo.pop()
+        if id(node) in seen:
+            continue
+        seen[id(node)] = node
+        if not node.next_functions and hasattr(node, "variable"):
+            found[id(node)] = node
+        todo += [n for n, _ in node.next_functions if n is not None]
+    return found
+
+
+def _check_graphs(nodes):
+    """Refuses a capture of the graph behind `nodes` that meets one of a living loss on the default stream."""
+    losses = list(_on_default_stream)
+    if losses:
+        old = {k: n for k, n in _accumulation_nodes(losses).items() if n.metadata.get(_FIRST_STREAM, _DEFAULT) == _DEFAULT}
+        if old.keys() & _accumulation_nodes(nodes).keys():
+            raise RuntimeError(_REFUSED)
 
 
 def _loss(entry, model_out, mixing_logit, others, extra, args, stats):
@@ -208,10 +241,12 @@ def _loss(entry, model_out, mixing_logit, others, extra, args, stats):
     capture = _lib.capture_id(stream)
     if capture:
         _check_leaves(model_out, mixing_logit)
+        _check_graphs([torch.autograd.graph.get_gradient_edge(t).node for t in (model_out, mixing_logit) if t is not None and t.requires_grad])
     results, grads = _launch(entry, tensors, extra, args, stats, None, True, mixed)
     loss = LossFn.apply(model_out, mixing_logit, results[:1], grads, (entry, tensors, extra, args, stats, mixed), capture)
-    if not stream:
-        _mark_leaves(loss, model_out, mixing_logit)
+    _mark_leaves(loss, model_out, mixing_logit, stream=stream)
+    if stream == _DEFAULT:
+        _on_default_stream.add(loss.grad_fn)
     return [loss] + results[1:]
 
 

@@ -1,11 +1,13 @@
 """Calls of the fine-tuning operators that are refused, and rules of their plans, without a GPU."""
 import ctypes as C
+import gc
 import math
 import types
 
 import numpy as np
 import pytest
 import torch
+import torch.utils.checkpoint
 from torch.autograd import forward_ad
 
 import finetune_ref as R
@@ -265,3 +267,85 @@ def test_c_loss_again_refuses():
                      (dict(mixing_logit=None, ref_mixing_logit=None), b"d_logit goes"), (dict(dloss=66), b"aligned"), (dict(d_logit=66), b"aligned"),
                      (dict(d_out=65), b"aligned"), (dict(transition=65), b"aligned"), (dict(x_t=66), b"aligned"), (dict(B=0, noise_rows=0), b"empty batch")):
         assert again(**kw) == INVALID and text in c.error(), (kw, c.error())
+
+
+# ---- captures and the graphs that live beside them -------------------------------------------------------------------------------------
+def eager_loss(model_out, mixing_logit=None, stream=0):
+    """A loss's graph node as a call leaves it behind, without a launch."""
+    tensors = tuple(t if t is None else t.detach() for t in (model_out, None, None, None, None, mixing_logit, None, None))
+    loss = finetune.LossFn.apply(model_out, mixing_logit, [torch.zeros(())], None, (None, tensors, (), (), (), False), 0)
+    finetune._mark_leaves(loss, model_out, mixing_logit, stream=stream)
+    if not stream:
+        finetune._on_default_stream.add(loss.grad_fn)
+    return loss
+
+
+def captured(model_out, mixing_logit=None):
+    finetune._check_leaves(model_out, mixing_logit)
+    finetune._check_graphs([torch.autograd.graph.get_gradient_edge(t).node for t in (model_out, mixing_logit) if t is not None and t.requires_grad])
+
+
+def leaf():
+    return torch.ones(2, 3, requires_grad=True)
+
+
+@pytest.mark.parametrize("behind", [lambda w, b: (w * 2 + b) @ torch.ones(3, 3), lambda w, b: torch.utils.checkpoint.checkpoint(torch.mul, w, b, use_reentrant=False)],
+                         ids=["network", "checkpointed"])
+def test_a_capture_sees_the_parameters_behind_a_network(behind):
+    w, b, other = leaf(), leaf(), leaf()
+    loss = eager_loss(behind(w, b))                   # without a mixing logit: no leaf is an input of the loss
+    with pytest.raises(RuntimeError, match="captured while"):
+        captured(w.exp())
+    with pytest.raises(RuntimeError, match="captured while"):
+        captured(other * 2, b)
+    captured(other * 2)
+    captured(w.detach(), other)
+    held = loss * 3                                   # whatever keeps its graph keeps the loss
+    del loss
+    gc.collect()
+    with pytest.raises(RuntimeError, match="captured while"):
+        captured(w)
+    del held
+    gc.collect()
+    captured(w.exp() + b)
+
+
+def test_a_leaf_that_a_side_stream_saw_first_may_be_captured():
+    """The node is that of the first graph: a loss on the default stream that joins it later does not move it, also once it is gone."""
+    w = leaf()
+    first = eager_loss(w, stream=7)
+    second = eager_loss(w)
+    captured(w)
+    del second
+    gc.collect()
+    captured(w)
+    del first
+    gc.collect()
+    last = eager_loss(w)
+    with pytest.raises(RuntimeError, match="captured while"):
+        captured(w)
+    del last
+    gc.collect()
+    captured(w)
+
+
+def test_a_leaf_that_the_default_stream_saw_first_stays_refused_while_its_node_lives():
+    w = leaf()
+    first, second = eager_loss(w), eager_loss(w, stream=7)
+    del first
+    gc.collect()
+    with pytest.raises(RuntimeError, match="captured while"):
+        captured(w)
+    del second
+    gc.collect()
+    captured(w)
+
+
+def test_losses_on_the_default_stream_are_not_kept_alive():
+    before = len(finetune._on_default_stream)
+    w = leaf()
+    losses = [eager_loss(w * k) for k in range(3)]
+    assert len(finetune._on_default_stream) == before + 3
+    del losses
+    gc.collect()
+    assert len(finetune._on_default_stream) == before

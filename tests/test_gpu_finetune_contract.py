@@ -1,4 +1,5 @@
 """What the fine-tuning operators promise at the edges of their arguments, on the GPU."""
+import gc
 import math
 
 import pytest
@@ -144,3 +145,36 @@ def test_inputs_changed_before_a_backward_that_reads_them():
     d["x_t"].add_(1)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         loss.backward()
+
+
+# ---- captures ------------------------------------------------------------------------------------------------------------------------------
+def test_capture_refused_over_parameters_of_a_living_eager_loss():
+    """The parameters lie behind the network's output and there is no mixing logit; once the eager loss is gone, the capture runs."""
+    d = R.make("pref", 6, 7, 131, mixed=False, device=DEV)
+    w = torch.full((7, 1), 0.5, device=DEV, requires_grad=True)
+    base = d["model_out"]
+
+    def grad():
+        return torch.autograd.grad(preference_loss(**dict(d, model_out=base * w)).loss, w)[0]
+
+    eager = preference_loss(**dict(d, model_out=base * w))
+    refused, graph = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    other = torch.zeros(1, device=DEV)
+    with torch.cuda.graph(refused):
+        with pytest.raises(RuntimeError, match="captured while the graph of an eager loss"):
+            preference_loss(**dict(d, model_out=base * w))
+        other.add_(1)
+    del eager
+    gc.collect()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        want = grad()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        got = grad()
+    for _ in range(3):
+        graph.replay()
+        eager = preference_loss(**dict(d, model_out=base.clone().requires_grad_())).loss      # eager work of other leaves
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
