@@ -199,6 +199,7 @@ SYMBOLS = {
     "ddmi_train_loss_again": (_I, [C.POINTER(LossIn), _I, _I, _VP, _VP, _VP, C.c_size_t, _VP, _VP, _VP]),
     "ddmi_stream_capture_id": (_I, [_VP, C.POINTER(C.c_uint64)]),
     "ddmi_debug_loss_polls": (_I, [_I]),
+    "ddmi_debug_loss_plan": (_I, [_I, _I, C.c_int64, _I, _I, _I, _I, C.POINTER(_I), C.POINTER(_I)]),
     "ddmi_train_adamw_multi": (_I, [_VP, _I, C.c_double, C.c_double, C.c_double, C.c_double, C.c_uint32, _I, _I, _I, _VP]),
 }
 

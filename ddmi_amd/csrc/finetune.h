@@ -38,13 +38,17 @@ struct FtArgs {
   // workspace
   double* total;             // sum of the weights
   int* done;                 // one pass: whether a span's gradient is written
+  int* late;                 // one pass: whether a workgroup has waited in vain
   float2* coef;              // a sample: factors of the residual and of the step away from the reference
   double* term;
   double2* part;             // a workgroup of sums_kernel
   double2* chan;             // a (sample, channel, segment, wave): sums the mixing logit's gradient needs
 };
-// rows_of: samples whose sums meet (2: a pair); keep: vectors a thread may keep for one pass over the inputs, 0: two passes
-int ft_plan(FtArgs* a, int B, int C, int64_t HW, bool mixed, int rows_of, int keep);
+// rows_of: samples whose sums meet (2: a pair); keep: vectors a thread may keep for one pass over the inputs, 0: two passes; units: compute units
+// of the card, FT_ANY_CARD: one pass wherever a card of some size would take it (to size a workspace)
+#define FT_ANY_CARD -1
+int ft_plan(FtArgs* a, int B, int C, int64_t HW, bool mixed, int rows_of, int keep, int units);
+int ft_units();              // of the current device, 0 where there is none
 size_t ft_workspace_bytes(const FtArgs& a);
 void ft_carve(FtArgs* a, void* ws);
 void ft_set_polls(int n);

@@ -25,7 +25,7 @@ int common_args(FtArgs* a, const ddmi_loss_in* in, int B, int rows_of, int keep,
                    aligned({in->x_t, in->second, in->sqrt_1mac, in->mixing_logit, in->ref_mixing_logit, in->weight}, 4),
                "fine-tuning loss: inputs aligned to their values");
   DDMI_REQUIRE((double)in->C * (double)in->HW < 1.1e12, "fine-tuning loss: sample too large");
-  DDMI_TRY(ft_plan(a, B, in->C, in->HW, in->mixing_logit != nullptr, rows_of, keep));
+  DDMI_TRY(ft_plan(a, B, in->C, in->HW, in->mixing_logit != nullptr, rows_of, keep, ft_units()));
   DDMI_REQUIRE(ws && ((uintptr_t)ws & 15) == 0 && ws_bytes >= ft_workspace_bytes(*a), "fine-tuning loss: workspace too small or not 16-byte aligned");
   ft_carve(a, ws);
   a->out = in->model_out; a->ref = in->ref_out; a->x = in->x_t; a->second = in->second; a->s1 = in->mixing_logit ? in->sqrt_1mac : nullptr;
@@ -46,9 +46,9 @@ int ddmi_train_loss_workspace_bytes(int B, int C, int64_t HW, int mixed, size_t*
   DDMI_REQUIRE(bytes && B > 0 && C > 0 && HW > 0 && (double)C * (double)HW < 1.1e12, "train_loss_workspace_bytes: bad arguments");
   *bytes = 0;
   for (int rows_of = 1; rows_of <= 2; ++rows_of)
-    for (int keep : {0, FT_VECS / 2, FT_VECS}) {      // whichever loss the call is, with or without its gradient
+    for (int keep : {0, FT_VECS / 2, FT_VECS}) {      // whichever loss the call is, with or without its gradient, on whichever card
       FtArgs a{};
-      DDMI_TRY(ft_plan(&a, B, C, HW, mixed != 0, rows_of, keep));
+      DDMI_TRY(ft_plan(&a, B, C, HW, mixed != 0, rows_of, keep, FT_ANY_CARD));
       *bytes = std::max(*bytes, ft_workspace_bytes(a));
     }
   return DDMI_OK;
@@ -116,6 +116,14 @@ int ddmi_stream_capture_id(void* stream, uint64_t* id) {
   unsigned long long n = 0;
   HIP_TRY(hipStreamGetCaptureInfo((hipStream_t)stream, &status, &n));
   if (status == hipStreamCaptureStatusActive) *id = n;
+  return DDMI_OK;
+}
+int ddmi_debug_loss_plan(int B, int C, int64_t HW, int mixed, int policy, int has_ref, int units, int* one_pass, int* spans) {
+  DDMI_REQUIRE(one_pass && spans && B > 0 && C > 0 && HW > 0 && (double)C * (double)HW < 1.1e12 && units >= 0, "debug_loss_plan: bad arguments");
+  FtArgs a{};
+  DDMI_TRY(ft_plan(&a, B, C, HW, mixed != 0, policy ? 1 : 2, policy && has_ref ? FT_VECS / 2 : FT_VECS, units));
+  *one_pass = a.fused;
+  *spans = a.wps;
   return DDMI_OK;
 }
 int ddmi_debug_loss_polls(int n) {

@@ -12,6 +12,7 @@
 // Factors are rounded in fp32, products and sums are held in fp64: a margin is the difference of two nearly equal errors times
 // beta ~ 10^3, and a logit's gradient a sum of either sign over the batch.  No float atomics: every sum has a fixed order.
 #include <algorithm>
+#include <atomic>
 #include "kernels.h"
 #include "finetune.h"
 #include "prof.h"
@@ -240,7 +241,8 @@ __device__ __forceinline__ RowOut policy_row(const FtArgs& a, bool used, double 
   return o;
 }
 constexpr unsigned long long FT_OPEN = 0xFFFFFFFFFFFFFFFFull;   // a sum that is not there yet (one pass, below); no sum is stored as this NaN
-// the sums of one sample, by one wave: lane i adds those of spans i, i + 64 ...; false when one did not show up within `polls` looks
+// the sums of one sample, by one wave: lane i adds those of spans i, i + 64 ...; false when one did not show up within `polls` looks, or
+// where another workgroup has waited in vain already (what holds the compute units holds them for all: the whole call waits once)
 __device__ __forceinline__ bool wave_sums(const FtArgs& a, int64_t first, int& polls, double2& out) {
   unsigned long long* p = reinterpret_cast<unsigned long long*>(a.part + first);
   double u = 0.0, v = 0.0;
@@ -248,12 +250,13 @@ __device__ __forceinline__ bool wave_sums(const FtArgs& a, int64_t first, int& p
     const int j = j0 + (threadIdx.x & 63);
     unsigned long long x = 0, y = 0;
     for (;;) {
+      const int late = __hip_atomic_load(a.late, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);      // in flight with the sums
       if (j < a.wps) {
         x = __hip_atomic_load(p + 2 * j, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
         y = __hip_atomic_load(p + 2 * j + 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
       }
       if (__all(x != FT_OPEN && y != FT_OPEN)) break;
-      if (--polls < 0) return false;
+      if (--polls < 0 || __any(late)) return false;
       __builtin_amdgcn_s_sleep(8);
     }
     u += __longlong_as_double((long long)x);
@@ -326,15 +329,17 @@ __global__ void __launch_bounds__(FT_THREADS) loss_kernel(FtArgs a, int rows) {
 // A workgroup reads its span, adds up, publishes its two sums, waits for those of the pair's (transition's) other spans and writes the
 // gradient from the residuals in its registers: every input is read once.  The sums' own bits are the signal - open_kernel fills their
 // places with a NaN that no sum is stored as - so publishing is two relaxed agent-scope stores, with no fence and no counter.  The wait is
-// bounded: a workgroup whose neighbours do not show up (other kernels hold the compute units) leaves its span undone, and grad_kernel,
-// which runs after it in any case (loss and logits' gradients need every sample), computes what is not done.
-int g_polls = 1 << 12;                  // some milliseconds; the spans of a row start within microseconds of each other
+// bounded: a workgroup whose neighbours do not show up (other kernels hold the compute units) leaves its span undone, as then do all that
+// would have to wait after it, and grad_kernel, which runs after it in any case (loss and logits' gradients need every sample), computes what
+// is not done.
+std::atomic<int> g_polls{1 << 12};      // some milliseconds; the spans of a row start within microseconds of each other
 
 template <int MODE>
 __global__ void __launch_bounds__(FT_THREADS) open_kernel(FtArgs a, int64_t places) {
   __shared__ double red[FT_THREADS / 64];
   unsigned long long* p = reinterpret_cast<unsigned long long*>(a.part);
   for (int64_t i = (int64_t)blockIdx.x * FT_THREADS + threadIdx.x; i < places; i += (int64_t)gridDim.x * FT_THREADS) p[i] = FT_OPEN;
+  if (blockIdx.x == 0 && threadIdx.x == 0) *a.late = 0;
   if (blockIdx.x == 0) total_weight<MODE>(a, red);
 }
 __device__ __forceinline__ void publish(double* place, double v) {
@@ -471,6 +476,7 @@ __global__ void __launch_bounds__(FT_THREADS, 2) fused_kernel(FtArgs a) {
       factor = make_float2(k.x * up, k.y * up);
       whole = ok;
       a.done[blockIdx.x] = ok;
+      if (!ok) __hip_atomic_store(a.late, 1, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
     }
   }
   __syncthreads();
@@ -593,7 +599,7 @@ int launch_sums_t(const FtArgs& a, int dt, hipStream_t s) {
     constexpr int NV = (MODE == FT_POLICY && REF) ? FT_VECS / 2 : FT_VECS;
     const int64_t places = 2ll * a.B * a.wps;
     FtArgs f = a;
-    f.polls = g_polls;
+    f.polls = g_polls.load(std::memory_order_relaxed);
     hipLaunchKernelGGL((open_kernel<MODE>), dim3((unsigned)std::min<int64_t>(cdiv64(places, FT_THREADS), 256)), dim3(FT_THREADS), 0, s, a, places);
     if (dt == DT_F32) hipLaunchKernelGGL((fused_kernel<MODE, MIX, REF, float, NV>), grid, dim3(FT_THREADS), 0, s, f);
     else hipLaunchKernelGGL((fused_kernel<MODE, MIX, REF, bf16_t, NV>), grid, dim3(FT_THREADS), 0, s, f);
@@ -653,7 +659,17 @@ static void ft_split(FtArgs* a, int64_t want) {
   a->log_g = 0;
   while (a->log_g < 8 && (((int64_t)16 << a->log_g) <= std::min(a->seg, a->T) || (FT_THREADS >> a->log_g) > a->rows_per_wg)) ++a->log_g;
 }
-int ft_plan(FtArgs* a, int B, int C, int64_t HW, bool mixed, int rows_of, int keep) {
+int ft_units() {
+  static std::atomic<int> known[64];                    // a device's, plus one; asked once
+  int dev = 0, units = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 0;
+  if ((units = known[dev].load(std::memory_order_relaxed)) == 0) {
+    if (hipDeviceGetAttribute(&units, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess) return 0;
+    known[dev].store(++units, std::memory_order_relaxed);
+  }
+  return units - 1;
+}
+int ft_plan(FtArgs* a, int B, int C, int64_t HW, bool mixed, int rows_of, int keep, int units) {
   a->B = B;
   a->C = mixed ? C : 1;                       // without a logit nothing depends on the channel: a sample is one row
   a->T = mixed ? HW : HW * C;
@@ -665,11 +681,13 @@ int ft_plan(FtArgs* a, int B, int C, int64_t HW, bool mixed, int rows_of, int ke
     const int64_t turns = cdiv64(cdiv64(std::min(a->seg, a->T), 4), 1ll << a->log_g), groups = FT_THREADS >> a->log_g;
     a->rows_per_wg = (int)std::max<int64_t>(1, std::min<int64_t>(a->rows_per_wg, keep / std::max<int64_t>(turns, 1) * groups));
     const int64_t wps = cdiv64(a->C, a->rows_per_wg) * a->nseg;
-    // One pass pays from 384 workgroups on, one and a half for each compute unit (64 x 64 x 64 latents, two passes | one: 8 pairs 40 | 48 us,
-    // 12: 52 | 50, 16: 65 | 53, 256: 680 | 477; transitions with KL 8: 33 | 39, 12: 43 | 41, 512: 894 | 533).  The spans that wait for each
-    // other are resident together with room to spare (two workgroups a compute unit), and the threads' registers are mostly in use.
+    // One pass pays from one and a half workgroups a compute unit on, 384 on the whole card's 256 (64 x 64 x 64 latents, two passes | one:
+    // 8 pairs 40 | 48 us, 12: 52 | 50, 16: 65 | 53, 256: 680 | 477; transitions with KL 8: 33 | 39, 12: 43 | 41, 512: 894 | 533).  The spans that
+    // wait for each other are at most as many as the compute units, each of which holds two: they are resident together with room to spare.  The
+    // units are those of the card as it is partitioned.  And the threads' registers are mostly in use.
     const double filled = (double)a->rows_per_wg * (double)std::min(a->seg, a->T) / (1024.0 * keep);
-    a->fused = wps * B >= 384 && wps * rows_of <= 256 && turns <= keep && filled >= 0.5;
+    const bool room = units == FT_ANY_CARD || (units > 0 && 2 * wps * B >= 3 * (int64_t)units && wps * rows_of <= units);
+    a->fused = room && turns <= keep && filled >= 0.5;
   }
   if (!a->fused) {
     int64_t want = 8192;
@@ -681,7 +699,7 @@ int ft_plan(FtArgs* a, int B, int C, int64_t HW, bool mixed, int rows_of, int ke
   a->wps = (int)wps;
   return DDMI_OK;
 }
-void ft_set_polls(int n) { g_polls = n; }
+void ft_set_polls(int n) { g_polls.store(n, std::memory_order_relaxed); }
 static size_t up256(size_t b) { return (b + 255) & ~(size_t)255; }
 size_t ft_workspace_bytes(const FtArgs& a) {
   const int wpg = a.log_g > 6 ? 1 << (a.log_g - 6) : 1;
@@ -690,7 +708,7 @@ size_t ft_workspace_bytes(const FtArgs& a) {
 }
 void ft_carve(FtArgs* a, void* ws) {
   unsigned char* p = (unsigned char*)ws;
-  a->total = (double*)p; p += 256;
+  a->total = (double*)p; a->late = (int*)(p + 128); p += 256;
   a->coef = (float2*)p; p += up256((size_t)a->B * sizeof(float2));
   a->term = (double*)p; p += up256((size_t)a->B * sizeof(double));
   a->part = (double2*)p; p += up256((size_t)a->B * a->wps * sizeof(double2));

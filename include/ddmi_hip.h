@@ -552,6 +552,9 @@ int ddmi_stream_capture_id(void* stream, uint64_t* id);
 /* how often a workgroup of a loss's one-pass form looks for its neighbours' sums before it leaves its part to the kernel after it (4096
  * by default; 0: one look - the results are the same bits) */
 int ddmi_debug_loss_polls(int n);
+/* host-only: whether a loss call with its gradient reads its inputs once on a card of `units` compute units, and how many workgroups share a
+ * sample then (policy: 0 = the preference loss of B samples; has_ref: whether a policy loss has ref_out) */
+int ddmi_debug_loss_plan(int B, int C, int64_t HW, int mixed, int policy, int has_ref, int units, int* one_pass, int* spans);
 /* One tensor of an AdamW step.  Moments in 32 bits: exp_avg, exp_avg_sq fp32 [numel].  In 8 bits: e4m3 codes [numel] of the first moment
  * and of the ROOT of the second, one fp32 power-of-two scale for each 256 values (exp_avg_scale, exp_avg_sq_scale [ceil(numel / 256)]). */
 typedef struct {

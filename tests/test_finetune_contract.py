@@ -349,3 +349,48 @@ def test_losses_on_the_default_stream_are_not_kept_alive():
     del losses
     gc.collect()
     assert len(finetune._on_default_stream) == before
+
+
+# ---- the one-pass form and the card ----------------------------------------------------------------------------------------------------
+def plan(B, channels, hw, mixed, policy, has_ref, units):
+    one, spans = C.c_int(-1), C.c_int(-1)
+    assert _lib.lib().ddmi_debug_loss_plan(B, channels, hw, mixed, policy, has_ref, units, C.byref(one), C.byref(spans)) == 0
+    return one.value, spans.value
+
+
+@pytest.mark.parametrize("policy,has_ref", [(0, 1), (1, 0), (1, 1)])
+@pytest.mark.parametrize("mixed", [0, 1])
+def test_workgroups_that_wait_for_each_other_fit_the_card(policy, has_ref, mixed):
+    """On a card of any number of compute units: those of a sample (a pair) are no more than the units, which hold two workgroups each, and
+    the launch has one and a half for each."""
+    rows_of = 1 if policy else 2
+    taken = {}
+    for units in (0, 1, 8, 32, 64, 128, 256, 304):
+        taken[units] = 0
+        for B in (2, 8, 48, 140, 512, 4096):
+            for channels in (1, 3, 64, 190, 1100):
+                for hw in (1, 77, 1295, 2048, 4096, 33001, 1 << 20, 1 << 24):
+                    if B * channels * hw > 1 << 36:           # more than any card holds: refused
+                        continue
+                    one, spans = plan(B, channels, hw, mixed, policy, has_ref, units)
+                    taken[units] += one
+                    if one:
+                        assert spans * rows_of <= units and spans * B >= 1.5 * units, (units, B, channels, hw)
+    assert taken[0] == 0 and all(taken[u] > 0 for u in (8, 32, 64, 128, 256)), taken
+
+
+def test_smaller_cards_take_smaller_batches_in_one_pass():
+    """64 x 64 x 64 latents, 16 (with KL: 32) spans a sample: 12 pairs fill the whole card, a few fill an eighth of it; 32 spans of a pair do
+    not fit sixteen units."""
+    assert plan(24, 64, 4096, 1, 0, 1, 256) == (1, 16) and plan(16, 64, 4096, 1, 0, 1, 256)[0] == 0
+    assert plan(4, 64, 4096, 1, 0, 1, 32) == (1, 16) and plan(2, 64, 4096, 1, 0, 1, 32)[0] == 0
+    assert plan(512, 64, 4096, 1, 0, 1, 16)[0] == 0 and plan(512, 64, 4096, 1, 1, 1, 32) == (1, 32)
+
+
+def test_workspace_covers_every_card():
+    """What a call needs does not depend on the card: a plan of one pass on some card has its room."""
+    size = C.c_size_t(0)
+    for B, channels, hw in ((48, 64, 2048), (4, 64, 4096), (2, 64, 4096)):
+        assert _lib.lib().ddmi_train_loss_workspace_bytes(B, channels, hw, 1, C.byref(size)) == 0
+        most = max(plan(B, channels, hw, 1, 0, 1, u)[1] for u in (0, 8, 32, 256))
+        assert size.value >= 256 + B * most * (16 + 4)

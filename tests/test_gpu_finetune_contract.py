@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import finetune_ref as R
+from ddmi_amd import _lib
 from ddmi_amd.finetune import policy_loss, preference_loss, transition_log_prob
 from test_gpu_finetune import DEV, SHAPES, call, reference
 
@@ -178,3 +179,22 @@ def test_capture_refused_over_parameters_of_a_living_eager_loss():
         eager = preference_loss(**dict(d, model_out=base.clone().requires_grad_())).loss      # eager work of other leaves
         torch.cuda.synchronize()
         assert torch.equal(got, want)
+
+
+# ---- waits that end early ------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("op", ["pref", "policy"])
+@pytest.mark.parametrize("polls", [1, 3, 20])
+@pytest.mark.parametrize("B,C,T", [(48, 64, 2048), (140, 3, 33001)])
+def test_workgroups_that_stop_waiting_leave_the_same_bits(op, polls, B, C, T):
+    """Some find their neighbours' sums, one does not, and those after it look once: whoever computes a span, it is the same."""
+    d = R.make(op, B, C, T, seed=8, device=DEV)
+    want = call(op, d)
+    try:
+        _lib.check(_lib.lib().ddmi_debug_loss_polls(polls))
+        got = [call(op, d) for _ in range(3)]
+    finally:
+        _lib.check(_lib.lib().ddmi_debug_loss_polls(4096))
+    got.append(call(op, d))                           # the next call waits again: the mark is that of a call
+    for g in got:
+        for k in want:
+            assert torch.equal(want[k], g[k]), k
