@@ -289,7 +289,7 @@ def refuse_tangents(who: str, *tensors) -> None:
     """Raises where a tensor carries a forward-mode derivative: the kernels go by its pointer, which would drop the tangent in silence (a
     dual tensor does not require a gradient)."""
     from torch.autograd import forward_ad
-    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise NotImplementedError(f"{who}: forward-mode derivatives are not offered")
 
 

@@ -26,6 +26,7 @@ import weakref
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import _lib
@@ -111,10 +112,10 @@ def _flat(t):
 
 
 def _launch(entry, tensors, extra, args, stats, g, grads, mixed):
-    """One call of a loss's C entry point: ((loss, *statistics), (d_model_out, d_logit, its workspace if
-    gradients may be asked of it again)).  tensors: model_out, ref_out, x_t, noise / x_prev,
-    sqrt_1mac, mixing_logit, ref_mixing_logit, weight - contiguous; extra: the tensors, args: the numbers behind them; stats: rows of each
-    statistic; g: the upstream gradient (None: 1); grads, mixed: whether the output's / the logit's gradient is wanted."""
+    """One call of a loss's C entry point: ((loss, *statistics), (d_model_out, d_logit, what it takes to ask for them again)).  tensors:
+    model_out, ref_out, x_t, noise / x_prev, sqrt_1mac, mixing_logit, ref_mixing_logit, weight - contiguous; extra: the tensors, args: the
+    numbers behind them; stats: rows of each statistic; g: the upstream gradient (None: 1); grads, mixed: whether the output's / the logit's
+    gradient is wanted."""
     out, logit = tensors[0], tensors[5]
     B, Cc, dev = out.shape[0], out.shape[1], out.device
     HW = out.numel() // (B * Cc)
@@ -122,14 +123,14 @@ def _launch(entry, tensors, extra, args, stats, g, grads, mixed):
     d_logit = torch.empty_like(logit) if mixed else None
     results = [torch.empty((), dtype=torch.float32, device=dev)] + [torch.empty((n,), dtype=torch.float32, device=dev) for n in stats]
     ws = torch.empty(_workspace_bytes(B, Cc, HW, logit is not None), dtype=torch.uint8, device=dev)
-    _lib.check(entry(C.byref(_given(tensors)), *args[0], *map(_p, extra), *args[1], _p(g), ws.data_ptr(), ws.numel(), *map(_p, results), _p(d_out),
-                     _p(d_logit), _lib.raw_stream(out.get_device())))
-    return results, (d_out, d_logit, None if out.dtype == torch.float32 else ws)
-
-
-def _given(tensors):
-    out = tensors[0]
-    return _lib.LossIn(*map(_p, tensors), out.numel() // (out.shape[0] * out.shape[1]), out.shape[1], _OUT_TYPES[out.dtype])
+    given = _lib.LossIn(*map(_p, tensors), HW, Cc, _OUT_TYPES[out.dtype])
+    at = list(map(_p, extra))
+    _lib.check(entry(C.byref(given), *args[0], *at, *args[1], _p(g), ws.data_ptr(), ws.numel(), *map(_p, results), _p(d_out), _p(d_logit),
+                     _lib.raw_stream(out.get_device())))
+    again = None
+    if grads and out.dtype != torch.float32:      # (the noise's rows are the preference loss's, the transition is the policy loss's)
+        again = (C.byref(given), B, tensors[3].shape[0], at[0] if at else None), (ws.data_ptr(), ws.numel()), ws
+    return results, (d_out, d_logit, again)
 
 
 class LossFn(torch.autograd.Function):
@@ -145,6 +146,8 @@ class LossFn(torch.autograd.Function):
         ctx.beside = {i: t for i, t in enumerate(saved) if t is not None and t.is_inference()}      # autograd does not save these itself
         ctx.save_for_backward(*(saved if not ctx.beside else [None if i in ctx.beside else t for i, t in enumerate(saved)]))
         ctx.grads, ctx.again, ctx.index, ctx.capture = grads, (entry, rest), model_out.get_device(), capture
+        if grads and grads[2] and torch._C._autograd._top_saved_tensors_default_hooks(False):
+            ctx.grads = None      # a hook moves the inputs that these would be computed again from: as for a later backward then
         return loss[0]
 
     @staticmethod
@@ -156,28 +159,24 @@ class LossFn(torch.autograd.Function):
         if not g.is_contiguous():
             g = g.contiguous()
         with _lib.on_device(ctx.index):
-            capture = _lib.capture_id(_lib.raw_stream(ctx.index))
+            stream = _lib.raw_stream(ctx.index)
+            capture = _lib.capture_id(stream)
             if capture not in (0, ctx.capture):      # a backward alone is captured: of a graph that was not looked at when it was built
                 _check_graphs([n for n, _ in ctx.next_functions])
             if ctx.grads is not None and capture == ctx.capture:
-                (d_out, d_logit, ws), ctx.grads = ctx.grads, None
+                (d_out, d_logit, again), ctx.grads = ctx.grads, None
                 if d_out.dtype == torch.float32:
                     _lib.check(_lib.lib().ddmi_train_loss_scale(g.data_ptr(), d_out.data_ptr(), _lib.DTYPE_F32, d_out.numel(), _p(d_logit),
-                                                                0 if d_logit is None else d_logit.numel(), _lib.raw_stream(ctx.index)))
+                                                                0 if d_logit is None else d_logit.numel(), stream))
                 else:
-                    saved = LossFn._saved(ctx)
-                    noise_rows = saved[3].shape[0]      # not read of the policy loss, which has a transition
-                    _lib.check(_lib.lib().ddmi_train_loss_again(C.byref(_given(saved[:8])), d_out.shape[0], noise_rows, _p(saved[8]) if saved[8:] else None,
-                                                                g.data_ptr(), ws.data_ptr(), ws.numel(), d_out.data_ptr(), _p(d_logit),
-                                                                _lib.raw_stream(ctx.index)))
+                    ctx.saved_tensors      # the inputs are read where the forward had them: raises where one was changed since
+                    inputs, workspace, _ = again
+                    _lib.check(_lib.lib().ddmi_train_loss_again(*inputs, g.data_ptr(), *workspace, d_out.data_ptr(), _p(d_logit), stream))
             else:
-                saved, (entry, (args, stats, mixed)) = LossFn._saved(ctx), ctx.again
+                saved, (entry, (args, stats, mixed)) = ctx.saved_tensors, ctx.again
+                saved = tuple(ctx.beside.get(i, t) for i, t in enumerate(saved))
                 d_out, d_logit, _ = _launch(entry, saved[:8], saved[8:], args, stats, g, True, mixed)[1]
         return d_out, d_logit, None, None, None, None
-
-    @staticmethod
-    def _saved(ctx):
-        return [ctx.beside.get(i, t) for i, t in enumerate(ctx.saved_tensors)]
 
     _with_graph = staticmethod(once_differentiable(_gradients.__func__))      # create_graph: a second derivative through here raises
 
@@ -185,11 +184,32 @@ class LossFn(torch.autograd.Function):
 # A leaf's gradient is added on the stream that was current when the first graph on that leaf was built, as long as such a graph lives.  If that
 # is the default stream, a captured backward of the leaf would draw it into the capture, which ends the process.  Python cannot ask a node for
 # its stream, so what these losses see is kept: a leaf that is given to a loss has the first loss's stream noted on its node (gone with the
-# node), and the losses built on the default stream are kept in a weak set, whose graphs a capture walks for the leaves behind a network.  A
+# node), and the losses built on the default stream are known while they live, and a capture walks their graphs for the leaves behind a network.  A
 # capture that finds one of its own leaves there is refused before anything is recorded.  Graphs that no loss of this module ends are not seen.
 _FIRST_STREAM = "ddmi: stream of the first loss"
 _DEFAULT = 0
-_on_default_stream = weakref.WeakSet()
+
+
+class _Living:
+    """Objects for as long as something else holds them; adding one costs an append, the dead are swept out now and then."""
+
+    def __init__(self):
+        self.refs, self.sweep = [], 64
+
+    def add(self, node):
+        self.refs.append(weakref.ref(node))
+        if len(self.refs) > self.sweep:
+            self.refs = [r for r in self.refs if r() is not None]
+            self.sweep = max(64, 2 * len(self.refs))
+
+    def __iter__(self):
+        return iter([n for n in (r() for r in self.refs) if n is not None])
+
+    def __len__(self):
+        return len(list(iter(self)))
+
+
+_on_default_stream = _Living()
 _REFUSED = ("fine-tuning loss: captured while the graph of an eager loss of the same tensors, built on the default stream, lives (or another graph "
             "that keeps their accumulation nodes since): drop it first, or build it on a side stream")
 
@@ -277,7 +297,8 @@ def preference_loss(model_out, ref_out, x_t, noise, sqrt_1mac, beta, mixing_logi
     if not math.isfinite(beta) or not 0.0 <= label_smoothing <= 1.0:
         raise ValueError(f"{who}: beta is finite and label_smoothing in [0, 1], got {beta}, {label_smoothing}")
     _check_constants(who, ref_out=ref_out, x_t=x_t, noise=noise, sqrt_1mac=sqrt_1mac, ref_mixing_logit=ref_mixing_logit, weight=weight)
-    _lib.refuse_tangents(who, model_out, ref_out, x_t, noise, sqrt_1mac, mixing_logit, ref_mixing_logit, weight)
+    if forward_ad._current_level >= 0:
+        _lib.refuse_tangents(who, model_out, ref_out, x_t, noise, sqrt_1mac, mixing_logit, ref_mixing_logit, weight)
     dev = _check_device(who, model_out, ref_out, x_t, noise, sqrt_1mac, mixing_logit, ref_mixing_logit, weight)
     with _lib.on_device(dev):
         _lib.init_device(dev)
@@ -315,7 +336,8 @@ def policy_loss(model_out, x_t, x_prev, transition, sqrt_1mac, logp_old, advanta
         raise ValueError(f"{who}: kl_coef without ref_out, the reference network's output")
     _check_constants(who, ref_out=ref_out, x_t=x_t, x_prev=x_prev, transition=transition, sqrt_1mac=sqrt_1mac, logp_old=logp_old, advantage=advantage,
                      ref_mixing_logit=ref_mixing_logit, weight=weight)
-    _lib.refuse_tangents(who, model_out, ref_out, x_t, x_prev, transition, sqrt_1mac, logp_old, advantage, mixing_logit, ref_mixing_logit, weight)
+    if forward_ad._current_level >= 0:
+        _lib.refuse_tangents(who, model_out, ref_out, x_t, x_prev, transition, sqrt_1mac, logp_old, advantage, mixing_logit, ref_mixing_logit, weight)
     dev = _check_device(who, model_out, ref_out, x_t, x_prev, transition, sqrt_1mac, logp_old, advantage, mixing_logit, ref_mixing_logit, weight)
     with _lib.on_device(dev):
         _lib.init_device(dev)
@@ -330,7 +352,8 @@ def transition_log_prob(model_out, x_t, x_prev, transition, sqrt_1mac, mixing_lo
     who = "transition_log_prob"
     _check_outputs(who, model_out, None, x_t, sqrt_1mac, mixing_logit, None)
     _check_transition(who, model_out, x_prev, transition, weight)
-    _lib.refuse_tangents(who, model_out, x_t, x_prev, transition, sqrt_1mac, mixing_logit, weight)
+    if forward_ad._current_level >= 0:
+        _lib.refuse_tangents(who, model_out, x_t, x_prev, transition, sqrt_1mac, mixing_logit, weight)
     dev = _check_device(who, model_out, x_t, x_prev, transition, sqrt_1mac, mixing_logit, weight)
     with _lib.on_device(dev):
         _lib.init_device(dev)
@@ -340,6 +363,7 @@ def transition_log_prob(model_out, x_t, x_prev, transition, sqrt_1mac, mixing_lo
         transition = _flat(transition)
         logp = torch.empty((B,), dtype=torch.float32, device=model_out.device)
         ws = torch.empty(_workspace_bytes(B, Cc, HW, mixing_logit is not None), dtype=torch.uint8, device=model_out.device)
-        _lib.check(_lib.lib().ddmi_train_policy_loss(C.byref(_given(tensors)), B, transition.data_ptr(), None, None, 0.0, 0.0, None, ws.data_ptr(), ws.numel(), None,
+        given = _lib.LossIn(*map(_p, tensors), HW, Cc, _OUT_TYPES[model_out.dtype])
+        _lib.check(_lib.lib().ddmi_train_policy_loss(C.byref(given), B, transition.data_ptr(), None, None, 0.0, 0.0, None, ws.data_ptr(), ws.numel(), None,
                                                      logp.data_ptr(), None, None, None, None, _lib.raw_stream(dev)))
         return logp

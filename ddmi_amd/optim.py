@@ -15,6 +15,7 @@ from typing import Dict, List, Optional, Sequence, Union
 
 import numpy as np
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -101,7 +102,8 @@ def adamw_step(params: Sequence[torch.Tensor], grads: Sequence[torch.Tensor], ex
     b1, b2 = float(betas[0]), float(betas[1])
     if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and eps >= 0.0):
         raise ValueError(f"{who}: betas in [0, 1) and eps >= 0, got {betas}, {eps}")
-    _lib.refuse_tangents(who, *flat)
+    if forward_ad._current_level >= 0:
+        _lib.refuse_tangents(who, *flat)
     dev = params[0].get_device()
     if dev < 0 or not params[0].is_cuda or set(map(_DEVICE, flat)) != {dev}:
         raise ValueError(f"{who}: all tensors live on one GPU, got {sorted({str(t.device) for t in flat})}")

@@ -394,3 +394,12 @@ def test_workspace_covers_every_card():
         assert _lib.lib().ddmi_train_loss_workspace_bytes(B, channels, hw, 1, C.byref(size)) == 0
         most = max(plan(B, channels, hw, 1, 0, 1, u)[1] for u in (0, 8, 32, 256))
         assert size.value >= 256 + B * most * (16 + 4)
+
+
+def test_many_losses_leave_no_long_list_behind():
+    w = leaf()
+    kept = [eager_loss(w * k) for k in range(10)]
+    for k in range(1000):
+        eager_loss(w * k)
+    gc.collect()
+    assert len(finetune._on_default_stream.refs) <= 2 * 64 + 1 and all(n.grad_fn in list(finetune._on_default_stream) for n in kept)

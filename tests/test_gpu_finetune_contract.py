@@ -198,3 +198,21 @@ def test_workgroups_that_stop_waiting_leave_the_same_bits(op, polls, B, C, T):
     for g in got:
         for k in want:
             assert torch.equal(want[k], g[k]), k
+
+
+@pytest.mark.parametrize("op", ["pref", "policy"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_saved_tensors_that_a_hook_moves(op, dtype):
+    """Inputs packed to the host and back: handed-out gradients and computed ones are those without a hook."""
+    d = R.make(op, 6, 7, 131, dtype, device=DEV)
+    leaves = [d["model_out"].requires_grad_(), d["mixing_logit"].requires_grad_()]
+    loss_of = preference_loss if op == "pref" else policy_loss
+    up = torch.tensor(3.0, device=DEV)
+    loss = loss_of(**d).loss
+    want = [torch.autograd.grad(loss, leaves, up, retain_graph=True) for _ in range(2)]
+    with torch.autograd.graph.save_on_cpu():
+        loss = loss_of(**{k: t.clone() if k in ("x_t", "noise", "x_prev", "ref_out") else t for k, t in d.items()}).loss
+    junk = [torch.full_like(d["x_t"], math.nan) for _ in range(8)]      # what was freed is used again
+    for w in want:
+        assert all(map(torch.equal, torch.autograd.grad(loss, leaves, up, retain_graph=True), w))
+    del junk
