@@ -153,8 +153,9 @@ template <bool ROOT> __device__ __forceinline__ unsigned encode4(const float (&x
 }
 
 // One step of four values.  v: the second moment, or its root (8 bits).  The root is correctly rounded - r = x - s^2 is exact in an FMA, so
-// one correction of s = x rsq(x) is enough (checked on every fraction) - at half the instructions of sqrtf; the quotient by the hardware's
-// reciprocal is within 1.5 ulp, of a change that is a small part of the parameter.
+// one correction of s = x rsq(x) is enough (checked on every fraction) - at half the instructions of sqrtf.  The quotient is a division, as in
+// the step over one slab; with 8-bit moments, whose arithmetic is as long as the memory's time, it is m times the hardware's reciprocal, within
+// 1.5 ulp, of a change that the moments' 8 bits have made coarser by 2^18.
 template <int BITS>
 __device__ __forceinline__ void step4(const AdArgs& a, const AdTensor& t, float (&p)[4], const float (&g)[4], float (&m)[4], float (&v)[4],
                                       float (&root)[4]) {
@@ -173,7 +174,10 @@ __device__ __forceinline__ void step4(const AdArgs& a, const AdTensor& t, float 
     for (int i = 0; i < 4; ++i) root[i] = sqrtf(v[i]);
   }
 #pragma unroll
-  for (int i = 0; i < 4; ++i) p[i] = p[i] * t.decay - (m[i] * __builtin_amdgcn_rcpf(root[i] * t.inv_bc2 + a.eps)) * t.size;
+  for (int i = 0; i < 4; ++i) {
+    const float denom = root[i] * t.inv_bc2 + a.eps;
+    p[i] = p[i] * t.decay - (BITS == 32 ? m[i] / denom : m[i] * __builtin_amdgcn_rcpf(denom)) * t.size;
+  }
 }
 __device__ __forceinline__ void random4(unsigned key, int64_t blk, int lane, unsigned (&rnd)[4]) {
   const unsigned kb = mix32(key + (unsigned)blk * 0x9E3779B9u);

@@ -8,6 +8,7 @@ import torch
 import finetune_ref as R
 from ddmi_amd import _lib
 from ddmi_amd.finetune import policy_loss, preference_loss, transition_log_prob
+from ddmi_amd.optim import adamw_step
 from test_gpu_finetune import DEV, SHAPES, call, reference
 
 pytestmark = pytest.mark.gpu
@@ -216,3 +217,16 @@ def test_saved_tensors_that_a_hook_moves(op, dtype):
     for w in want:
         assert all(map(torch.equal, torch.autograd.grad(loss, leaves, up, retain_graph=True), w))
     del junk
+
+
+# ---- AdamW's quotient ----------------------------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("g_type", [torch.float32, torch.bfloat16])
+def test_adamw_divides(g_type):
+    """With betas of zero and no eps the change is lr g / |g|: the root of a rounded square is the number itself, and a number divided by itself
+    is one, so the parameters are lr exactly."""
+    n = 100003
+    g = torch.randn(n, generator=torch.Generator().manual_seed(3)).to(g_type).to(DEV)
+    g[g == 0] = 1.0
+    p, m, v = (torch.zeros(n, device=DEV) for _ in range(3))
+    adamw_step([p], [g], [m], [v], 1, lr=0.5, betas=(0.0, 0.0), eps=0.0)
+    assert torch.equal(p, -0.5 * g.float().sign())
