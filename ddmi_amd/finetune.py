@@ -19,6 +19,7 @@ are the caller's to drop.  A backward that is captured apart from its forward ne
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import functools
 import math
@@ -31,6 +32,7 @@ from torch.autograd.function import once_differentiable
 
 from . import _lib
 
+_HERE = contextlib.nullcontext()
 _OUT_TYPES = {torch.float32: _lib.DTYPE_F32, torch.bfloat16: _lib.DTYPE_BF16}
 
 
@@ -124,12 +126,11 @@ def _launch(entry, tensors, extra, args, stats, g, grads, mixed):
     results = [torch.empty((), dtype=torch.float32, device=dev)] + [torch.empty((n,), dtype=torch.float32, device=dev) for n in stats]
     ws = torch.empty(_workspace_bytes(B, Cc, HW, logit is not None), dtype=torch.uint8, device=dev)
     given = _lib.LossIn(*map(_p, tensors), HW, Cc, _OUT_TYPES[out.dtype])
-    at = list(map(_p, extra))
-    _lib.check(entry(C.byref(given), *args[0], *at, *args[1], _p(g), ws.data_ptr(), ws.numel(), *map(_p, results), _p(d_out), _p(d_logit),
-                     _lib.raw_stream(out.get_device())))
+    at, workspace, outputs = list(map(_p, extra)), (ws.data_ptr(), ws.numel()), (_p(d_out), _p(d_logit))
+    _lib.check(entry(C.byref(given), *args[0], *at, *args[1], _p(g), *workspace, *map(_p, results), *outputs, _lib.raw_stream(out.get_device())))
     again = None
     if grads and out.dtype != torch.float32:      # (the noise's rows are the preference loss's, the transition is the policy loss's)
-        again = (C.byref(given), B, tensors[3].shape[0], at[0] if at else None), (ws.data_ptr(), ws.numel()), ws
+        again = (C.byref(given), B, tensors[3].shape[0], at[0] if at else None), workspace, outputs, ws
     return results, (d_out, d_logit, again)
 
 
@@ -156,22 +157,22 @@ class LossFn(torch.autograd.Function):
 
     @staticmethod
     def _gradients(ctx, g):
-        if not g.is_contiguous():
-            g = g.contiguous()
-        with _lib.on_device(ctx.index):
-            stream = _lib.raw_stream(ctx.index)
-            capture = _lib.capture_id(stream)
-            if capture not in (0, ctx.capture):      # a backward alone is captured: of a graph that was not looked at when it was built
+        with _lib.on_device(ctx.index) if torch._C._cuda_getDevice() != ctx.index else _HERE:
+            stream = torch._C._cuda_getCurrentRawStream(ctx.index)
+            capture = _lib.capture_id(stream) if stream else 0
+            if capture and capture != ctx.capture:      # a backward alone is captured: of a graph that was not looked at when it was built
                 _check_graphs([n for n, _ in ctx.next_functions])
+            if not g.is_contiguous():
+                g = g.contiguous()
             if ctx.grads is not None and capture == ctx.capture:
                 (d_out, d_logit, again), ctx.grads = ctx.grads, None
-                if d_out.dtype == torch.float32:
+                if again is None:
                     _lib.check(_lib.lib().ddmi_train_loss_scale(g.data_ptr(), d_out.data_ptr(), _lib.DTYPE_F32, d_out.numel(), _p(d_logit),
                                                                 0 if d_logit is None else d_logit.numel(), stream))
                 else:
                     ctx.saved_tensors      # the inputs are read where the forward had them: raises where one was changed since
-                    inputs, workspace, _ = again
-                    _lib.check(_lib.lib().ddmi_train_loss_again(*inputs, g.data_ptr(), *workspace, d_out.data_ptr(), _p(d_logit), stream))
+                    inputs, workspace, outputs, _ = again
+                    _lib.check(_lib.lib().ddmi_train_loss_again(*inputs, g.data_ptr(), *workspace, *outputs, stream))
             else:
                 saved, (entry, (args, stats, mixed)) = ctx.saved_tensors, ctx.again
                 saved = tuple(ctx.beside.get(i, t) for i, t in enumerate(saved))
