@@ -2,6 +2,24 @@
 #pragma once
 #include "common.h"
 
+typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));            // rows of an odd plane, tensors of a slab start at any element
+typedef unsigned short u16x4u __attribute__((ext_vector_type(4), aligned(2)));
+typedef unsigned u32u __attribute__((aligned(1)));
+// NT: past the caches, for streams of which nothing is found there again.
+// (overloads, not a template: a deduced type would lose its alignment)
+#define FT_GET_PUT(V)                                                                                   \
+  template <bool NT> __device__ __forceinline__ V get(const V* p) {                                     \
+    if constexpr (NT) return __builtin_nontemporal_load(p);                                             \
+    else return *p;                                                                                     \
+  }                                                                                                     \
+  template <bool NT> __device__ __forceinline__ void put(V* p, V v) {                                   \
+    if constexpr (NT) __builtin_nontemporal_store(v, p);                                                \
+    else *p = v;                                                                                        \
+  }
+FT_GET_PUT(f32x4u)
+FT_GET_PUT(u16x4u)
+FT_GET_PUT(u32u)
+
 enum { FT_PREF = 0, FT_POLICY = 1 };
 #define FT_THREADS 256
 #define FT_VECS 16       // vectors of four residuals that a thread of the one-pass kernel keeps in registers

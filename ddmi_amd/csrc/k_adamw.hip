@@ -41,10 +41,8 @@ struct AdArgs {
 };
 static_assert(sizeof(AdArgs) <= 4096, "kernel arguments");
 
-typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
-typedef unsigned short u16x4u __attribute__((ext_vector_type(4), aligned(2)));
-typedef unsigned u32u __attribute__((aligned(1)));
-
+// the published finaliser of MurmurHash3 (two multiplications, three shifts); the odd constants it is fed with elsewhere are 2^32 / golden
+// ratio and multipliers of published integer hashes, any of which would do
 __host__ __device__ __forceinline__ unsigned mix32(unsigned x) {
   x ^= x >> 16;
   x *= 0x85EBCA6Bu;
@@ -53,21 +51,8 @@ __host__ __device__ __forceinline__ unsigned mix32(unsigned x) {
   return x ^ (x >> 16);
 }
 
-// NT: past the caches.  A step over more than the last-level cache leaves nothing there that the next reader finds, and the memory runs
+// A step over more than the last-level cache goes past the caches: it leaves nothing there that the next reader finds, and the memory runs
 // 9 % faster without it (519 M parameters: 2.79 -> 2.56 ms); a smaller step's parameters are the next forward's to find.
-// (overloads, not a template: a deduced type would lose its alignment)
-#define FT_GET_PUT(V)                                                                                   \
-  template <bool NT> __device__ __forceinline__ V get(const V* p) {                                     \
-    if constexpr (NT) return __builtin_nontemporal_load(p);                                             \
-    else return *p;                                                                                     \
-  }                                                                                                     \
-  template <bool NT> __device__ __forceinline__ void put(V* p, V v) {                                   \
-    if constexpr (NT) __builtin_nontemporal_store(v, p);                                                \
-    else *p = v;                                                                                        \
-  }
-FT_GET_PUT(f32x4u)
-FT_GET_PUT(u16x4u)
-FT_GET_PUT(u32u)
 // four values at `at`, of which `left` (1..4) exist
 template <bool NT> __device__ __forceinline__ void load(const float* base, int64_t at, int left, float (&v)[4]) {
   const float* p = base + at;

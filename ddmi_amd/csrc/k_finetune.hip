@@ -18,23 +18,8 @@
 #include "prof.h"
 
 namespace {
-typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));            // rows of an odd plane start at any element
-typedef unsigned short u16x4u __attribute__((ext_vector_type(4), aligned(2)));
-
-// NT: past the caches.  One pass over a large batch leaves nothing in them that anyone finds again, and the memory runs faster without
-// (256 pairs of 64 x 64 x 64: 508 -> 473 us; 16 pairs: 62 -> 53)
-// (overloads, not a template: a deduced type would lose its alignment)
-#define FT_GET_PUT(V)                                                                                   \
-  template <bool NT> __device__ __forceinline__ V get(const V* p) {                                     \
-    if constexpr (NT) return __builtin_nontemporal_load(p);                                             \
-    else return *p;                                                                                     \
-  }                                                                                                     \
-  template <bool NT> __device__ __forceinline__ void put(V* p, V v) {                                   \
-    if constexpr (NT) __builtin_nontemporal_store(v, p);                                                \
-    else *p = v;                                                                                        \
-  }
-FT_GET_PUT(f32x4u)
-FT_GET_PUT(u16x4u)
+// One pass over a large batch leaves nothing in the caches that anyone finds again, and the memory runs faster past them (256 pairs of
+// 64 x 64 x 64: 508 -> 473 us; 16 pairs: 62 -> 53)
 template <bool NT = false> __device__ __forceinline__ void load4(const float* p, float (&v)[4]) {
   const f32x4u t = get<NT>(reinterpret_cast<const f32x4u*>(p));
   v[0] = t.x; v[1] = t.y; v[2] = t.z; v[3] = t.w;
