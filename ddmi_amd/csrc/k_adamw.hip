@@ -227,7 +227,8 @@ __device__ __forceinline__ void finish_block(const AdArgs& a, const AdTensor& t,
 }
 
 // A wave takes AD_UNROLL blocks: all their loads are issued before the first is worked on.  A stream: 519 M parameters in 368 tensors, 28
-// bytes each with 32-bit moments 2.56 ms = 5.7 TB/s, 16 with 8-bit ones 1.44 ms = 5.8 TB/s (a plain copy reaches 5.5 here).  The 8-bit form
+// bytes each with 32-bit moments 2.57 ms = 5.7 TB/s, 16 with 8-bit ones 1.43 ms = 5.8 TB/s (a copy by the library's own kernel reaches 5.5 over
+// 4 GiB, 5.7 over 2 and 6.0 over 1); the memory counters see the bytes counted here to 2 %.  The 8-bit form
 // stays one as long as its arithmetic is short: with sqrtf, a true division, codes in integer steps and maxima through LDS - 133 vector
 // instructions a value - it took 1.90 ms.
 template <typename PT, typename GT, int BITS, bool NT>

@@ -365,9 +365,10 @@ template <typename T> __device__ __forceinline__ void store_some(T* p, int left,
 
 // NV vectors of four values a thread; a row's vectors lie on its G lanes in turn, `turns` to a lane.  Sixteen vectors of residuals (two
 // times eight with KL) leave room for four workgroups a compute unit, so that three load while one waits (256 pairs as a graph, 8 | 12 | 16 |
-// 20 | 24 vectors: 488 | 506 | 470 | 501 | 509 us; 512 transitions: 605 | 633 | 519 | 520 | 529).  256 pairs of 64 x 64 x 64: 453 us
-// for the 2.42 GB that any form has to move, 5.3 TB/s; 512 transitions with KL: 492 us, 5.5 TB/s.  What is left is the wait for the last of
-// a sample's spans; loading a vector ahead of its use costs more registers than it gains (2 % slower).
+// 20 | 24 vectors: 488 | 506 | 470 | 501 | 509 us; 512 transitions: 605 | 633 | 519 | 520 | 529).  256 pairs of 64 x 64 x 64: 452 us
+// for the 2.42 GB that any form has to move, 5.3 TB/s (the memory counters see 2.55: half of the noise that a pair shares is found in the
+// caches by its second sample); 512 transitions with KL: 473 us, 5.7 TB/s, 2.70 GB counted of 2.68.  What is left is the wait for the last
+// of a sample's spans; loading a vector ahead of its use costs more registers than it gains (2 % slower).
 template <int MODE, bool MIX, bool REF, typename T, int NV>
 __global__ void __launch_bounds__(FT_THREADS, 2) fused_kernel(FtArgs a) {
   constexpr bool TWO = MODE == FT_POLICY && REF;
@@ -666,10 +667,21 @@ int ft_plan(FtArgs* a, int B, int C, int64_t HW, bool mixed, int rows_of, int ke
     const int64_t turns = cdiv64(cdiv64(std::min(a->seg, a->T), 4), 1ll << a->log_g), groups = FT_THREADS >> a->log_g;
     a->rows_per_wg = (int)std::max<int64_t>(1, std::min<int64_t>(a->rows_per_wg, keep / std::max<int64_t>(turns, 1) * groups));
     const int64_t wps = cdiv64(a->C, a->rows_per_wg) * a->nseg;
-    // One pass pays from one and a half workgroups a compute unit on, 384 on the whole card's 256 (64 x 64 x 64 latents, two passes | one:
-    // 8 pairs 40 | 48 us, 12: 52 | 50, 16: 65 | 53, 256: 680 | 477; transitions with KL 8: 33 | 39, 12: 43 | 41, 512: 894 | 533).  The spans that
-    // wait for each other are at most as many as the compute units, each of which holds two: they are resident together with room to spare.  The
-    // units are those of the card as it is partitioned.  And the threads' registers are mostly in use.
+    // One pass pays from one and a half workgroups a compute unit on, 384 on the whole card's 256 (64 x 64 x 64 latents as graphs, us, two
+    // passes | one; 16 workgroups a sample, with KL 32):
+    //   samples                 8          12          16          24          32          48         256
+    //   preference fp32     30.3|42.9   36.0|44.1   40.9|44.3   49.0|47.1   57.9|51.0   76.3|60.0   407|257
+    //   preference bf16     28.0|42.8   34.2|43.6   36.5|43.7   44.7|46.2   48.9|47.0   64.0|51.1   319|201
+    //   no mixing fp32      26.1|38.0   29.2|38.4   33.1|39.4   40.8|41.4   45.5|43.5   60.5|50.9   312|208
+    //   no mixing bf16      21.6|37.1   26.0|37.5   29.1|38.0   33.3|40.1   37.6|40.9   46.9|43.6   220|151
+    //   policy KL fp32      32.2|32.9   39.8|35.1   42.5|36.6   55.0|41.1   63.6|47.5   82.7|65.4   446|259
+    //   policy KL bf16      29.7|33.5   35.9|35.1   36.8|35.8   46.1|38.5   51.6|42.3   68.2|58.7   340|221
+    //   policy fp32         29.4|39.4   34.9|40.8   37.3|41.7   46.5|43.5   54.2|45.3   68.8|52.6   353|211
+    //   policy bf16         27.8|40.0   33.1|40.7   33.9|41.0   41.5|43.1   46.8|43.8   59.2|46.7   288|175
+    // One rule for all of them: it is early for bf16 without mixing, whose second reading is the cheapest, by up to 7 us between 384 and 640
+    // workgroups, and by 2 us for bf16 with mixing up to 450.  The spans that wait for each other are at most as many as the compute units,
+    // each of which holds two: they are resident together with room to spare.  The units are those of the card as it is partitioned.  And the
+    // threads' registers are mostly in use.
     const double filled = (double)a->rows_per_wg * (double)std::min(a->seg, a->T) / (1024.0 * keep);
     const bool room = units == FT_ANY_CARD || (units > 0 && 2 * wps * B >= 3 * (int64_t)units && wps * rows_of <= units);
     a->fused = room && turns <= keep && filled >= 0.5;

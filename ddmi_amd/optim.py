@@ -164,7 +164,11 @@ class AdamW:
     """The optimizer over parameters or parameter groups ({"params": [...], "lr": ..., "weight_decay": ...}), as torch.optim.AdamW is made;
     a parameter whose `.grad` is None sits the step out, its step count too.  `param_groups[i]["lr"]` and `["weight_decay"]` are read at every
     step.  state_bits: 32 or 8.  The moments of all parameters lie in one
-    slab each, a parameter's from a multiple of 256 values on."""
+    slab each, a parameter's from a multiple of 256 values on.
+
+    It is not a torch.optim.Optimizer: a torch scheduler does not take it (set the groups' lr), betas and eps are those of all groups, zero_grad
+    clears the gradients in place unless told otherwise, and bf16 parameters are rounded stochastically with either kind of moments.  The seed
+    of the rounding is an argument and no part of the state: a resumed run gives the same bits with the same seed."""
 
     def __init__(self, params, lr: float = 1e-4, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 0.0, state_bits: int = 32, seed: int = 0):
         if state_bits not in (32, 8):

@@ -528,14 +528,15 @@ int ddmi_train_loss_workspace_bytes(int B, int C, int64_t HW, int mixed, size_t*
 /* Preference loss over `pairs` pairs: samples [0, pairs) preferred, [pairs, 2 pairs) rejected (B = 2 pairs).  e = mean((eps - noise)^2),
  * margin = -beta / 2 ((e - e_ref) of the preferred - that of the rejected), loss = weighted mean of
  * -(1 - label_smoothing) log sigma(margin) - label_smoothing log sigma(-margin).  noise_rows: 2 pairs, or pairs when both samples of a
- * pair got the same noise.  margin [pairs], mse [2 pairs] = e; 0 for pairs left out. */
+ * pair got the same noise.  margin [pairs], mse [2 pairs] = e; 0 for pairs left out.
+ * beta is finite, as is the policy loss's kl_coef: an infinite one times the zero of a row left out is a NaN. */
 int ddmi_train_pref_loss(const ddmi_loss_in* in, int pairs, int noise_rows, double beta, double label_smoothing, const float* dloss, void* ws,
                          size_t ws_bytes, float* loss, float* margin, float* mse, void* d_model_out, float* d_logit, void* stream);
 /* Clipped policy loss over B denoising transitions x_t -> second: mean mu = A x_t + E eps and deviation s with transition[b] = (A, E, s);
  * logp = mean over the values of log N(second; mu, s^2), ratio = exp(logp - logp_old), kl = mean((mu - mu_ref)^2) / (2 s^2), loss =
  * weighted mean of max(-advantage ratio, -advantage clip(ratio, 1 -+ clip_range)) + kl_coef kl.  A transition with s = 0 has no density
- * and is left out like one of weight 0; a negative or NaN deviation shows as NaN in logp and loss.  logp_old = NULL: logp alone is computed (a rollout records it), the other outputs are not
- * touched.  logp, ratio, kl [B]; 0 for transitions left out. */
+ * and is left out like one of weight 0; a negative or NaN deviation shows as NaN in logp and loss.  logp_old = NULL: logp alone is computed
+ * (a rollout records it), the other outputs are not touched.  logp, ratio, kl [B]; 0 for transitions left out. */
 int ddmi_train_policy_loss(const ddmi_loss_in* in, int B, const float* transition, const float* logp_old, const float* advantage, double clip_range,
                            double kl_coef, const float* dloss, void* ws, size_t ws_bytes, float* loss, float* logp, float* ratio, float* kl,
                            void* d_model_out, float* d_logit, void* stream);
