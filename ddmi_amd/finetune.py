@@ -241,13 +241,24 @@ def _accumulation_nodes(starts):
     return found
 
 
-def _check_graphs(nodes):
-    """Refuses a capture of the graph behind `nodes` that meets one of a living loss on the default stream."""
+def _meets_default_stream(nodes) -> bool:
+    """Whether the graph behind `nodes` meets one of a living loss on the default stream."""
     losses = list(_on_default_stream)
-    if losses:
-        old = {k: n for k, n in _accumulation_nodes(losses).items() if n.metadata.get(_FIRST_STREAM, _DEFAULT) == _DEFAULT}
-        if old.keys() & _accumulation_nodes(nodes).keys():
-            raise RuntimeError(_REFUSED)
+    if not losses:
+        return False
+    old = {k: n for k, n in _accumulation_nodes(losses).items() if n.metadata.get(_FIRST_STREAM, _DEFAULT) == _DEFAULT}
+    return bool(old.keys() & _accumulation_nodes(nodes).keys())
+
+
+def _check_graphs(nodes):
+    if _meets_default_stream(nodes):
+        nodes.clear()      # the error's traceback keeps none of them alive
+        raise RuntimeError(_REFUSED)
+
+
+def may_be_captured(leaves) -> bool:
+    """Whether a backward that ends in these leaves may be captured now: not while an eager loss on the default stream reaches one of them."""
+    return not _meets_default_stream([torch.autograd.graph.get_gradient_edge(t).node for t in leaves if t.requires_grad])
 
 
 def _loss(entry, model_out, mixing_logit, others, extra, args, stats):

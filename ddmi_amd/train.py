@@ -25,7 +25,7 @@ import torch.nn.functional as F
 
 from . import _lib
 from .ddpm import make_beta_schedule
-from .finetune import policy_loss, preference_loss, transition_log_prob
+from .finetune import may_be_captured, policy_loss, preference_loss, transition_log_prob
 from .optim import AdamW
 
 
@@ -1103,6 +1103,8 @@ class LDMTrainStep:
             self._graphs[key] = "warm"
             return self._micro_body(z0, t, noise)
         if g == "warm":
+            if not may_be_captured(self.flat.params):     # an eager fine-tuning loss of the caller's lives on them: later, then
+                return self._micro_body(z0, t, noise)
             bufs = (torch.empty_like(z0), torch.empty_like(t), torch.empty_like(noise))
             for dst, src in zip(bufs, (z0, t, noise)):
                 dst.copy_(src)

@@ -11,7 +11,7 @@ import torch.utils.checkpoint
 from torch.autograd import forward_ad
 
 import finetune_ref as R
-from ddmi_amd import _lib, finetune
+from ddmi_amd import _lib, finetune, train
 from ddmi_amd.finetune import policy_loss, preference_loss, transition_log_prob
 from ddmi_amd.optim import _ENTRY, AdamW, adamw_step
 from ddmi_amd.train import FlatParams, LDMTrainStep
@@ -341,6 +341,17 @@ def test_a_leaf_that_the_default_stream_saw_first_stays_refused_while_its_node_l
     captured(w)
 
 
+def test_a_refusal_that_is_kept_keeps_no_node():
+    w = leaf()
+    loss = eager_loss(w * 2)
+    with pytest.raises(RuntimeError) as kept:
+        finetune._check_graphs([torch.autograd.graph.get_gradient_edge(w).node])
+    torch.autograd.graph.get_gradient_edge(w).node.metadata["alive"] = True
+    del loss
+    gc.collect()
+    assert not torch.autograd.graph.get_gradient_edge(w).node.metadata and "captured while" in str(kept.value)
+
+
 def test_losses_on_the_default_stream_are_not_kept_alive():
     before = len(finetune._on_default_stream)
     w = leaf()
@@ -403,3 +414,21 @@ def test_many_losses_leave_no_long_list_behind():
         eager_loss(w * k)
     gc.collect()
     assert len(finetune._on_default_stream.refs) <= 2 * 64 + 1 and all(n.grad_fn in list(finetune._on_default_stream) for n in kept)
+
+
+def test_a_training_step_asks_before_it_captures(monkeypatch):
+    """With an eager loss of the caller's alive on its parameters, a step that would record its graph runs as it is, and records later."""
+    p, q = leaf(), leaf()
+    assert finetune.may_be_captured([p, q])
+    loss = eager_loss(p.exp())
+    assert not finetune.may_be_captured([q, p]) and finetune.may_be_captured([q, p.detach()])
+    monkeypatch.setattr(train._lib, "check", lambda rc: None)
+    monkeypatch.setattr(train._lib, "lib", lambda: types.SimpleNamespace(ddmi_train_arena_generation=lambda *a: 0))
+    monkeypatch.setattr(torch.cuda, "CUDAGraph", lambda: pytest.fail("a capture was begun"))
+    z = torch.zeros(2, 3)
+    host = types.SimpleNamespace(model=types.SimpleNamespace(tc=types.SimpleNamespace(h=0)), _graph_generation=0, _graphs={(2, 3): "warm"},
+                                 flat=types.SimpleNamespace(params=[p, q]), _micro_body=lambda *a: "eager")
+    assert LDMTrainStep._graphed_micro(host, z, z, z) == "eager" and host._graphs == {(2, 3): "warm"}
+    del loss
+    gc.collect()
+    assert finetune.may_be_captured([p, q])

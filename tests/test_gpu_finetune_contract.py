@@ -10,6 +10,7 @@ from ddmi_amd import _lib
 from ddmi_amd.finetune import policy_loss, preference_loss, transition_log_prob
 from ddmi_amd.optim import adamw_step
 from test_gpu_finetune import DEV, SHAPES, call, reference
+from test_gpu_finetune_step import pairs, trainer
 
 pytestmark = pytest.mark.gpu
 # two passes; one pass
@@ -230,3 +231,31 @@ def test_adamw_divides(g_type):
     p, m, v = (torch.zeros(n, device=DEV) for _ in range(3))
     adamw_step([p], [g], [m], [v], 1, lr=0.5, betas=(0.0, 0.0), eps=0.0)
     assert torch.equal(p, -0.5 * g.float().sign())
+
+
+def test_a_graphed_training_step_beside_a_living_loss():
+    """use_graph records on the second step of a shape; while the caller holds an eager loss on the parameters it runs eagerly instead, with
+    the same numbers, and records once the loss is gone."""
+    def eager_loss(tr, z, noise, t):
+        x = torch.cat([z, z])
+        out = tr.model(x, torch.cat([t, t]))
+        return preference_loss(out, out.detach(), x, noise, torch.full((6,), 0.5, device=DEV), 1.0)
+
+    nodes = lambda tr: [torch.autograd.graph.get_gradient_edge(p).node for p in tr.flat.params]      # noqa: E731
+    runs = []
+    for hold in (False, True):
+        tr = trainer(use_graph=True).set_reference()
+        held = []
+        for k in range(4):
+            zw, _, noise, t = (v.to(DEV) for v in pairs(seed=k))
+            if hold and k == 1:
+                held.append(eager_loss(tr, zw, noise, t))
+                assert not any(n.metadata.update(held=True) for n in nodes(tr))
+            if k == 3:
+                held.clear()
+                gc.collect()
+                assert not any(n.metadata for n in nodes(tr))           # nothing of it is left before anything is recorded
+            tr.train_step(zw, t, noise)
+            assert isinstance(tr._graphs[tuple(zw.shape)], tuple) == (k >= (3 if hold else 1))
+        runs.append(tr.flat.data.clone())
+    assert torch.equal(*runs)
