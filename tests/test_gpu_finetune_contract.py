@@ -259,3 +259,51 @@ def test_a_graphed_training_step_beside_a_living_loss():
             assert isinstance(tr._graphs[tuple(zw.shape)], tuple) == (k >= (3 if hold else 1))
         runs.append(tr.flat.data.clone())
     assert torch.equal(*runs)
+
+
+@pytest.mark.parametrize("op", ["pref", "policy"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("which", ["output", "logit"])
+@pytest.mark.parametrize("B,C,T", BOTH)
+def test_gradients_of_one_leaf_alone(op, dtype, which, B, C, T):
+    """The output's without the logit's and the other way round, for an upstream gradient that is not 1: what both together give."""
+    d = R.make(op, B, C, T, dtype, seed=11, device=DEV)
+    loss_of = preference_loss if op == "pref" else policy_loss
+    up = torch.tensor(-1.7, device=DEV)
+    names = ["model_out", "mixing_logit"]
+    both = {n: d[n].clone().requires_grad_() for n in names}
+    want = dict(zip(names, torch.autograd.grad(loss_of(**dict(d, **both)).loss, both.values(), up)))
+    name = names[which == "logit"]
+    w, bound = (t.to(DEV).reshape(d[name].shape) for t in reference(op, d)["d_logit" if which == "logit" else "d_model_out"])
+    w, scale = w * up.double(), float(up.double().abs())
+    one = d[name].clone().requires_grad_()
+    loss = loss_of(**dict(d, **{name: one})).loss
+    assert torch.equal(torch.autograd.grad(loss, one, up, retain_graph=True)[0], want[name])
+    again = torch.autograd.grad(loss, one, up)[0]
+    # Computed anew, an fp32 gradient is not the multiplied one to the last bits, and where the residual's and the KL term's parts cancel a
+    # rounding of a part is many of their sum (k up rounded before the sum, against the sum times up): both are within the formula's bound,
+    # which counts the parts' roundings, and two more of the value's.
+    assert ((again.double() - w).abs() <= bound * scale + 2.02 * R.U * (w.abs() + bound * scale) + 2.0 ** -133).all()
+    if dtype == torch.bfloat16:
+        assert torch.equal(again, want[name])
+
+
+@pytest.mark.parametrize("op", ["pref", "policy"])
+def test_upstream_gradients_of_more_than_2_to_31_values(op):
+    """bf16 gradients computed again behind offsets of 2^31: times four is exact, so they are four times the handed-out ones."""
+    C, T, B = 64, 65536, 514
+    small = R.make(op, 2 if op == "pref" else 1, C, T, torch.bfloat16, seed=3, device=DEV)
+    d = {}
+    for k, t in small.items():
+        if not isinstance(t, torch.Tensor) or "logit" in k:
+            d[k] = t
+        elif op == "pref":
+            d[k] = torch.cat([h.expand((B // 2,) + h.shape[1:]) for h in t.split(1)]).contiguous()
+        else:
+            d[k] = t.expand((B,) + t.shape[1:]).contiguous()
+    d["model_out"].requires_grad_()
+    loss_of = preference_loss if op == "pref" else policy_loss
+    one = torch.autograd.grad(loss_of(**d).loss, d["model_out"], torch.ones((), device=DEV))[0]
+    four = torch.autograd.grad(loss_of(**d).loss, d["model_out"], torch.full((), 4.0, device=DEV))[0]
+    normal = one.abs() >= 2.0 ** -126
+    assert torch.equal(torch.where(normal, one * 4, one), torch.where(normal, four, one)) and bool(normal[[0, -1]].any())
